@@ -33,7 +33,7 @@ enum vla_error {
 };
 
 enum vla_model_kind { VLA_PI0 = 0, VLA_PI05 = 1 };
-enum vla_dtype { VLA_BF16 = 0, VLA_F32 = 1 };
+enum vla_dtype { VLA_BF16 = 0, VLA_F32 = 1, VLA_F16 = 2 /* operators below only */ };
 
 /* Mirrors the constructor arguments: Pi0Inference(checkpoint, num_views, chunk_size) (pi0_infer.py:1239),
  * Pi05Inference(checkpoint, num_views, chunk_size, ..., max_prompt_len) (pi05_infer.py:531-561).
@@ -274,6 +274,82 @@ int vla_op_gemm_noalloc_status(int* out);
 
 /* y bf16 [rows,D] = norm(x fp32 [rows,D]); mode 0 LayerNorm (w,b), 1 RMS, 2 adaRMS (w = style[3*D]); D 1024|1152|2048. */
 int vla_op_norm(const float* x, void* y, int rows, int D, int mode, const float* w, const float* b, void* stream);
+
+/* ---- a key/value cache in pages, held in 8 bits ---------------------------------------------------------
+ * Sequences of different lengths share one cache of `num_blocks` pages of `block_size` tokens.  Pages are held as e4m3
+ * codes, k_codes / v_codes [num_blocks][kv_heads][block_size][head_dim], with one fp32 scale for each page and head,
+ * k_scale / v_scale [num_blocks][kv_heads]; a value is code * scale.  block_table [n_seqs][width] (row stride
+ * table_stride, int32) names each sequence's pages in order.  A step of a serving loop is: vla_op_block_plan (pages and slots for
+ * the new tokens), vla_op_cache_append (their keys and values), then vla_op_prompt_attention (new prompts among
+ * themselves) or vla_op_paged_attention (the newest tokens over the whole cache).
+ *
+ * These calls only enqueue work on `stream` (asynchronous, no allocation, nothing kept from one call to the next), on the
+ * current device, which must be the one the pointers belong to; they may be captured into a graph and issued from several
+ * threads and streams.  All pointers are device pointers; strides count elements; the head dim is contiguous.  They have
+ * no counterpart in the reference, whose cache is one dense bf16 array (pi0_infer.py:1276-1277). */
+
+/* Block table and slot map from the lengths, all on the device.  Request b holds context_lens[b] tokens and gets
+ * new_lens[b]; it takes ceil((context + new) / bs) - ceil(context / bs) blocks off free_blocks[n_free], from index
+ * *first_free on (null: 0), in request order, and their ids go into its table row behind the ones it has.
+ *   slots[total_new]      block id * bs + offset of each new token, packed in request order; -1 where the free list or the
+ *                         table had no block left, and in rows behind the last token
+ *   positions[total_new]  position of each new token in its sequence (0 in rows behind the last token)
+ *   cu_new[n_seqs + 1]    first row of each request; rows beyond total_new are dropped
+ *   seq_lens[n_seqs]      tokens of each request that have a slot
+ *   counts[3]             first free index after the call, blocks that were missing, sum of new_lens
+ * Lengths below zero count as zero.  n_seqs <= 8192.  slots and positions start on 16 bytes. */
+typedef struct vla_block_plan_desc {
+  const int32_t* context_lens; const int32_t* new_lens; int n_seqs;
+  int32_t* block_table; int width; long long table_stride;
+  const int32_t* free_blocks; int n_free; const int32_t* first_free;
+  int block_size; int total_new;
+  int32_t* slots; int32_t* positions; int32_t* cu_new; int32_t* seq_lens; int32_t* counts;
+} vla_block_plan_desc;
+int vla_op_block_plan(const vla_block_plan_desc* d, void* stream);
+
+/* Writes tokens into the cache: token t (bf16 or f16 rows of k and v, [tokens][kv_heads][head_dim] by strides) goes to
+ * slots[t]; a slot outside [0, num_blocks * block_size) is skipped.  For each block, head and K / V the scale needed is the smallest power
+ * of two >= 2^-60 that brings the largest finite magnitude of the call's tokens to 448 or less.  A block whose first
+ * slot is written starts anew with that scale; any other block keeps the larger of its scale and that one, and where
+ * the scale grows all its codes are rounded again.  Codes are x / scale, nearest even, saturating; NaN stays NaN.
+ * The tokens of one block must be consecutive rows of the call (as vla_op_block_plan lays them out); of two consecutive tokens
+ * with the same slot the later one is kept.  head_dim 64 | 128 | 256, block_size a multiple of 16 up to 256. */
+typedef struct vla_cache_append_desc {
+  const void* k; const void* v; const int32_t* slots; int tokens;
+  long long k_tok_stride, k_head_stride, v_tok_stride, v_head_stride;
+  void* k_codes; void* v_codes; float* k_scale; float* v_scale;
+  int num_blocks, kv_heads, block_size, head_dim; int dtype;
+} vla_cache_append_desc;
+int vla_op_cache_append(const vla_cache_append_desc* d, void* stream);
+
+/* O = softmax(scale Q K^T) V of the last n_q tokens of every sequence over the cache: q, o [n_seqs][n_q][heads][head_dim] by
+ * strides; query i of sequence b is token seq_lens[b] - n_q + i and sees itself and what is before it (a row before the
+ * sequence's start is zero).  Page ids outside the cache are not seen; seq_lens is cut to width * block_size.
+ * heads is a multiple of kv_heads (consecutive query heads share a key/value head); head_dim 64 | 128 | 256. */
+typedef struct vla_paged_attn_desc {
+  const void* q; void* o;
+  long long q_seq_stride, q_tok_stride, q_head_stride, o_seq_stride, o_tok_stride, o_head_stride;
+  const void* k_codes; const void* v_codes; const float* k_scale; const float* v_scale;
+  const int32_t* block_table; long long table_stride; const int32_t* seq_lens;
+  int n_seqs, n_q, heads, kv_heads, head_dim;
+  int num_blocks, block_size, width;
+  float scale; int dtype;
+} vla_paged_attn_desc;
+int vla_op_paged_attention(const vla_paged_attn_desc* d, void* stream);
+
+/* O = softmax(scale Q K^T) V over packed prompts: q, o [tokens_q][heads][head_dim], k, v [tokens_k][kv_heads][head_dim] by
+ * strides; sequence b owns rows cu_q[b] .. cu_q[b + 1] and cu_k[b] .. cu_k[b + 1] (device memory, ascending).  With causal set, the
+ * last query of a sequence sees all its keys, the one before it all but the last, and so on; a row that sees nothing is
+ * zero.  Rows of o behind the last sequence are left as they were.  head_dim a multiple of 8 up to 256,
+ * heads / kv_heads <= 128. */
+typedef struct vla_prompt_attn_desc {
+  const void* q; const void* k; const void* v; void* o;
+  const int32_t* cu_q; const int32_t* cu_k;
+  int n_seqs, tokens_q, tokens_k, heads, kv_heads, head_dim;
+  long long q_tok_stride, q_head_stride, k_tok_stride, k_head_stride, v_tok_stride, v_head_stride, o_tok_stride, o_head_stride;
+  int causal; float scale; int dtype;
+} vla_prompt_attn_desc;
+int vla_op_prompt_attention(const vla_prompt_attn_desc* d, void* stream);
 
 #ifdef __cplusplus
 }

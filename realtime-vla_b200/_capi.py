@@ -7,7 +7,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libvla_b200.so")
 
 VLA_PI0, VLA_PI05 = 0, 1
-VLA_BF16, VLA_F32 = 0, 1
+VLA_BF16, VLA_F32, VLA_F16 = 0, 1, 2
 ERRORS = {1: "CUDA", 2: "KEY", 3: "SHAPE", 4: "STATE", 5: "LIMIT", 6: "DEVICE"}
 
 
@@ -52,6 +52,26 @@ class GemmNoAllocDesc(C.Structure):
                 ("bias", C.c_void_p), ("out_bf16", C.c_void_p), ("split", C.c_int)]
 
 
+def _desc(name, *fields):
+    """Structure from (type, "names in order") pairs."""
+    return type(name, (C.Structure,), {"_fields_": [(n, t) for t, names in fields for n in names.split()]})
+
+
+_P, _I, _L = C.c_void_p, C.c_int, C.c_longlong
+BlockPlanDesc = _desc("BlockPlanDesc", (_P, "context_lens new_lens"), (_I, "n_seqs"), (_P, "block_table"), (_I, "width"),
+                      (_L, "table_stride"), (_P, "free_blocks"), (_I, "n_free"), (_P, "first_free"), (_I, "block_size total_new"),
+                      (_P, "slots positions cu_new seq_lens counts"))
+CacheAppendDesc = _desc("CacheAppendDesc", (_P, "k v slots"), (_I, "tokens"),
+                        (_L, "k_tok_stride k_head_stride v_tok_stride v_head_stride"), (_P, "k_codes v_codes k_scale v_scale"),
+                        (_I, "num_blocks kv_heads block_size head_dim dtype"))
+PagedAttnDesc = _desc("PagedAttnDesc", (_P, "q o"),
+                      (_L, "q_seq_stride q_tok_stride q_head_stride o_seq_stride o_tok_stride o_head_stride"),
+                      (_P, "k_codes v_codes k_scale v_scale block_table"), (_L, "table_stride"), (_P, "seq_lens"),
+                      (_I, "n_seqs n_q heads kv_heads head_dim num_blocks block_size width"), (C.c_float, "scale"), (_I, "dtype"))
+PromptAttnDesc = _desc("PromptAttnDesc", (_P, "q k v o cu_q cu_k"), (_I, "n_seqs tokens_q tokens_k heads kv_heads head_dim"),
+                       (_L, "q_tok_stride q_head_stride k_tok_stride k_head_stride v_tok_stride v_head_stride o_tok_stride o_head_stride"),
+                       (_I, "causal"), (C.c_float, "scale"), (_I, "dtype"))
+
 EXPORTS = {
     "vla_create": (C.c_int, [C.POINTER(VlaConfig), C.POINTER(C.c_void_p)]),
     "vla_load_weight": (C.c_int, [C.c_void_p, C.c_char_p, C.c_void_p, C.POINTER(C.c_int64), C.c_int, C.c_int]),
@@ -86,6 +106,10 @@ EXPORTS = {
     "vla_expert_timeline": (C.c_int, [C.c_void_p, C.POINTER(C.c_ulonglong), C.c_int, C.POINTER(C.c_int)]),
     "vla_op_attention": (C.c_int, [C.POINTER(AttnDesc), C.c_void_p]),
     "vla_op_attention_tc": (C.c_int, [C.POINTER(AttnTcDesc), C.c_void_p]),
+    "vla_op_block_plan": (C.c_int, [C.POINTER(BlockPlanDesc), C.c_void_p]),
+    "vla_op_cache_append": (C.c_int, [C.POINTER(CacheAppendDesc), C.c_void_p]),
+    "vla_op_paged_attention": (C.c_int, [C.POINTER(PagedAttnDesc), C.c_void_p]),
+    "vla_op_prompt_attention": (C.c_int, [C.POINTER(PromptAttnDesc), C.c_void_p]),
     "vla_op_norm": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p]),
 }
 

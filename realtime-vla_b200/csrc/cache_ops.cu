@@ -1,0 +1,187 @@
+// C entry points of the operators around a key/value cache in pages (include/vla_b200.h): argument checks, launches.
+// All of them only enqueue work on the caller's stream: no allocation, no synchronisation, nothing kept between calls, so
+// they can be captured into a graph and called from several threads and streams at once.
+#include <algorithm>
+#include <cstdarg>
+#include <cstdio>
+
+#include "../../include/vla_b200.h"
+#include "attention_paged.cuh"
+#include "attention_prompt.cuh"
+#include "cache_pages.cuh"
+#include "host.cuh"
+
+namespace {
+
+int refuse(int code, const char* fmt, ...) {
+  char buf[320];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof buf, fmt, ap);
+  va_end(ap);
+  try {
+    g_last_error = buf;
+  } catch (...) {   // no memory for the message: the code still says what happened
+  }
+  return code;
+}
+
+int launched(const char* who, cudaError_t e) {
+  return e == cudaSuccess ? VLA_OK : refuse(VLA_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
+}
+
+// No C++ exception leaves a C entry point.
+template <typename F>
+int guarded(const char* who, F f) {
+  try {
+    return f();
+  } catch (...) {
+    return refuse(VLA_ERR_STATE, "%s: out of host memory", who);
+  }
+}
+
+int sm_count() {
+  int dev = 0, n = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  return n;
+}
+
+bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+
+// 16-byte rows: base and strides of a 16-bit tensor that is read in vectors of eight
+bool vectors(const void* p, long long a, long long b) { return aligned(p, 16) && a % 8 == 0 && b % 8 == 0; }
+
+constexpr long long INT_TOP = 0x7fffffff;
+
+}  // namespace
+
+extern "C" {
+
+int vla_op_block_plan(const vla_block_plan_desc* d, void* stream) {
+  const char* who = "vla_op_block_plan";
+  return guarded(who, [&]() -> int {
+    if (!d) return refuse(VLA_ERR_STATE, "%s: null descriptor", who);
+    if (d->n_seqs < 0 || d->n_seqs > PLAN_MAX_SEQS) return refuse(VLA_ERR_LIMIT, "%s: %d requests, at most %d are served", who, d->n_seqs, PLAN_MAX_SEQS);
+    if (d->block_size < 1 || d->width < 0 || d->n_free < 0 || d->total_new < 0 || d->table_stride < d->width)
+      return refuse(VLA_ERR_SHAPE, "%s: negative size, or a table stride below its width", who);
+    if (!d->cu_new || !d->counts) return refuse(VLA_ERR_STATE, "%s: null output", who);
+    if (d->n_seqs && (!d->context_lens || !d->new_lens || !d->seq_lens)) return refuse(VLA_ERR_STATE, "%s: null lengths", who);
+    if (d->n_seqs && d->width && !d->block_table) return refuse(VLA_ERR_STATE, "%s: null block table", who);
+    if (d->n_free && !d->free_blocks) return refuse(VLA_ERR_STATE, "%s: null free list", who);
+    if (d->total_new && (!d->slots || !d->positions)) return refuse(VLA_ERR_STATE, "%s: null slots or positions", who);
+    if (!aligned(d->slots, 16) || !aligned(d->positions, 16)) return refuse(VLA_ERR_SHAPE, "%s: slots and positions must start on 16 bytes", who);
+    PlanParams p;
+    p.ctx = d->context_lens; p.n_new = d->new_lens; p.n_seqs = d->n_seqs;
+    p.table = d->block_table; p.width = d->width; p.table_ld = d->table_stride;
+    p.free_ids = d->free_blocks; p.n_free = d->n_free; p.first = d->first_free;
+    p.block = d->block_size; p.total = d->total_new;
+    p.slots = d->slots; p.positions = d->positions; p.cu_new = d->cu_new; p.seq_lens = d->seq_lens; p.counts = d->counts;
+    const size_t smem = (size_t)(2 * d->n_seqs + 2) * sizeof(int);
+    if (smem > 40 * 1024)
+      if (cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(block_plan_kernel), (2 * PLAN_MAX_SEQS + 2) * (int)sizeof(int)); e != cudaSuccess)
+        return launched(who, e);
+    const long long rows = std::max<long long>(((long long)d->total_new + 3) / 4, d->n_seqs);
+    const int ctas = (int)std::min<long long>(std::max<long long>(1, (rows + PLAN_THREADS - 1) / PLAN_THREADS), 2 * sm_count());
+    return launched(who, launch_ex(block_plan_kernel, dim3(ctas), dim3(PLAN_THREADS), smem, reinterpret_cast<cudaStream_t>(stream), 1, false, p));
+  });
+}
+
+int vla_op_cache_append(const vla_cache_append_desc* d, void* stream) {
+  const char* who = "vla_op_cache_append";
+  return guarded(who, [&]() -> int {
+    if (!d) return refuse(VLA_ERR_STATE, "%s: null descriptor", who);
+    if (d->tokens < 0 || d->kv_heads < 1 || d->num_blocks < 1) return refuse(VLA_ERR_SHAPE, "%s: bad sizes", who);
+    if (d->head_dim != 64 && d->head_dim != 128 && d->head_dim != 256) return refuse(VLA_ERR_SHAPE, "%s: head_dim must be 64, 128 or 256", who);
+    if (d->block_size < 16 || d->block_size % 16 || d->block_size > 256) return refuse(VLA_ERR_SHAPE, "%s: block_size must be a multiple of 16 up to 256", who);
+    if ((long long)d->num_blocks * d->block_size > INT_TOP) return refuse(VLA_ERR_LIMIT, "%s: more than 2^31 - 1 slots", who);
+    if (d->dtype != VLA_BF16 && d->dtype != VLA_F16) return refuse(VLA_ERR_SHAPE, "%s: keys and values must be bf16 or f16", who);
+    if (!d->k_codes || !d->v_codes || !d->k_scale || !d->v_scale) return refuse(VLA_ERR_STATE, "%s: null cache", who);
+    if (!aligned(d->k_codes, 16) || !aligned(d->v_codes, 16)) return refuse(VLA_ERR_SHAPE, "%s: the cache must start on 16 bytes", who);
+    if (d->tokens == 0) return VLA_OK;
+    if (!d->k || !d->v || !d->slots) return refuse(VLA_ERR_STATE, "%s: null keys, values or slots", who);
+    if (!vectors(d->k, d->k_tok_stride, d->k_head_stride) || !vectors(d->v, d->v_tok_stride, d->v_head_stride))
+      return refuse(VLA_ERR_SHAPE, "%s: rows of k and v must start on 16 bytes", who);
+    AppendParams p;
+    p.x[0] = d->k; p.x[1] = d->v;
+    p.x_tok[0] = d->k_tok_stride; p.x_tok[1] = d->v_tok_stride; p.x_head[0] = d->k_head_stride; p.x_head[1] = d->v_head_stride;
+    p.codes[0] = reinterpret_cast<uint8_t*>(d->k_codes); p.codes[1] = reinterpret_cast<uint8_t*>(d->v_codes);
+    p.scale[0] = d->k_scale; p.scale[1] = d->v_scale;
+    p.slots = d->slots; p.tokens = d->tokens; p.kv_heads = d->kv_heads; p.block = d->block_size;
+    p.n_slots = (long long)d->num_blocks * d->block_size;
+    p.window = d->tokens <= 4096 ? 1 : 16;
+    const dim3 grid((d->tokens + p.window - 1) / p.window);
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    auto go = [&](auto kern) { return launched(who, launch_ex(kern, grid, dim3(APPEND_THREADS), 0, st, 1, false, p)); };
+    if (d->dtype == VLA_BF16)
+      return d->head_dim == 64 ? go(cache_append_kernel<bf16, 64>) : d->head_dim == 128 ? go(cache_append_kernel<bf16, 128>) : go(cache_append_kernel<bf16, 256>);
+    return d->head_dim == 64 ? go(cache_append_kernel<__half, 64>) : d->head_dim == 128 ? go(cache_append_kernel<__half, 128>) : go(cache_append_kernel<__half, 256>);
+  });
+}
+
+int vla_op_paged_attention(const vla_paged_attn_desc* d, void* stream) {
+  const char* who = "vla_op_paged_attention";
+  return guarded(who, [&]() -> int {
+    if (!d) return refuse(VLA_ERR_STATE, "%s: null descriptor", who);
+    if (d->n_seqs < 0 || d->n_q < 1 || d->heads < 1 || d->kv_heads < 1 || d->num_blocks < 1 || d->width < 0 || d->table_stride < d->width)
+      return refuse(VLA_ERR_SHAPE, "%s: bad sizes", who);
+    if (d->heads % d->kv_heads) return refuse(VLA_ERR_SHAPE, "%s: heads must be a multiple of kv_heads", who);
+    if (d->head_dim != 64 && d->head_dim != 128 && d->head_dim != 256) return refuse(VLA_ERR_SHAPE, "%s: head_dim must be 64, 128 or 256", who);
+    if (d->block_size < 16 || d->block_size % 16 || d->block_size > 256) return refuse(VLA_ERR_SHAPE, "%s: block_size must be a multiple of 16 up to 256", who);
+    if ((long long)d->width * d->block_size > INT_TOP || (long long)d->num_blocks * d->block_size > INT_TOP)
+      return refuse(VLA_ERR_LIMIT, "%s: more than 2^31 - 1 tokens", who);
+    if (d->dtype != VLA_BF16 && d->dtype != VLA_F16) return refuse(VLA_ERR_SHAPE, "%s: q must be bf16 or f16", who);
+    if (!(d->scale > 0.f) || d->scale > 3e38f) return refuse(VLA_ERR_SHAPE, "%s: scale must be positive and finite", who);
+    if (d->n_seqs == 0) return VLA_OK;
+    if (!d->q || !d->o || !d->k_codes || !d->v_codes || !d->k_scale || !d->v_scale || !d->seq_lens || (d->width && !d->block_table))
+      return refuse(VLA_ERR_STATE, "%s: null argument", who);
+    if (!aligned(d->k_codes, 16) || !aligned(d->v_codes, 16)) return refuse(VLA_ERR_SHAPE, "%s: the cache must start on 16 bytes", who);
+    if (!vectors(d->q, d->q_seq_stride, d->q_tok_stride) || d->q_head_stride % 8 || !vectors(d->o, d->o_seq_stride, d->o_tok_stride) || d->o_head_stride % 8)
+      return refuse(VLA_ERR_SHAPE, "%s: rows of q and o must start on 16 bytes", who);
+    PagedAttnParams p;
+    p.q = d->q; p.o = d->o;
+    p.q_seq = d->q_seq_stride; p.q_tok = d->q_tok_stride; p.q_head = d->q_head_stride;
+    p.o_seq = d->o_seq_stride; p.o_tok = d->o_tok_stride; p.o_head = d->o_head_stride;
+    p.kc = reinterpret_cast<const uint8_t*>(d->k_codes); p.vc = reinterpret_cast<const uint8_t*>(d->v_codes);
+    p.ks = d->k_scale; p.vs = d->v_scale;
+    p.table = d->block_table; p.table_ld = d->table_stride; p.lens = d->seq_lens;
+    p.n_seqs = d->n_seqs; p.n_q = d->n_q; p.heads = d->heads; p.kv_heads = d->kv_heads; p.dim = d->head_dim;
+    p.blocks = d->num_blocks; p.block = d->block_size; p.width = d->width;
+    p.scale_log2e = d->scale * 1.4426950408889634f;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    const dim3 grid(d->n_seqs * d->n_q, (d->heads + 3) / 4);
+    auto go = [&](auto kern) { return launched(who, launch_ex(kern, grid, dim3(128), 0, st, 1, false, p)); };
+    return d->dtype == VLA_BF16 ? go(paged_attention_kernel<bf16>) : go(paged_attention_kernel<__half>);
+  });
+}
+
+int vla_op_prompt_attention(const vla_prompt_attn_desc* d, void* stream) {
+  const char* who = "vla_op_prompt_attention";
+  return guarded(who, [&]() -> int {
+    if (!d) return refuse(VLA_ERR_STATE, "%s: null descriptor", who);
+    if (d->n_seqs < 0 || d->tokens_q < 0 || d->tokens_k < 0 || d->heads < 1 || d->kv_heads < 1) return refuse(VLA_ERR_SHAPE, "%s: bad sizes", who);
+    if (d->heads % d->kv_heads) return refuse(VLA_ERR_SHAPE, "%s: heads must be a multiple of kv_heads", who);
+    if (d->heads / d->kv_heads > 128) return refuse(VLA_ERR_LIMIT, "%s: at most 128 query heads share a key/value head", who);
+    if (d->head_dim < 8 || d->head_dim % 8 || d->head_dim > 256) return refuse(VLA_ERR_SHAPE, "%s: head_dim must be a multiple of 8 up to 256", who);
+    if (d->dtype != VLA_BF16 && d->dtype != VLA_F16) return refuse(VLA_ERR_SHAPE, "%s: q, k and v must be bf16 or f16", who);
+    if (!(d->scale > 0.f) || d->scale > 3e38f) return refuse(VLA_ERR_SHAPE, "%s: scale must be positive and finite", who);
+    if (d->n_seqs == 0 || d->tokens_q == 0) return VLA_OK;
+    if (!d->q || !d->o || !d->cu_q || !d->cu_k || (d->tokens_k && (!d->k || !d->v))) return refuse(VLA_ERR_STATE, "%s: null argument", who);
+    if (!vectors(d->q, d->q_tok_stride, d->q_head_stride) || !vectors(d->k, d->k_tok_stride, d->k_head_stride) ||
+        !vectors(d->v, d->v_tok_stride, d->v_head_stride) || !vectors(d->o, d->o_tok_stride, d->o_head_stride))
+      return refuse(VLA_ERR_SHAPE, "%s: rows of q, k, v and o must start on 16 bytes", who);
+    PromptAttnParams p;
+    p.q = d->q; p.k = d->k; p.v = d->v; p.o = d->o; p.cu_q = d->cu_q; p.cu_k = d->cu_k;
+    p.n_seqs = d->n_seqs; p.tokens_q = d->tokens_q; p.tokens_k = d->tokens_k;
+    p.heads = d->heads; p.kv_heads = d->kv_heads; p.dim = d->head_dim;
+    p.q_tok = d->q_tok_stride; p.q_head = d->q_head_stride; p.k_tok = d->k_tok_stride; p.k_head = d->k_head_stride;
+    p.v_tok = d->v_tok_stride; p.v_head = d->v_head_stride; p.o_tok = d->o_tok_stride; p.o_head = d->o_head_stride;
+    p.causal = d->causal ? 1 : 0;
+    p.scale_log2e = d->scale * 1.4426950408889634f;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    const dim3 grid(d->tokens_q, (d->heads + 3) / 4);
+    auto go = [&](auto kern) { return launched(who, launch_ex(kern, grid, dim3(128), 0, st, 1, false, p)); };
+    return d->dtype == VLA_BF16 ? go(prompt_attention_kernel<bf16>) : go(prompt_attention_kernel<__half>);
+  });
+}
+
+}  // extern "C"

@@ -25,33 +25,15 @@
 #include "elementwise.cuh"
 #include "expert_persistent.cuh"
 #include "gemm_sm100.cuh"
+#include "host.cuh"
 #include "link.cuh"
 #include "preprocess.cuh"
 
 namespace {
 
-thread_local std::string g_last_error;
-
 // The persistent action-expert kernel serves eligible handles by default when true; flags bit 5 selects it
 // explicitly, bit 4 refuses it.
 constexpr bool XP_DEFAULT_ON = true;
-
-// ---------------------------------------------------------------------------------------------------
-// driver entry point for tensor-map encoding (no link-time dependency on libcuda)
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeTiledFn get_encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  if (!fn) {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult qres;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qres) == cudaSuccess &&
-        qres == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-  }
-  return fn;
-}
 
 // bf16 [rows, K] row-major with row pitch ld (elements): box = 64 (K) x box_rows, 128-byte swizzle.
 bool make_tmap(CUtensorMap* tm, const void* base, long long K, long long rows, long long ld, int box_rows,
@@ -117,51 +99,6 @@ bool make_out_tmap(CUtensorMap* tm, const void* base, bool f32, long long cols, 
     return false;
   }
   return true;
-}
-
-// ---------------------------------------------------------------------------------------------------
-// generic launch with optional cluster dimension and programmatic dependent launch
-template <typename... KArgs, typename... Args>
-cudaError_t launch_ex(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, int cluster_x, bool pdl,
-                      Args&&... args) {
-  cudaLaunchConfig_t cfg;
-  memset(&cfg, 0, sizeof cfg);
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attrs[2];
-  int n = 0;
-  if (cluster_x > 1) {
-    attrs[n].id = cudaLaunchAttributeClusterDimension;
-    attrs[n].val.clusterDim.x = cluster_x;
-    attrs[n].val.clusterDim.y = 1;
-    attrs[n].val.clusterDim.z = 1;
-    ++n;
-  }
-  if (pdl) {
-    attrs[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attrs[n].val.programmaticStreamSerializationAllowed = 1;
-    ++n;
-  }
-  cfg.attrs = attrs;
-  cfg.numAttrs = n;
-  return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
-}
-
-// The dynamic shared-memory opt-in of a kernel applies to the CURRENT device only, so it is remembered per
-// (device, kernel): a process may hold handles on several GPUs.
-cudaError_t ensure_smem_attr(const void* func, int bytes) {
-  static std::mutex mu;
-  static std::set<std::pair<int, const void*>> done;
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  std::lock_guard<std::mutex> lock(mu);
-  if (done.count({dev, func})) return cudaSuccess;
-  e = cudaFuncSetAttribute(func, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess) done.insert({dev, func});
-  return e;
 }
 
 // ---------------------------------------------------------------------------------------------------

@@ -1,6 +1,11 @@
 """Python callers of the single-operator C-ABI entry points (vla_op_*): kernel-level parity tests and
-micro-benchmarks call the kernels through these."""
+micro-benchmarks call the kernels through these.
+
+The operators around a key/value cache in pages (block_plan, cache_append, paged_attention, prompt_attention) are for
+programs that serve sequences of different lengths: they take torch tensors, enqueue on the current stream of the tensors'
+device and return without synchronising, so they can be captured into a CUDA graph.  They run forward only."""
 import ctypes as C
+from typing import NamedTuple
 
 import torch
 
@@ -107,3 +112,179 @@ def vit_attention_tc(qkv, *, scale, iters=0):
     stream = torch.cuda.current_stream(qkv.device).cuda_stream
     _capi.check(lib.vla_op_vit_attention_tc(_p(qkv), _p(out), views, float(scale), iters, C.byref(ms), C.c_void_p(stream)))
     return (out, ms.value) if iters else out
+
+
+# ---- a key/value cache in pages, held in 8 bits -----------------------------------------------------------------------
+_DTYPES = {torch.bfloat16: _capi.VLA_BF16, torch.float16: _capi.VLA_F16}
+
+
+class KvCache(NamedTuple):
+    """Pages of tokens as e4m3 codes with one scale for each page and head; a value is code * scale."""
+    k: torch.Tensor          # float8_e4m3fn [blocks, kv_heads, block_size, head_dim]
+    v: torch.Tensor
+    k_scale: torch.Tensor    # float32 [blocks, kv_heads]
+    v_scale: torch.Tensor
+
+
+class BlockPlan(NamedTuple):
+    slots: torch.Tensor       # int32 [total_new]: block * block_size + offset of each new token, -1: none
+    positions: torch.Tensor   # int32 [total_new]: position in its sequence
+    cu_new: torch.Tensor      # int32 [n + 1]: first row of each request
+    seq_lens: torch.Tensor    # int32 [n]: tokens of each request that have a slot
+    counts: torch.Tensor      # int32 [3]: next free index, blocks missing, sum of new tokens
+
+
+def kv_cache(blocks, kv_heads, block_size, head_dim, device=None):
+    """An empty cache (all pages zero)."""
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
+    codes = [torch.zeros(blocks, kv_heads, block_size, head_dim, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+             for _ in range(2)]
+    scales = [torch.zeros(blocks, kv_heads, device=device) for _ in range(2)]
+    return KvCache(*codes, *scales)
+
+
+def _refuse(cond, text):
+    if cond:
+        raise _capi.VlaError("vla_ops: " + text)
+
+
+def _whole(t, name, device, dim=1):
+    """int32 tensor of `dim` dimensions on `device`, rows contiguous."""
+    _refuse(t.dtype != torch.int32 or t.dim() != dim, "%s must be int32 with %d dimension(s), got %s %s" % (name, dim, t.dtype, tuple(t.shape)))
+    _refuse(t.device != device, "%s is on %s, not on %s" % (name, t.device, device))
+    _refuse(t.shape[-1] > 1 and t.stride(-1) != 1, "%s must be contiguous" % name)
+    return t.data_ptr()
+
+
+def _rows(t, name, device, dtype, dim):
+    _refuse(t.dtype != dtype or t.dim() != dim or t.device != device,
+            "%s must be %s with %d dimensions on %s, got %s %s on %s" % (name, dtype, dim, device, t.dtype, tuple(t.shape), t.device))
+    _refuse(t.stride(-1) != 1 and t.shape[-1] > 1, "the last dimension of %s must be contiguous" % name)
+    _refuse(t.requires_grad and torch.is_grad_enabled(), "%s requires a gradient; this operator has no backward pass" % name)
+    return t.data_ptr()
+
+
+def _cache(cache, device):
+    k, v, ks, vs = cache
+    _refuse(k.dim() != 4 or k.shape != v.shape or ks.shape != k.shape[:2] or vs.shape != ks.shape, "cache tensors do not fit each other")
+    _refuse(k.dtype != torch.float8_e4m3fn or v.dtype != k.dtype or ks.dtype != torch.float32 or vs.dtype != ks.dtype,
+            "a cache is held as float8_e4m3fn with float32 scales")
+    for t in cache:
+        _refuse(t.device != device or not t.is_contiguous(), "cache tensors must be contiguous and on %s" % device)
+    return k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr()
+
+
+def _enqueue(fn, desc, device):
+    stream = C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    if torch.cuda.current_device() == device.index:
+        rc = fn(C.byref(desc), stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(C.byref(desc), stream)
+    if rc:
+        _capi.check(rc)
+
+
+def _on_gpu(t, name):
+    _refuse(not t.is_cuda, "%s must be on a GPU; there is no CPU path" % name)
+    return t.device
+
+
+def block_plan(context_lens, new_lens, block_table, free_blocks, *, block_size, total_new, first_free=None):
+    """Pages and slots for the new tokens of every request, from the lengths alone, on the device.
+
+    context_lens, new_lens int32 [n]; block_table int32 [n, width], updated in place with the blocks each request gets;
+    free_blocks int32 [f], taken in order from index first_free (int32 [1] on the device, e.g. counts[:1] of the call
+    before; None: 0).  total_new is the number of rows of slots and positions (the sum of new_lens, or more for a padded
+    batch).  Returns a BlockPlan; counts[1] > 0 says that blocks were missing and some tokens have slot -1."""
+    dev = _on_gpu(context_lens, "context_lens")
+    n = context_lens.shape[0]
+    _refuse(new_lens.shape[0] != n or block_table.shape[0] != n, "context_lens, new_lens and block_table do not fit each other")
+    _refuse(first_free is not None and first_free.numel() != 1, "first_free must hold one number")
+    rows = (total_new + 3) // 4 * 4       # each part of the one allocation starts on 16 bytes
+    seqs = (n + 4) // 4 * 4
+    out = torch.empty(2 * rows + 2 * seqs + 4, dtype=torch.int32, device=dev)
+    slots, positions = out[:total_new], out[rows:rows + total_new]
+    cu, lens, counts = out[2 * rows:2 * rows + n + 1], out[2 * rows + seqs:2 * rows + seqs + n], out[2 * rows + 2 * seqs:2 * rows + 2 * seqs + 3]
+    base = out.data_ptr()
+    d = _capi.BlockPlanDesc(_whole(context_lens, "context_lens", dev), _whole(new_lens, "new_lens", dev), n,
+                            _whole(block_table, "block_table", dev, 2), block_table.shape[1],
+                            block_table.stride(0) if n > 1 else block_table.shape[1],
+                            _whole(free_blocks, "free_blocks", dev), free_blocks.shape[0],
+                            None if first_free is None else _whole(first_free, "first_free", dev), block_size, total_new,
+                            base, base + 4 * rows, base + 8 * rows, base + 8 * rows + 4 * seqs, base + 8 * rows + 8 * seqs)
+    _enqueue(_capi.lib().vla_op_block_plan, d, dev)
+    return BlockPlan(slots, positions, cu, lens, counts)
+
+
+def cache_append(k, v, cache, slots):
+    """Keys and values (bf16 or fp16 [tokens, kv_heads, head_dim]) into the cache at slots (int32 [tokens]), in place.
+
+    Slots outside the cache are skipped; the tokens of one block must be consecutive rows.  A block whose first slot is written
+    starts anew; another block's scale grows where the new tokens need it and its codes are rounded again."""
+    dev = _on_gpu(k, "k")
+    t = k.dtype
+    _refuse(t not in _DTYPES, "k and v must be bfloat16 or float16, got %s" % t)
+    codes = _cache(cache, dev)
+    blocks, heads, block, dim = cache.k.shape
+    pk, pv = _rows(k, "k", dev, t, 3), _rows(v, "v", dev, t, 3)
+    _refuse(k.shape != v.shape or k.shape[1:] != (heads, dim) or slots.shape[0] != k.shape[0],
+            "k %s, v %s and slots %s do not fit the cache %s" % (tuple(k.shape), tuple(v.shape), tuple(slots.shape), tuple(cache.k.shape)))
+    d = _capi.CacheAppendDesc(pk, pv, _whole(slots, "slots", dev), k.shape[0], k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+                              *codes, blocks, heads, block, dim, _DTYPES[t])
+    _enqueue(_capi.lib().vla_op_cache_append, d, dev)
+
+
+def paged_attention(q, cache, block_table, seq_lens, *, scale=None, out=None):
+    """Attention of the newest tokens of every sequence over the cache.
+
+    q bf16 or fp16 [n, tokens, heads, head_dim]: the last tokens of each sequence, whose keys are in the cache already;
+    each sees itself and what is before it.  block_table int32 [n, width], seq_lens int32 [n].  scale: head_dim ** -0.5
+    unless given.  Returns out, or a new tensor like q; a row that sees nothing is zero."""
+    dev = _on_gpu(q, "q")
+    t = q.dtype
+    _refuse(t not in _DTYPES, "q must be bfloat16 or float16, got %s" % t)
+    codes = _cache(cache, dev)
+    blocks, kv_heads, block, dim = cache.k.shape
+    pq = _rows(q, "q", dev, t, 4)
+    n, tokens, heads, _ = q.shape
+    _refuse(q.shape[3] != dim or block_table.shape[0] != n or seq_lens.shape[0] != n,
+            "q %s, block_table %s, seq_lens %s and cache %s do not fit each other" % (
+                tuple(q.shape), tuple(block_table.shape), tuple(seq_lens.shape), tuple(cache.k.shape)))
+    if out is None:
+        out = torch.empty(q.shape, dtype=t, device=dev)
+    po = _rows(out, "out", dev, t, 4)
+    _refuse(out.shape != q.shape, "out must have the shape of q")
+    d = _capi.PagedAttnDesc(pq, po, *q.stride()[:3], *out.stride()[:3], *codes, _whole(block_table, "block_table", dev, 2),
+                            block_table.stride(0) if n > 1 else block_table.shape[1], _whole(seq_lens, "seq_lens", dev),
+                            n, tokens, heads, kv_heads, dim, blocks, block, block_table.shape[1],
+                            dim ** -0.5 if scale is None else scale, _DTYPES[t])
+    _enqueue(_capi.lib().vla_op_paged_attention, d, dev)
+    return out
+
+
+def prompt_attention(q, k, v, cu_q, cu_k=None, *, causal=True, scale=None, out=None):
+    """Attention over packed prompts of different lengths.
+
+    q bf16 or fp16 [tokens, heads, head_dim], k and v [keys, kv_heads, head_dim]; sequence b owns rows cu_q[b] .. cu_q[b + 1] of
+    q and cu_k[b] .. cu_k[b + 1] of k and v (int32 [n + 1] on the device, ascending; cu_k: as cu_q unless given).  causal: the last row
+    of a sequence sees all its keys, each row before it one less; otherwise every row sees all.  Returns out, or a new
+    tensor like q; a row that sees nothing is zero, rows behind the last sequence are not written."""
+    dev = _on_gpu(q, "q")
+    t = q.dtype
+    _refuse(t not in _DTYPES, "q, k and v must be bfloat16 or float16, got %s" % t)
+    cu_k = cu_q if cu_k is None else cu_k
+    pq, pk, pv = _rows(q, "q", dev, t, 3), _rows(k, "k", dev, t, 3), _rows(v, "v", dev, t, 3)
+    _refuse(k.shape != v.shape or k.shape[2] != q.shape[2] or cu_q.shape != cu_k.shape or cu_q.shape[0] < 1,
+            "q %s, k %s, v %s, cu_q %s and cu_k %s do not fit each other" % (
+                tuple(q.shape), tuple(k.shape), tuple(v.shape), tuple(cu_q.shape), tuple(cu_k.shape)))
+    if out is None:
+        out = torch.empty(q.shape, dtype=t, device=dev)
+    po = _rows(out, "out", dev, t, 3)
+    _refuse(out.shape != q.shape, "out must have the shape of q")
+    tokens, heads, dim = q.shape
+    d = _capi.PromptAttnDesc(pq, pk, pv, po, _whole(cu_q, "cu_q", dev), _whole(cu_k, "cu_k", dev), cu_q.shape[0] - 1, tokens,
+                             k.shape[0], heads, k.shape[1], dim, *q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *out.stride()[:2],
+                             1 if causal else 0, dim ** -0.5 if scale is None else scale, _DTYPES[t])
+    _enqueue(_capi.lib().vla_op_prompt_attention, d, dev)
+    return out

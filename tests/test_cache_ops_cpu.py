@@ -1,0 +1,102 @@
+"""What the C entry points and the wrappers of the operators around a key/value cache in pages refuse, without a GPU: every
+refusal comes before a launch, with a code and a message."""
+import ctypes as C
+import os
+
+import pytest
+import torch
+
+import _capi
+import vla_ops
+
+needs_library = pytest.mark.skipif(not os.path.exists(_capi.LIB_PATH), reason="library not built")
+P = 4096          # an address for arguments that are only checked, never followed
+
+
+def call(name, desc):
+    lib = _capi.lib()
+    rc = getattr(lib, name)(C.byref(desc) if desc is not None else None, None)
+    return rc, lib.vla_last_error(None).decode()
+
+
+def plan_desc(**kw):
+    d = _capi.BlockPlanDesc(P, P, 2, P, 4, 4, P, 8, None, 16, 5, P, P, P, P, P)
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+def append_desc(**kw):
+    d = _capi.CacheAppendDesc(P, P, P, 3, 256, 128, 256, 128, P, P, P, P, 8, 2, 16, 128, _capi.VLA_BF16)
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+def paged_desc(**kw):
+    d = _capi.PagedAttnDesc(P, P, 1024, 1024, 128, 1024, 1024, 128, P, P, P, P, P, 4, P, 2, 1, 8, 2, 128, 8, 16, 4, 0.1, _capi.VLA_BF16)
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+def prompt_desc(**kw):
+    d = _capi.PromptAttnDesc(P, P, P, P, P, P, 2, 9, 9, 8, 2, 128, 1024, 128, 256, 128, 256, 128, 1024, 128, 1, 0.1, _capi.VLA_BF16)
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+STATE, SHAPE, LIMIT = 4, 3, 5
+CASES = [
+    ("vla_op_block_plan", plan_desc, [
+        (STATE, dict(context_lens=None)), (STATE, dict(block_table=None)), (STATE, dict(free_blocks=None)), (STATE, dict(slots=None)),
+        (STATE, dict(counts=None)), (STATE, dict(seq_lens=None)), (SHAPE, dict(block_size=0)), (SHAPE, dict(total_new=-1)),
+        (SHAPE, dict(table_stride=3)), (SHAPE, dict(slots=P + 4)), (LIMIT, dict(n_seqs=8193)), (LIMIT, dict(n_seqs=-1))]),
+    ("vla_op_cache_append", append_desc, [
+        (STATE, dict(k=None)), (STATE, dict(slots=None)), (STATE, dict(v_codes=None)), (STATE, dict(k_scale=None)), (SHAPE, dict(tokens=-1)),
+        (SHAPE, dict(head_dim=96)), (SHAPE, dict(head_dim=0)), (SHAPE, dict(block_size=8)), (SHAPE, dict(block_size=272)),
+        (SHAPE, dict(dtype=_capi.VLA_F32)), (SHAPE, dict(k=P + 2)), (SHAPE, dict(v_tok_stride=257)), (SHAPE, dict(k_codes=P + 8)),
+        (SHAPE, dict(kv_heads=0)), (LIMIT, dict(num_blocks=2 ** 27))]),
+    ("vla_op_paged_attention", paged_desc, [
+        (STATE, dict(q=None)), (STATE, dict(o=None)), (STATE, dict(block_table=None)), (STATE, dict(seq_lens=None)), (STATE, dict(v_scale=None)),
+        (SHAPE, dict(heads=7)), (SHAPE, dict(heads=0)), (SHAPE, dict(kv_heads=0)), (SHAPE, dict(n_q=0)), (SHAPE, dict(head_dim=72)),
+        (SHAPE, dict(block_size=24)), (SHAPE, dict(dtype=_capi.VLA_F32)), (SHAPE, dict(scale=0.0)), (SHAPE, dict(scale=float("nan"))),
+        (SHAPE, dict(scale=float("inf"))), (SHAPE, dict(q=P + 8)), (SHAPE, dict(o_head_stride=4)), (SHAPE, dict(table_stride=3)),
+        (SHAPE, dict(num_blocks=0)), (LIMIT, dict(width=2 ** 28, table_stride=2 ** 28))]),
+    ("vla_op_prompt_attention", prompt_desc, [
+        (STATE, dict(q=None)), (STATE, dict(v=None)), (STATE, dict(cu_k=None)), (STATE, dict(o=None)), (SHAPE, dict(heads=3)),
+        (SHAPE, dict(head_dim=4)), (SHAPE, dict(head_dim=264)), (SHAPE, dict(head_dim=100)), (SHAPE, dict(tokens_q=-1)), (SHAPE, dict(n_seqs=-2)),
+        (SHAPE, dict(dtype=7)), (SHAPE, dict(scale=-1.0)), (SHAPE, dict(k=P + 4)), (SHAPE, dict(v_tok_stride=4)), (LIMIT, dict(heads=129, kv_heads=1))]),
+]
+
+
+@needs_library
+@pytest.mark.parametrize("name,make,code,change", [(n, m, c, k) for n, m, cases in CASES for c, k in cases])
+def test_entry_points_refuse(name, make, code, change):
+    rc, text = call(name, make(**change))
+    assert rc == code and name in text
+
+
+@needs_library
+@pytest.mark.parametrize("name", [c[0] for c in CASES])
+def test_null_descriptor(name):
+    assert call(name, None)[0] == STATE
+
+
+@needs_library
+@pytest.mark.parametrize("name,desc", [("vla_op_cache_append", append_desc(tokens=0, k=None, v=None, slots=None)),
+                                       ("vla_op_paged_attention", paged_desc(n_seqs=0, q=None)),
+                                       ("vla_op_prompt_attention", prompt_desc(n_seqs=0)), ("vla_op_prompt_attention", prompt_desc(tokens_q=0, q=None))])
+def test_nothing_to_do_is_no_error(name, desc):
+    assert call(name, desc)[0] == 0
+
+
+def test_wrappers_refuse_the_cpu():
+    q, i = torch.zeros(2, 4, 64, dtype=torch.bfloat16), torch.zeros(2, dtype=torch.int32)
+    cache = vla_ops.kv_cache(2, 2, 16, 64, "cpu")
+    assert cache.k.shape == (2, 2, 16, 64) and cache.k.dtype == torch.float8_e4m3fn and cache.v_scale.shape == (2, 2)
+    for f in (lambda: vla_ops.prompt_attention(q, q, q, i), lambda: vla_ops.paged_attention(q[None], cache, i[None], i[:1]),
+              lambda: vla_ops.cache_append(q[:, :2], q[:, :2], cache, i), lambda: vla_ops.block_plan(i, i, i[None], i, block_size=16, total_new=0)):
+        with pytest.raises(_capi.VlaError, match="no CPU path"):
+            f()

@@ -351,6 +351,10 @@ typedef struct vla_prompt_attn_desc {
 } vla_prompt_attn_desc;
 int vla_op_prompt_attention(const vla_prompt_attn_desc* d, void* stream);
 
+/* Status word of the calls above on the current device: bit 0 = a bounded wait inside a kernel ran out, and the output of an
+ * earlier call is not to be trusted.  Synchronises, returns the word and clears it. */
+int vla_op_cache_status(int* out);
+
 #ifdef __cplusplus
 }
 #endif

@@ -3,70 +3,441 @@
 // last row sees every key; keys that stand before the prompt's own are seen by all of its rows):
 //     o_i = sum_{j < L_i} p_ij v_j / sum_{j < L_i} p_ij,   p_ij = exp(scale q_i . k_j - max_j)
 // A row with L_i <= 0 is zero.  heads / kv_heads consecutive query heads share a key/value head.
+//
+// One CTA = one tile of 128 rows: the G = heads / kv_heads query heads of 128 / G consecutive tokens, which share their
+// keys, so that short prompts fill tiles too and a causal tile's diagonal is only 128 / G keys wide.  Chunks of 128 keys:
+//     S[128 x 128]  = Q . K_chunk^T       tcgen05.mma, both operands K-major in shared memory
+//     P             = exp2(S scale - m)   one thread per row, straight from TMEM, written back over S as 16-bit pairs
+//     O[128 x dim] += P . V_chunk         tcgen05.mma, A = P in TMEM, B = V as it lies in memory (MN-major), so V needs
+//                                         neither a transposed copy nor a pass through registers
+// The maximum m a row subtracts is only moved when it grows by more than 2^8 (probabilities then stay below 2^8, sums in
+// fp32), so that O in TMEM is rescaled a few times per tile instead of once per chunk.
+// Roles: warp 0 = tile lookup and TMA producer, warp 1 = MMA issuer and TMEM owner, warps 2..5 = softmax and epilogue.
+// All mbarrier waits are bounded.
 #pragma once
 #include <cuda_fp16.h>
 #include "common.cuh"
 
 struct PromptAttnParams {
-  const void* q;
-  const void* k;
+  CUtensorMap tmQ;   // [token][kv head][group head][dim], box 64 x G x 1 x tokens of a tile
+  CUtensorMap tmK;   // [token][kv head][dim], box 64 x 1 x 128
+  CUtensorMap tmV;   // the same, box 64 x 1 x V_ROWS
   const void* v;
   void* o;
   const int* cu_q;
   const int* cu_k;
   int n_seqs, tokens_q, tokens_k;
-  int heads, kv_heads, dim;
-  long long q_tok, q_head, k_tok, k_head, v_tok, v_head, o_tok, o_head;
+  int kv_heads, group, dim;
+  int tile_tokens;   // 128 / group
+  long long v_tok, v_head, o_tok, o_head;
   int causal;
   float scale_log2e;
 };
 
-// One warp per (row, head), lanes over the head dim, one key after the other.
+// Bits VLA_ST_* of the operators in this translation unit: a bounded wait that ran out.
+static __device__ int cache_ops_status;
+
+// Up to 128 columns of head dim a CTA needs half an SM (96 KB of shared memory, 256 TMEM columns), and the two CTAs of an
+// SM fill each other's waits between S, softmax and P V.  Wider heads need the whole SM: two S buffers, so that the next
+// chunk's S is there when the softmax has finished a chunk, and K and V in half chunks of 32 KB.
+template <bool WIDE>
+struct PromptCfg {
+  static constexpr int BOXES = WIDE ? 4 : 2;              // 64-column boxes of head dim, at most
+  static constexpr int AHEAD = WIDE ? 2 : 1;              // S buffers = chunks of S in flight
+  static constexpr int UNITS = WIDE ? 2 : 1;              // ring slots per K or V chunk
+  static constexpr int STAGES = WIDE ? 5 : 2;
+  static constexpr int V_ROWS = 128 / UNITS;
+  static constexpr int BOX_BYTES = 128 * 128;             // 64 columns x 128 rows
+  static constexpr int SLOT_BYTES = 2 * BOX_BYTES;        // K: 2 boxes x 128 keys; V: BOXES boxes x V_ROWS keys
+  static constexpr int Q_BYTES = BOXES * BOX_BYTES;
+  static constexpr int SMEM_BYTES = Q_BYTES + STAGES * SLOT_BYTES + 256 + 1024;
+  static constexpr int TMEM_COLS = WIDE ? 512 : 256;      // S buffers, then O
+  static constexpr int O_COL = AHEAD * 128;
+  static constexpr int THREADS = 192;
+};
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tm, uint32_t bar, int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(dst), "l"(tm), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem desc]; A holds two consecutive K elements per 32-bit column.
+__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
+      ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// MN-major operand (rows of K, 64 MN columns of 128 bytes each, 128-byte swizzle): 8-row groups 1024 bytes apart, the next
+// 64 columns `box_bytes` further.
+__device__ __forceinline__ uint64_t prompt_desc_mn(uint32_t smem_addr, uint32_t box_bytes) {
+  return (uint64_t)((smem_addr & 0x3FFFF) >> 4) | ((uint64_t)(box_bytes >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+
 template <typename T>
-__global__ void __launch_bounds__(128) prompt_attention_kernel(const PromptAttnParams p) {
-  const int lane = threadIdx.x & 31;
-  const int t = blockIdx.x, head = blockIdx.y * 4 + (threadIdx.x >> 5);
-  if (head >= p.heads) return;
-  int b = 0, q0 = 0, q1 = 0;
-  for (; b < p.n_seqs; ++b) {
-    q0 = min(max(p.cu_q[b], 0), p.tokens_q);
-    q1 = min(max(p.cu_q[b + 1], q0), p.tokens_q);
-    if (t >= q0 && t < q1) break;
+struct Half16;   // what differs between the two 16-bit types
+template <>
+struct Half16<bf16> {
+  static constexpr uint32_t MMA_TYPE = 1u;
+  static constexpr uint32_t EXP_LO = 0x7f80u;
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
   }
-  if (b == p.n_seqs) return;
-  const int k0 = min(max(p.cu_k[b], 0), p.tokens_k), k1 = min(max(p.cu_k[b + 1], k0), p.tokens_k);
-  const int nk = k1 - k0;
-  const int limit = p.causal ? min(nk, t - q0 + nk - (q1 - q0) + 1) : nk;
-  const int hk = head / (p.heads / p.kv_heads);
-  const T* q = reinterpret_cast<const T*>(p.q) + t * p.q_tok + head * p.q_head;
-  const T* k = reinterpret_cast<const T*>(p.k) + k0 * p.k_tok + hk * p.k_head;
-  const T* v = reinterpret_cast<const T*>(p.v) + k0 * p.v_tok + hk * p.v_head;
-  float qr[8], acc[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int d = lane + 32 * i;
-    qr[i] = d < p.dim ? (float)q[d] : 0.f;
-    acc[i] = 0.f;
+  static __device__ __forceinline__ float value(uint32_t bits) { return __uint_as_float(bits << 16); }
+};
+template <>
+struct Half16<__half> {
+  static constexpr uint32_t MMA_TYPE = 0u;
+  static constexpr uint32_t EXP_LO = 0x7c00u;
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
   }
-  float m = -INFINITY, l = 0.f;
-  for (int j = 0; j < limit; ++j) {
-    float s = 0.f;
+  static __device__ __forceinline__ float value(uint32_t bits) { return __half2float(__ushort_as_half((unsigned short)bits)); }
+};
+
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(PromptCfg<WIDE>::THREADS, WIDE ? 1 : 2) prompt_attention_kernel(const __grid_constant__ PromptAttnParams p) {
+  using C = PromptCfg<WIDE>;
+  using H = Half16<T>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  const uint32_t pad = (1024u - (raw_addr & 1023u)) & 1023u;
+  const uint32_t sQ = raw_addr + pad, sRing = sQ + C::Q_BYTES;
+  uint8_t* ring = smem_raw + pad + C::Q_BYTES;
+  uint8_t* bar_ptr = ring + C::STAGES * C::SLOT_BYTES;
+  const uint32_t bars = sRing + C::STAGES * C::SLOT_BYTES;
+  const uint32_t q_full = bars;
+  auto full = [&](int s) { return bars + 8 + 16 * s; };
+  auto empty = [&](int s) { return bars + 16 + 16 * s; };
+  auto s_full = [&](int b) { return bars + 96 + 8 * b; };
+  auto p_ready = [&](int b) { return bars + 112 + 8 * b; };
+  auto o_done = [&](int b) { return bars + 128 + 8 * b; };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_ptr + 160);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bar_ptr + 164);
+  volatile int* poison = reinterpret_cast<volatile int*>(bar_ptr + 168);   // a hidden value was not finite
+  volatile int* tile_seq = reinterpret_cast<volatile int*>(bar_ptr + 172);
+  volatile int* tile_at = reinterpret_cast<volatile int*>(bar_ptr + 176);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kvh = blockIdx.x % p.kv_heads;
+  if (warp == 0) {
+    // Which tile this CTA is: the sequences' tiles are counted from cu_q on the device, 32 sequences at a time.  A
+    // causal sequence hands out its last tiles first, because they have the most keys.
+    int idx = blockIdx.x / p.kv_heads, seq = -1, at = 0;
+    for (int base = 0; base < p.n_seqs && seq < 0; base += 32) {
+      int tiles = 0;
+      if (base + lane < p.n_seqs) {
+        const int a = min(max(p.cu_q[base + lane], 0), p.tokens_q), e = min(max(p.cu_q[base + lane + 1], a), p.tokens_q);
+        tiles = (e - a + p.tile_tokens - 1) / p.tile_tokens;
+      }
+      int sum = tiles;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (lane + 32 * i < p.dim) s = fmaf(qr[i], (float)k[j * p.k_tok + lane + 32 * i], s);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    s *= p.scale_log2e;
-    const float m_new = fmaxf(m, s);
-    const float a = exp2f(m - m_new), e = exp2f(s - m_new);
-    m = m_new;
-    l = l * a + e;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (lane + 32 * i < p.dim) acc[i] = acc[i] * a + e * (float)v[j * p.v_tok + lane + 32 * i];
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += u;
+      }
+      const int total = __shfl_sync(0xffffffffu, sum, 31);
+      if (idx < total) {
+        const int l = __ffs(__ballot_sync(0xffffffffu, sum > idx)) - 1;
+        const int t = idx - __shfl_sync(0xffffffffu, sum - tiles, l);
+        seq = base + l;
+        at = p.causal ? __shfl_sync(0xffffffffu, tiles, l) - 1 - t : t;
+      }
+      idx -= total;
+    }
+    if (lane == 0) {
+      *tile_seq = seq;
+      *tile_at = at * p.tile_tokens;
+    }
+  } else if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
+  } else if (threadIdx.x == 64) {
+    mbar_init(q_full, 1);
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(s_full(b), 1);
+      mbar_init(p_ready(b), 128);
+      mbar_init(o_done(b), 1);
+    }
+    *abort_flag = 0;
+    *poison = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&p.tmQ);
+    tma_prefetch_desc(&p.tmK);
+    tma_prefetch_desc(&p.tmV);
   }
-  T* o = reinterpret_cast<T*>(p.o) + t * p.o_tok + head * p.o_head;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int seq = *tile_seq;
+
+  // Lengths, and the limits of the tile's first and last row (every thread: four words from L1 / L2)
+  int q0 = 0, nq = 0, k0 = 0, nk = 0;
+  const int tok0 = *tile_at;
+  if (seq >= 0) {
+    q0 = min(max(p.cu_q[seq], 0), p.tokens_q);
+    nq = min(max(p.cu_q[seq + 1], q0), p.tokens_q) - q0;
+    k0 = min(max(p.cu_k[seq], 0), p.tokens_k);
+    nk = min(max(p.cu_k[seq + 1], k0), p.tokens_k) - k0;
+  }
+  const int last_tok = min(tok0 + p.tile_tokens, nq) - 1;
+  auto limit_of = [&](int tok) { return p.causal ? min(max(tok + nk - nq + 1, 0), nk) : nk; };
+  const int lim_min = seq >= 0 ? limit_of(tok0) : 0, lim_max = seq >= 0 ? limit_of(last_tok) : 0;
+  const int n_chunks = (lim_max + 127) / 128;
+  const int boxes = (p.dim + 63) / 64;
+  // position of a K or V chunk in the ring's order of use: K_0 .. K_{AHEAD-1}, then V_c, K_{c+AHEAD} in turn
+  auto k_pos = [&](int c) { return C::UNITS * (c < C::AHEAD ? c : 2 * c - C::AHEAD + 1); };
+  auto v_pos = [&](int c) { return C::UNITS * (min(c + C::AHEAD, n_chunks) + c); };
+
+  if (warp == 0) {
+    if (lane == 0 && n_chunks > 0) {
+      const int rows = p.group * p.tile_tokens;
+      mbar_expect_tx(q_full, boxes * rows * 128);
+      for (int x = 0; x < boxes; ++x) tma_load_4d(sQ + x * C::BOX_BYTES, &p.tmQ, q_full, x * 64, 0, kvh, q0 + tok0);
+      bool ok = true;
+      auto slot_free = [&](int pos) {
+        return pos < C::STAGES || mbar_wait(empty(pos % C::STAGES), (uint32_t)(pos / C::STAGES - 1) & 1u, abort_flag);
+      };
+      const uint64_t pol = policy_evict_last();   // other tiles of this sequence read the same keys
+      auto load_k = [&](int c) {
+        for (int u = 0; u < C::UNITS && ok; ++u) {
+          const int pos = k_pos(c) + u, s = pos % C::STAGES;
+          ok = slot_free(pos);
+          if (!ok) return;
+          const int b0 = u * 2, nb = min(boxes - b0, 2);
+          if (nb <= 0) {                           // heads of at most 128 columns in the wide kernel do not occur
+            mbar_arrive(full(s));
+            continue;
+          }
+          mbar_expect_tx(full(s), nb * C::BOX_BYTES);
+          for (int x = 0; x < nb; ++x)
+            tma_load_3d(sRing + s * C::SLOT_BYTES + x * C::BOX_BYTES, &p.tmK, full(s), (b0 + x) * 64, kvh, k0 + c * 128, pol);
+        }
+      };
+      auto load_v = [&](int c) {
+        for (int u = 0; u < C::UNITS && ok; ++u) {
+          const int pos = v_pos(c) + u, s = pos % C::STAGES;
+          ok = slot_free(pos);
+          if (!ok) return;
+          mbar_expect_tx(full(s), boxes * C::V_ROWS * 128);
+          for (int x = 0; x < boxes; ++x)
+            tma_load_3d(sRing + s * C::SLOT_BYTES + x * C::V_ROWS * 128, &p.tmV, full(s), x * 64, kvh, k0 + c * 128 + u * C::V_ROWS, pol);
+        }
+      };
+      for (int c = 0; c < min(C::AHEAD, n_chunks); ++c) load_k(c);
+      for (int c = 0; c < n_chunks && ok; ++c) {
+        load_v(c);
+        if (c + C::AHEAD < n_chunks) load_k(c + C::AHEAD);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0 && n_chunks > 0) {
+      const uint32_t idesc = (1u << 4) | (H::MMA_TYPE << 7) | (H::MMA_TYPE << 10) | (8u << 24);
+      const int k_steps = (p.dim + 15) / 16;
+      const uint32_t idesc_o = idesc | (1u << 16) | ((uint32_t)(k_steps * 2) << 17);      // N = head dim, B MN-major
+      bool ok = mbar_wait(q_full, 0, abort_flag);
+      auto issue_s = [&](int c) {
+        // the last chunk multiplies only the keys that some row sees, rounded up to 16
+        const int keys16 = (min(lim_max - c * 128, 128) + 15) / 16;
+        const uint32_t idesc_s = idesc | ((uint32_t)(keys16 * 2) << 17);
+        for (int u = 0; u < C::UNITS; ++u) {
+          const int pos = k_pos(c) + u, s = pos % C::STAGES;
+          ok = ok && mbar_wait(full(s), (uint32_t)(pos / C::STAGES) & 1u, abort_flag);
+          if (!ok) return;
+          tc_fence_after();
+          for (int ks = u * 8; ks < min(k_steps, u * 8 + 8); ++ks) {
+            const uint64_t da = attn_desc_sw128(sQ + (ks >> 2) * C::BOX_BYTES) + 2 * (ks & 3);
+            const uint64_t db = attn_desc_sw128(sRing + s * C::SLOT_BYTES + ((ks >> 2) - 2 * u) * C::BOX_BYTES) + 2 * (ks & 3);
+            umma_bf16(tmem + (c % C::AHEAD) * 128, da, db, idesc_s, ks != 0);
+          }
+          umma_commit(empty(s));
+        }
+        umma_commit(s_full(c % C::AHEAD));
+      };
+      for (int c = 0; c < min(C::AHEAD, n_chunks) && ok; ++c) issue_s(c);
+      for (int c = 0; c < n_chunks && ok; ++c) {
+        const int buf = c % C::AHEAD;
+        ok = mbar_wait(p_ready(buf), (uint32_t)(c / C::AHEAD) & 1u, abort_flag);
+        const int keys16 = (min(lim_max - c * 128, 128) + 15) / 16;
+        for (int u = 0; u < C::UNITS; ++u) {
+          const int pos = v_pos(c) + u, s = pos % C::STAGES;
+          ok = ok && mbar_wait(full(s), (uint32_t)(pos / C::STAGES) & 1u, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t db = prompt_desc_mn(sRing + s * C::SLOT_BYTES, C::V_ROWS * 128);
+          for (int kk = 0; kk < min(keys16 - u * (C::V_ROWS / 16), C::V_ROWS / 16); ++kk)
+            umma_ts(tmem + C::O_COL, tmem + buf * 128 + (u * (C::V_ROWS / 16) + kk) * 8, db + 128 * kk, idesc_o, (c | u | kk) != 0);
+          umma_commit(empty(s));
+        }
+        if (!ok) break;
+        umma_commit(o_done(c & 1));
+        // S of chunk c + AHEAD goes over P of chunk c: the tensor core takes MMAs in the order of their issue
+        if (c + C::AHEAD < n_chunks) issue_s(c + C::AHEAD);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---------------- softmax and epilogue: one row per thread ----------------
+    const int quarter = warp & 3, r = quarter * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+    const int tok = tok0 + r / p.group;
+    const bool row_ok = seq >= 0 && r < p.group * p.tile_tokens && tok < nq;
+    const int limit = row_ok ? limit_of(tok) : 0;
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int c = 0; c < n_chunks && ok; ++c) {
+      const int buf = c % C::AHEAD;
+      const int lo = max(lim_min - c * 128, 0), hi = (min(lim_max - c * 128, 128) + 15) / 16 * 16;
+      if (lo < hi) {
+        // Keys that not every row sees (the causal diagonal) or that none does (behind the last key, up to the MMA's
+        // step of 16): their P is zero in the rows that do not see them, but zero times NaN or infinity is NaN.  Such
+        // values are cleared in shared memory; the epilogue gives them back to the rows that see them.
+        for (int u = 0; u < C::UNITS; ++u) {
+          const int pos = v_pos(c) + u, s = pos % C::STAGES;
+          ok = ok && __all_sync(0xffffffffu, mbar_wait(full(s), (uint32_t)(pos / C::STAGES) & 1u, abort_flag));
+          if (!ok) break;
+          const int r0 = max(lo - u * C::V_ROWS, 0), r1 = min(hi - u * C::V_ROWS, C::V_ROWS);
+          const int tail = lim_max - c * 128 - u * C::V_ROWS;      // rows from here on are seen by none
+          for (int x = 0; x < boxes; ++x) {
+            uint8_t* box = ring + s * C::SLOT_BYTES + x * C::V_ROWS * 128;
+            for (int i = r0 * 8 + r; i < r1 * 8; i += 128) {
+              uint4* at = reinterpret_cast<uint4*>(box + i * 16);
+              if (i >= tail * 8) {
+                *at = make_uint4(0u, 0u, 0u, 0u);
+                continue;
+              }
+              const uint4 w4 = *at;
+              uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+              bool bad = false;
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (lane + 32 * i < p.dim) o[lane + 32 * i] = (T)(limit > 0 ? acc[i] / l : 0.f);
+              for (int e = 0; e < 4; ++e) {
+                if ((w[e] & H::EXP_LO) == H::EXP_LO) { w[e] &= 0xffff0000u; bad = true; }
+                if ((w[e] >> 16 & H::EXP_LO) == H::EXP_LO) { w[e] &= 0xffffu; bad = true; }
+              }
+              if (bad) {
+                *at = make_uint4(w[0], w[1], w[2], w[3]);
+                *poison = 1;
+              }
+            }
+          }
+        }
+        if (!ok) break;
+        fence_proxy_async_shared();
+      }
+      ok = __all_sync(0xffffffffu, mbar_wait(s_full(buf), (uint32_t)(c / C::AHEAD) & 1u, abort_flag));
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t ts = tmem + lane_off + buf * 128;
+      float s[128];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) tmem_ld32(ts + 32 * g, reinterpret_cast<uint32_t*>(s) + 32 * g);
+      tmem_ld_wait();
+      const int vis = limit - c * 128;
+      if (!__all_sync(0xffffffffu, vis >= 128)) {
+#pragma unroll
+        for (int j = 0; j < 128; ++j)
+          if (j >= vis) s[j] = -INFINITY;
+      }
+      float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+      for (int j = 4; j < 128; ++j) mx[j & 3] = fmaxf(mx[j & 3], s[j]);
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2e;
+      // the first chunk sets the maximum; later it moves when a row of this warp has outgrown it by 2^8
+      if (__any_sync(0xffffffffu, top > m + 8.f)) {
+        const float m_new = fmaxf(m, top);
+        if (c > 0) {
+          ok = __all_sync(0xffffffffu, mbar_wait(o_done((c - 1) & 1), (uint32_t)((c - 1) >> 1) & 1u, abort_flag));
+          if (!ok) break;
+          tc_fence_after();
+          const float a = m == m_new ? 1.f : ex2_approx(m - m_new);
+          l *= a;
+#pragma unroll 1
+          for (int d = 0; d < p.dim; d += 32) {
+            uint32_t v[32];
+            tmem_ld32(tmem + lane_off + C::O_COL + d, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * a);
+            tmem_st32(tmem + lane_off + C::O_COL + d, v);
+          }
+        }
+        m = m_new;
+      }
+      const float sub = m == -INFINITY ? 0.f : m;        // a row that has seen nothing yet
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        uint32_t w[32];
+#pragma unroll
+        for (int j = 0; j < 64; j += 2) {
+          const float a = ex2_approx(fmaf(s[64 * g + j], p.scale_log2e, -sub));
+          const float b = ex2_approx(fmaf(s[64 * g + j + 1], p.scale_log2e, -sub));
+          sum[j & 2] += a;
+          sum[(j & 2) + 1] += b;
+          w[j >> 1] = H::pack(a, b);
+        }
+        tmem_st32(ts + 32 * g, w);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(p_ready(buf));
+    }
+    if (ok && n_chunks > 0) {
+      ok = __all_sync(0xffffffffu, mbar_wait(o_done((n_chunks - 1) & 1), (uint32_t)((n_chunks - 1) >> 1) & 1u, abort_flag));
+      tc_fence_after();
+    }
+    if (ok && seq >= 0) {
+      const float inv = l != 0.f ? 1.f / l : 0.f;         // nothing seen: O is zero or was never written
+      const bool any_poison = *poison != 0;
+      T* orow = reinterpret_cast<T*>(p.o) + (long long)(q0 + tok) * p.o_tok + (long long)(kvh * p.group + r % p.group) * p.o_head;
+#pragma unroll 1
+      for (int d = 0; d < p.dim; d += 32) {
+        uint32_t v[32];
+        if (n_chunks > 0) {
+          tmem_ld32(tmem + lane_off + C::O_COL + d, v);
+          tmem_ld_wait();
+        }
+        if (row_ok) {
+          float f[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) f[j] = l != 0.f ? __uint_as_float(v[j]) * inv : 0.f;
+          if (any_poison) {
+            for (int key = lim_min; key < limit; ++key) {
+              const unsigned short* vr = reinterpret_cast<const unsigned short*>(p.v) + (long long)(k0 + key) * p.v_tok + kvh * p.v_head + d;
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (d + j < p.dim && (vr[j] & H::EXP_LO) == H::EXP_LO) f[j] += H::value(vr[j]);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 32; j += 8) {
+            if (d + j < p.dim)
+              *reinterpret_cast<uint4*>(orow + d + j) = make_uint4(H::pack(f[j], f[j + 1]), H::pack(f[j + 2], f[j + 3]),
+                                                                   H::pack(f[j + 4], f[j + 5]), H::pack(f[j + 6], f[j + 7]));
+          }
+        }
+        __syncwarp();
+      }
+    }
+  }
+
+  // ---------------- teardown ----------------
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {   // a wait ran out: say so, and let copies in flight land before the shared memory goes to another CTA
+    if (threadIdx.x == 0) atomicOr(&cache_ops_status, VLA_ST_WAIT_TIMEOUT);
+    for (int i = 0; i < 32; ++i) __nanosleep(1000);
+  }
+  if (warp == 1) tmem_dealloc(tmem, C::TMEM_COLS);
 }

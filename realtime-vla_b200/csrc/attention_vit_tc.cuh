@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(VitAttnTcCfg::THREADS, 1) vit_attention_tc_ker
     }
   }
   VIT_TRACE(3);
-  fence_proxy_async_smem();   // generic-proxy stores -> visible to the tensor core's async-proxy reads
+  fence_proxy_async_shared();   // generic-proxy stores -> visible to the tensor core's async-proxy reads
   __syncthreads();
   VIT_TRACE(4);
 
@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(VitAttnTcCfg::THREADS, 1) vit_attention_tc_ker
   }
   VIT_TRACE(6);
   xchg[half * 128 + r] = l_loc;
-  fence_proxy_async_smem();
+  fence_proxy_async_shared();
   tc_fence_before();
   __syncthreads();             // P complete (and the row sums exchanged) before the MMA is issued
   const float l_tot = l_loc + xchg[(half ^ 1) * 128 + r];

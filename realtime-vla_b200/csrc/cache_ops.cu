@@ -53,6 +53,25 @@ bool vectors(const void* p, long long a, long long b) { return aligned(p, 16) &&
 
 constexpr long long INT_TOP = 0x7fffffff;
 
+// Tensor map of a 16-bit tensor, innermost dimension first (contiguous); boxes of 64 elements in 128-byte rows, swizzled.
+// The stride of a dimension of size one is free in the caller's tensor and made valid here.
+template <int N>
+bool head_map(CUtensorMap* tm, const void* base, int dtype, const long long (&dims)[N], const long long (&strides)[N - 1], const int (&box)[N]) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (!fn) return false;
+  cuuint64_t gd[N], gs[N - 1];
+  cuuint32_t bx[N], es[N];
+  for (int i = 0; i < N; ++i) {
+    gd[i] = (cuuint64_t)dims[i];
+    bx[i] = (cuuint32_t)box[i];
+    es[i] = 1;
+    if (i > 0) gs[i - 1] = dims[i] > 1 ? (cuuint64_t)strides[i - 1] * 2 : (cuuint64_t)dims[0] * 2;
+  }
+  return fn(tm, dtype == VLA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, N, const_cast<void*>(base), gd, gs, bx, es,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 }  // namespace
 
 extern "C" {
@@ -170,18 +189,44 @@ int vla_op_prompt_attention(const vla_prompt_attn_desc* d, void* stream) {
         !vectors(d->v, d->v_tok_stride, d->v_head_stride) || !vectors(d->o, d->o_tok_stride, d->o_head_stride))
       return refuse(VLA_ERR_SHAPE, "%s: rows of q, k, v and o must start on 16 bytes", who);
     PromptAttnParams p;
-    p.q = d->q; p.k = d->k; p.v = d->v; p.o = d->o; p.cu_q = d->cu_q; p.cu_k = d->cu_k;
+    p.v = d->v; p.o = d->o; p.cu_q = d->cu_q; p.cu_k = d->cu_k;
     p.n_seqs = d->n_seqs; p.tokens_q = d->tokens_q; p.tokens_k = d->tokens_k;
-    p.heads = d->heads; p.kv_heads = d->kv_heads; p.dim = d->head_dim;
-    p.q_tok = d->q_tok_stride; p.q_head = d->q_head_stride; p.k_tok = d->k_tok_stride; p.k_head = d->k_head_stride;
+    p.kv_heads = d->kv_heads; p.group = d->heads / d->kv_heads; p.dim = d->head_dim;
+    p.tile_tokens = 128 / p.group;
     p.v_tok = d->v_tok_stride; p.v_head = d->v_head_stride; p.o_tok = d->o_tok_stride; p.o_head = d->o_head_stride;
     p.causal = d->causal ? 1 : 0;
     p.scale_log2e = d->scale * 1.4426950408889634f;
+    const bool wide = d->head_dim > 128;
+    // without keys the maps are never used: any valid tensor stands in
+    const void* k = d->tokens_k ? d->k : d->q;
+    const void* v = d->tokens_k ? d->v : d->q;
+    const long long nk = std::max(d->tokens_k, 1), dim = d->head_dim;
+    const int box_v = wide ? PromptCfg<true>::V_ROWS : PromptCfg<false>::V_ROWS;
+    bool made = head_map(&p.tmQ, d->q, d->dtype, {dim, p.group, d->kv_heads, d->tokens_q}, {d->q_head_stride, p.group * d->q_head_stride, d->q_tok_stride},
+                         {64, p.group, 1, p.tile_tokens});
+    made = made && head_map(&p.tmK, k, d->dtype, {dim, d->kv_heads, nk}, {d->k_head_stride, d->k_tok_stride}, {64, 1, 128});
+    made = made && head_map(&p.tmV, v, d->dtype, {dim, d->kv_heads, nk}, {d->v_head_stride, d->v_tok_stride}, {64, 1, box_v});
+    if (!made) return refuse(VLA_ERR_SHAPE, "%s: the strides of q, k or v cannot be described by a tensor map", who);
+    const long long tiles = d->tokens_q / p.tile_tokens + d->n_seqs;     // at most one tile of each sequence is not full
+    if (tiles * d->kv_heads > INT_TOP) return refuse(VLA_ERR_LIMIT, "%s: too many tiles", who);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    const dim3 grid(d->tokens_q, (d->heads + 3) / 4);
-    auto go = [&](auto kern) { return launched(who, launch_ex(kern, grid, dim3(128), 0, st, 1, false, p)); };
-    return d->dtype == VLA_BF16 ? go(prompt_attention_kernel<bf16>) : go(prompt_attention_kernel<__half>);
+    auto go = [&](auto kern, int smem) -> int {
+      if (cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kern), smem); e != cudaSuccess) return launched(who, e);
+      return launched(who, launch_ex(kern, dim3((unsigned)(tiles * d->kv_heads)), dim3(PromptCfg<false>::THREADS), smem, st, 1, false, p));
+    };
+    if (d->dtype == VLA_BF16)
+      return wide ? go(prompt_attention_kernel<bf16, true>, PromptCfg<true>::SMEM_BYTES) : go(prompt_attention_kernel<bf16, false>, PromptCfg<false>::SMEM_BYTES);
+    return wide ? go(prompt_attention_kernel<__half, true>, PromptCfg<true>::SMEM_BYTES) : go(prompt_attention_kernel<__half, false>, PromptCfg<false>::SMEM_BYTES);
   });
+}
+
+int vla_op_cache_status(int* out) {
+  const char* who = "vla_op_cache_status";
+  if (!out) return refuse(VLA_ERR_STATE, "%s: null argument", who);
+  const int zero = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(out, cache_ops_status, sizeof(int));
+  if (e == cudaSuccess && *out) e = cudaMemcpyToSymbol(cache_ops_status, &zero, sizeof(int));
+  return launched(who, e);
 }
 
 }  // extern "C"

@@ -334,7 +334,12 @@ typedef struct vla_paged_attn_desc {
   int n_seqs, n_q, heads, kv_heads, head_dim;
   int num_blocks, block_size, width;
   float scale; int dtype;
+  void* workspace; size_t workspace_bytes;
 } vla_paged_attn_desc;
+/* Bytes of device memory (16-byte aligned) that the call needs as `workspace`, from the sizes in *d alone (pointers are not looked at);
+ * 0: none.  A workspace belongs to one call at a time: calls that can overlap on the GPU (two streams, two graphs) need
+ * one each.  It needs no clearing. */
+int vla_op_paged_attention_workspace(const vla_paged_attn_desc* d, size_t* bytes);
 int vla_op_paged_attention(const vla_paged_attn_desc* d, void* stream);
 
 /* O = softmax(scale Q K^T) V over packed prompts: q, o [tokens_q][heads][head_dim], k, v [tokens_k][kv_heads][head_dim] by

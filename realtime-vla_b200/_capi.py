@@ -67,7 +67,8 @@ CacheAppendDesc = _desc("CacheAppendDesc", (_P, "k v slots"), (_I, "tokens"),
 PagedAttnDesc = _desc("PagedAttnDesc", (_P, "q o"),
                       (_L, "q_seq_stride q_tok_stride q_head_stride o_seq_stride o_tok_stride o_head_stride"),
                       (_P, "k_codes v_codes k_scale v_scale block_table"), (_L, "table_stride"), (_P, "seq_lens"),
-                      (_I, "n_seqs n_q heads kv_heads head_dim num_blocks block_size width"), (C.c_float, "scale"), (_I, "dtype"))
+                      (_I, "n_seqs n_q heads kv_heads head_dim num_blocks block_size width"), (C.c_float, "scale"), (_I, "dtype"),
+                      (_P, "workspace"), (C.c_size_t, "workspace_bytes"))
 PromptAttnDesc = _desc("PromptAttnDesc", (_P, "q k v o cu_q cu_k"), (_I, "n_seqs tokens_q tokens_k heads kv_heads head_dim"),
                        (_L, "q_tok_stride q_head_stride k_tok_stride k_head_stride v_tok_stride v_head_stride o_tok_stride o_head_stride"),
                        (_I, "causal"), (C.c_float, "scale"), (_I, "dtype"))
@@ -108,6 +109,7 @@ EXPORTS = {
     "vla_op_attention_tc": (C.c_int, [C.POINTER(AttnTcDesc), C.c_void_p]),
     "vla_op_block_plan": (C.c_int, [C.POINTER(BlockPlanDesc), C.c_void_p]),
     "vla_op_cache_append": (C.c_int, [C.POINTER(CacheAppendDesc), C.c_void_p]),
+    "vla_op_paged_attention_workspace": (C.c_int, [C.POINTER(PagedAttnDesc), C.POINTER(C.c_size_t)]),
     "vla_op_paged_attention": (C.c_int, [C.POINTER(PagedAttnDesc), C.c_void_p]),
     "vla_op_prompt_attention": (C.c_int, [C.POINTER(PromptAttnDesc), C.c_void_p]),
     "vla_op_cache_status": (C.c_int, [C.POINTER(C.c_int)]),

@@ -4,6 +4,7 @@
 #include <algorithm>
 #include <cstdarg>
 #include <cstdio>
+#include <type_traits>
 
 #include "../../include/vla_b200.h"
 #include "attention_paged.cuh"
@@ -72,6 +73,47 @@ bool head_map(CUtensorMap* tm, const void* base, int dtype, const long long (&di
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// How the calls of vla_op_paged_attention are shared out, from the sizes that the host knows (not the lengths).
+struct PagedShape {
+  int rows, nt, row_blocks;
+  long long ctas;
+  size_t workspace;        // bytes; 0: one CTA per unit, nothing to join
+};
+PagedShape paged_shape(const vla_paged_attn_desc* d) {
+  PagedShape s;
+  const long long rows = (long long)d->n_q * (d->heads / d->kv_heads);
+  s.rows = (int)std::min(rows, INT_TOP);
+  s.nt = s.rows > 8 ? 2 : 1;
+  s.row_blocks = (int)((rows + 8 * s.nt - 1) / (8 * s.nt));
+  const long long units = (long long)d->n_seqs * d->kv_heads * s.row_blocks;
+  const long long tiles = ((long long)d->width * d->block_size + 15) / 16;      // of a unit, at most
+  if (tiles <= 2 * PAGED_MIN_TILES) {
+    s.ctas = units;
+    s.workspace = 0;
+    return s;
+  }
+  s.ctas = (long long)sm_count() * (d->head_dim == 256 ? 1 : 2);
+  if (units < s.ctas) s.ctas = std::min(s.ctas, (units * tiles + PAGED_MIN_TILES - 1) / PAGED_MIN_TILES);
+  const size_t rows_kept = (size_t)s.ctas * 2 * 8 * s.nt;
+  s.workspace = rows_kept * ((size_t)d->head_dim * sizeof(float) + sizeof(float2)) + (size_t)s.ctas * 4 * sizeof(int);
+  return s;
+}
+
+// Sizes and types of a vla_paged_attn_desc
+int paged_check(const char* who, const vla_paged_attn_desc* d) {
+  if (!d) return refuse(VLA_ERR_STATE, "%s: null descriptor", who);
+  if (d->n_seqs < 0 || d->n_q < 1 || d->heads < 1 || d->kv_heads < 1 || d->num_blocks < 1 || d->width < 0 || d->table_stride < d->width)
+    return refuse(VLA_ERR_SHAPE, "%s: bad sizes", who);
+  if (d->heads % d->kv_heads) return refuse(VLA_ERR_SHAPE, "%s: heads must be a multiple of kv_heads", who);
+  if (d->head_dim != 64 && d->head_dim != 128 && d->head_dim != 256) return refuse(VLA_ERR_SHAPE, "%s: head_dim must be 64, 128 or 256", who);
+  if (d->block_size < 16 || d->block_size % 16 || d->block_size > 256) return refuse(VLA_ERR_SHAPE, "%s: block_size must be a multiple of 16 up to 256", who);
+  if ((long long)d->width * d->block_size > INT_TOP - 16 || (long long)d->num_blocks * d->block_size > INT_TOP || (long long)d->n_q * d->heads > 1 << 20)
+    return refuse(VLA_ERR_LIMIT, "%s: more than 2^31 - 17 tokens, or 2^20 rows of a sequence", who);
+  if (d->dtype != VLA_BF16 && d->dtype != VLA_F16) return refuse(VLA_ERR_SHAPE, "%s: q must be bf16 or f16", who);
+  if (!(d->scale > 0.f) || d->scale > 3e38f) return refuse(VLA_ERR_SHAPE, "%s: scale must be positive and finite", who);
+  return VLA_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -137,25 +179,30 @@ int vla_op_cache_append(const vla_cache_append_desc* d, void* stream) {
   });
 }
 
+int vla_op_paged_attention_workspace(const vla_paged_attn_desc* d, size_t* bytes) {
+  const char* who = "vla_op_paged_attention_workspace";
+  return guarded(who, [&]() -> int {
+    if (int rc = paged_check(who, d)) return rc;
+    if (!bytes) return refuse(VLA_ERR_STATE, "%s: null argument", who);
+    *bytes = d->n_seqs ? paged_shape(d).workspace : 0;
+    return VLA_OK;
+  });
+}
+
 int vla_op_paged_attention(const vla_paged_attn_desc* d, void* stream) {
   const char* who = "vla_op_paged_attention";
   return guarded(who, [&]() -> int {
-    if (!d) return refuse(VLA_ERR_STATE, "%s: null descriptor", who);
-    if (d->n_seqs < 0 || d->n_q < 1 || d->heads < 1 || d->kv_heads < 1 || d->num_blocks < 1 || d->width < 0 || d->table_stride < d->width)
-      return refuse(VLA_ERR_SHAPE, "%s: bad sizes", who);
-    if (d->heads % d->kv_heads) return refuse(VLA_ERR_SHAPE, "%s: heads must be a multiple of kv_heads", who);
-    if (d->head_dim != 64 && d->head_dim != 128 && d->head_dim != 256) return refuse(VLA_ERR_SHAPE, "%s: head_dim must be 64, 128 or 256", who);
-    if (d->block_size < 16 || d->block_size % 16 || d->block_size > 256) return refuse(VLA_ERR_SHAPE, "%s: block_size must be a multiple of 16 up to 256", who);
-    if ((long long)d->width * d->block_size > INT_TOP || (long long)d->num_blocks * d->block_size > INT_TOP)
-      return refuse(VLA_ERR_LIMIT, "%s: more than 2^31 - 1 tokens", who);
-    if (d->dtype != VLA_BF16 && d->dtype != VLA_F16) return refuse(VLA_ERR_SHAPE, "%s: q must be bf16 or f16", who);
-    if (!(d->scale > 0.f) || d->scale > 3e38f) return refuse(VLA_ERR_SHAPE, "%s: scale must be positive and finite", who);
+    if (int rc = paged_check(who, d)) return rc;
     if (d->n_seqs == 0) return VLA_OK;
     if (!d->q || !d->o || !d->k_codes || !d->v_codes || !d->k_scale || !d->v_scale || !d->seq_lens || (d->width && !d->block_table))
       return refuse(VLA_ERR_STATE, "%s: null argument", who);
     if (!aligned(d->k_codes, 16) || !aligned(d->v_codes, 16)) return refuse(VLA_ERR_SHAPE, "%s: the cache must start on 16 bytes", who);
     if (!vectors(d->q, d->q_seq_stride, d->q_tok_stride) || d->q_head_stride % 8 || !vectors(d->o, d->o_seq_stride, d->o_tok_stride) || d->o_head_stride % 8)
       return refuse(VLA_ERR_SHAPE, "%s: rows of q and o must start on 16 bytes", who);
+    const PagedShape s = paged_shape(d);
+    if (s.ctas > INT_TOP) return refuse(VLA_ERR_LIMIT, "%s: too many sequences", who);
+    if (s.workspace && (!d->workspace || d->workspace_bytes < s.workspace || !aligned(d->workspace, 16)))
+      return refuse(VLA_ERR_STATE, "%s: a workspace of %zu bytes on a 16-byte boundary is needed", who, s.workspace);
     PagedAttnParams p;
     p.q = d->q; p.o = d->o;
     p.q_seq = d->q_seq_stride; p.q_tok = d->q_tok_stride; p.q_head = d->q_head_stride;
@@ -163,13 +210,32 @@ int vla_op_paged_attention(const vla_paged_attn_desc* d, void* stream) {
     p.kc = reinterpret_cast<const uint8_t*>(d->k_codes); p.vc = reinterpret_cast<const uint8_t*>(d->v_codes);
     p.ks = d->k_scale; p.vs = d->v_scale;
     p.table = d->block_table; p.table_ld = d->table_stride; p.lens = d->seq_lens;
-    p.n_seqs = d->n_seqs; p.n_q = d->n_q; p.heads = d->heads; p.kv_heads = d->kv_heads; p.dim = d->head_dim;
+    p.n_seqs = d->n_seqs; p.n_q = d->n_q; p.group = d->heads / d->kv_heads; p.kv_heads = d->kv_heads;
+    p.rows = s.rows; p.row_blocks = s.row_blocks;
     p.blocks = d->num_blocks; p.block = d->block_size; p.width = d->width;
     p.scale_log2e = d->scale * 1.4426950408889634f;
+    p.split = s.workspace != 0;
+    p.part_o = reinterpret_cast<float*>(d->workspace);
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + s.ctas * 2 * 8 * s.nt * d->head_dim);
+    p.cut = reinterpret_cast<int*>(p.part_ml + s.ctas * 2 * 8 * s.nt);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    const dim3 grid(d->n_seqs * d->n_q, (d->heads + 3) / 4);
-    auto go = [&](auto kern) { return launched(who, launch_ex(kern, grid, dim3(128), 0, st, 1, false, p)); };
-    return d->dtype == VLA_BF16 ? go(paged_attention_kernel<bf16>) : go(paged_attention_kernel<__half>);
+    auto go = [&](auto type, auto dim, auto nt) -> int {
+      using T = decltype(type);
+      constexpr int D = decltype(dim)::value, NT = decltype(nt)::value;
+      auto kern = paged_attention_kernel<T, D, NT>;
+      cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kern), PagedCfg<D, NT>::SMEM_BYTES);
+      if (e == cudaSuccess) e = launch_ex(kern, dim3((unsigned)s.ctas), dim3(PAGED_THREADS), PagedCfg<D, NT>::SMEM_BYTES, st, 1, false, p);
+      if (e == cudaSuccess && p.split) e = launch_ex(paged_join_kernel<T, D, NT>, dim3((unsigned)s.ctas, std::min(8 * NT, s.rows)), dim3(D), 0, st, 1, true, p);
+      return launched(who, e);
+    };
+    auto with = [&](auto type, auto dim) -> int {
+      return s.nt == 1 ? go(type, dim, std::integral_constant<int, 1>{}) : go(type, dim, std::integral_constant<int, 2>{});
+    };
+    auto by_dim = [&](auto type) -> int {
+      return d->head_dim == 64 ? with(type, std::integral_constant<int, 64>{})
+             : d->head_dim == 128 ? with(type, std::integral_constant<int, 128>{}) : with(type, std::integral_constant<int, 256>{});
+    };
+    return d->dtype == VLA_BF16 ? by_dim(bf16{}) : by_dim(__half{});
   });
 }
 

@@ -259,6 +259,11 @@ def paged_attention(q, cache, block_table, seq_lens, *, scale=None, out=None):
                             block_table.stride(0) if n > 1 else block_table.shape[1], _whole(seq_lens, "seq_lens", dev),
                             n, tokens, heads, kv_heads, dim, blocks, block, block_table.shape[1],
                             dim ** -0.5 if scale is None else scale, _DTYPES[t])
+    need = C.c_size_t()
+    _capi.check(_capi.lib().vla_op_paged_attention_workspace(C.byref(d), C.byref(need)))
+    if need.value:
+        space = torch.empty(need.value, dtype=torch.uint8, device=dev)     # this call's own: the allocator orders its reuse
+        d.workspace, d.workspace_bytes = space.data_ptr(), need.value
     _enqueue(_capi.lib().vla_op_paged_attention, d, dev)
     return out
 

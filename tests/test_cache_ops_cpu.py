@@ -63,7 +63,7 @@ CASES = [
         (SHAPE, dict(heads=7)), (SHAPE, dict(heads=0)), (SHAPE, dict(kv_heads=0)), (SHAPE, dict(n_q=0)), (SHAPE, dict(head_dim=72)),
         (SHAPE, dict(block_size=24)), (SHAPE, dict(dtype=_capi.VLA_F32)), (SHAPE, dict(scale=0.0)), (SHAPE, dict(scale=float("nan"))),
         (SHAPE, dict(scale=float("inf"))), (SHAPE, dict(q=P + 8)), (SHAPE, dict(o_head_stride=4)), (SHAPE, dict(table_stride=3)),
-        (SHAPE, dict(num_blocks=0)), (LIMIT, dict(width=2 ** 28, table_stride=2 ** 28))]),
+        (SHAPE, dict(num_blocks=0)), (LIMIT, dict(n_q=2 ** 20)), (LIMIT, dict(width=2 ** 28, table_stride=2 ** 28))]),
     ("vla_op_prompt_attention", prompt_desc, [
         (STATE, dict(q=None)), (STATE, dict(v=None)), (STATE, dict(cu_k=None)), (STATE, dict(o=None)), (SHAPE, dict(heads=3)),
         (SHAPE, dict(head_dim=4)), (SHAPE, dict(head_dim=264)), (SHAPE, dict(head_dim=100)), (SHAPE, dict(tokens_q=-1)), (SHAPE, dict(n_seqs=-2)),
@@ -76,6 +76,21 @@ CASES = [
 def test_entry_points_refuse(name, make, code, change):
     rc, text = call(name, make(**change))
     assert rc == code and name in text
+
+
+@needs_library
+def test_paged_workspace():
+    """Nothing where one CTA does a unit; else what the sizes ask for, and the call refuses less or none."""
+    need = C.c_size_t(1)
+    f = _capi.lib().vla_op_paged_attention_workspace
+    assert f(C.byref(paged_desc()), C.byref(need)) == 0 and need.value == 0
+    long = paged_desc(width=200, table_stride=200)
+    assert f(C.byref(long), C.byref(need)) == 0 and need.value > 0
+    for kw in (dict(), dict(workspace=P, workspace_bytes=need.value - 1), dict(workspace=P + 4, workspace_bytes=need.value)):
+        rc, text = call("vla_op_paged_attention", paged_desc(width=200, table_stride=200, **kw))
+        assert rc == STATE and "workspace" in text
+    assert f(C.byref(paged_desc(heads=7)), C.byref(need)) == SHAPE
+    assert f(None, C.byref(need)) == STATE and f(C.byref(long), None) == STATE
 
 
 @needs_library

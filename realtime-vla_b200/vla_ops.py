@@ -5,6 +5,7 @@ The operators around a key/value cache in pages (block_plan, cache_append, paged
 programs that serve sequences of different lengths: they take torch tensors, enqueue on the current stream of the tensors'
 device and return without synchronising, so they can be captured into a CUDA graph.  They run forward only."""
 import ctypes as C
+import functools
 from typing import NamedTuple
 
 import torch
@@ -143,39 +144,59 @@ def kv_cache(blocks, kv_heads, block_size, head_dim, device=None):
     return KvCache(*codes, *scales)
 
 
-def _refuse(cond, text):
-    if cond:
-        raise _capi.VlaError("vla_ops: " + text)
+# The checks below run on every call of operators that take a few microseconds, so messages are formed only on refusal.
+def _refuse(text, *args):
+    raise _capi.VlaError("vla_ops: " + text % args)
+
+
+def _tell(t):
+    return "%s %s on %s" % (t.dtype, tuple(t.shape), t.device)
+
+
+def _on_gpu(t, name):
+    if not t.is_cuda:
+        _refuse("%s must be on a GPU; there is no CPU path", name)
+    return t.device
 
 
 def _whole(t, name, device, dim=1):
-    """int32 tensor of `dim` dimensions on `device`, rows contiguous."""
-    _refuse(t.dtype != torch.int32 or t.dim() != dim, "%s must be int32 with %d dimension(s), got %s %s" % (name, dim, t.dtype, tuple(t.shape)))
-    _refuse(t.device != device, "%s is on %s, not on %s" % (name, t.device, device))
-    _refuse(t.shape[-1] > 1 and t.stride(-1) != 1, "%s must be contiguous" % name)
+    """Address of an int32 tensor of `dim` dimensions on `device` with contiguous rows."""
+    if t.dtype is not torch.int32 or t.dim() != dim or t.device != device or (t.stride(-1) != 1 and t.shape[-1] > 1):
+        _refuse("%s must be int32 with %d dimension(s), contiguous rows, on %s; got %s", name, dim, device, _tell(t))
     return t.data_ptr()
 
 
 def _rows(t, name, device, dtype, dim):
-    _refuse(t.dtype != dtype or t.dim() != dim or t.device != device,
-            "%s must be %s with %d dimensions on %s, got %s %s on %s" % (name, dtype, dim, device, t.dtype, tuple(t.shape), t.device))
-    _refuse(t.stride(-1) != 1 and t.shape[-1] > 1, "the last dimension of %s must be contiguous" % name)
-    _refuse(t.requires_grad and torch.is_grad_enabled(), "%s requires a gradient; this operator has no backward pass" % name)
+    """Address of a 16-bit tensor of `dim` dimensions on `device` whose last one is contiguous."""
+    if t.dtype is not dtype or t.dim() != dim or t.device != device or (t.stride(-1) != 1 and t.shape[-1] > 1):
+        _refuse("%s must be %s with %d dimensions, the last one contiguous, on %s; got %s", name, dtype, dim, device, _tell(t))
+    if t.requires_grad and torch.is_grad_enabled():
+        _refuse("%s requires a gradient; this operator has no backward pass", name)
     return t.data_ptr()
 
 
 def _cache(cache, device):
     k, v, ks, vs = cache
-    _refuse(k.dim() != 4 or k.shape != v.shape or ks.shape != k.shape[:2] or vs.shape != ks.shape, "cache tensors do not fit each other")
-    _refuse(k.dtype != torch.float8_e4m3fn or v.dtype != k.dtype or ks.dtype != torch.float32 or vs.dtype != ks.dtype,
-            "a cache is held as float8_e4m3fn with float32 scales")
+    if k.dim() != 4 or k.shape != v.shape or ks.shape != k.shape[:2] or vs.shape != ks.shape:
+        _refuse("the tensors of the cache do not fit each other: %s, %s, %s, %s", *map(_tell, cache))
+    f8, f32 = torch.float8_e4m3fn, torch.float32
+    if k.dtype is not f8 or v.dtype is not f8 or ks.dtype is not f32 or vs.dtype is not f32:
+        _refuse("a cache is held as float8_e4m3fn with float32 scales: %s, %s, %s, %s", *map(_tell, cache))
     for t in cache:
-        _refuse(t.device != device or not t.is_contiguous(), "cache tensors must be contiguous and on %s" % device)
+        if t.device != device or not t.is_contiguous():
+            _refuse("the tensors of the cache must be contiguous and on %s; got %s", device, _tell(t))
     return k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr()
 
 
+def _type(t, name):
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        _refuse("%s must be bfloat16 or float16, got %s", name, t.dtype)
+    return code
+
+
 def _enqueue(fn, desc, device):
-    stream = C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    stream = torch.cuda.current_stream(device).cuda_stream
     if torch.cuda.current_device() == device.index:
         rc = fn(C.byref(desc), stream)
     else:
@@ -183,11 +204,6 @@ def _enqueue(fn, desc, device):
             rc = fn(C.byref(desc), stream)
     if rc:
         _capi.check(rc)
-
-
-def _on_gpu(t, name):
-    _refuse(not t.is_cuda, "%s must be on a GPU; there is no CPU path" % name)
-    return t.device
 
 
 def block_plan(context_lens, new_lens, block_table, free_blocks, *, block_size, total_new, first_free=None):
@@ -199,20 +215,18 @@ def block_plan(context_lens, new_lens, block_table, free_blocks, *, block_size, 
     batch).  Returns a BlockPlan; counts[1] > 0 says that blocks were missing and some tokens have slot -1."""
     dev = _on_gpu(context_lens, "context_lens")
     n = context_lens.shape[0]
-    _refuse(new_lens.shape[0] != n or block_table.shape[0] != n, "context_lens, new_lens and block_table do not fit each other")
-    _refuse(first_free is not None and first_free.numel() != 1, "first_free must hold one number")
-    rows = (total_new + 3) // 4 * 4       # each part of the one allocation starts on 16 bytes
-    seqs = (n + 4) // 4 * 4
-    out = torch.empty(2 * rows + 2 * seqs + 4, dtype=torch.int32, device=dev)
-    slots, positions = out[:total_new], out[rows:rows + total_new]
-    cu, lens, counts = out[2 * rows:2 * rows + n + 1], out[2 * rows + seqs:2 * rows + seqs + n], out[2 * rows + 2 * seqs:2 * rows + 2 * seqs + 3]
-    base = out.data_ptr()
+    if new_lens.shape[0] != n or block_table.shape[0] != n or (first_free is not None and first_free.numel() != 1):
+        _refuse("context_lens, new_lens, block_table (and first_free) do not fit each other")
+    if total_new < 0:
+        _refuse("total_new is negative")
+    make = context_lens.new_empty
+    slots, positions, cu, lens, counts = make(total_new), make(total_new), make(n + 1), make(n), make(3)
     d = _capi.BlockPlanDesc(_whole(context_lens, "context_lens", dev), _whole(new_lens, "new_lens", dev), n,
                             _whole(block_table, "block_table", dev, 2), block_table.shape[1],
                             block_table.stride(0) if n > 1 else block_table.shape[1],
                             _whole(free_blocks, "free_blocks", dev), free_blocks.shape[0],
                             None if first_free is None else _whole(first_free, "first_free", dev), block_size, total_new,
-                            base, base + 4 * rows, base + 8 * rows, base + 8 * rows + 4 * seqs, base + 8 * rows + 8 * seqs)
+                            slots.data_ptr(), positions.data_ptr(), cu.data_ptr(), lens.data_ptr(), counts.data_ptr())
     _enqueue(_capi.lib().vla_op_block_plan, d, dev)
     return BlockPlan(slots, positions, cu, lens, counts)
 
@@ -223,16 +237,26 @@ def cache_append(k, v, cache, slots):
     Slots outside the cache are skipped; the tokens of one block must be consecutive rows.  A block whose first slot is written
     starts anew; another block's scale grows where the new tokens need it and its codes are rounded again."""
     dev = _on_gpu(k, "k")
-    t = k.dtype
-    _refuse(t not in _DTYPES, "k and v must be bfloat16 or float16, got %s" % t)
+    code = _type(k, "k")
     codes = _cache(cache, dev)
     blocks, heads, block, dim = cache.k.shape
-    pk, pv = _rows(k, "k", dev, t, 3), _rows(v, "v", dev, t, 3)
-    _refuse(k.shape != v.shape or k.shape[1:] != (heads, dim) or slots.shape[0] != k.shape[0],
-            "k %s, v %s and slots %s do not fit the cache %s" % (tuple(k.shape), tuple(v.shape), tuple(slots.shape), tuple(cache.k.shape)))
-    d = _capi.CacheAppendDesc(pk, pv, _whole(slots, "slots", dev), k.shape[0], k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-                              *codes, blocks, heads, block, dim, _DTYPES[t])
+    pk, pv = _rows(k, "k", dev, k.dtype, 3), _rows(v, "v", dev, k.dtype, 3)
+    if k.shape != v.shape or k.shape[1:] != (heads, dim) or slots.shape[0] != k.shape[0]:
+        _refuse("k %s, v %s and slots %s do not fit the cache %s", *(tuple(x.shape) for x in (k, v, slots, cache.k)))
+    d = _capi.CacheAppendDesc(pk, pv, _whole(slots, "slots", dev), k.shape[0], *k.stride()[:2], *v.stride()[:2],
+                              *codes, blocks, heads, block, dim, code)
     _enqueue(_capi.lib().vla_op_cache_append, d, dev)
+
+
+@functools.lru_cache(maxsize=1024)
+def _paged_workspace(device, *sizes):
+    """Bytes of workspace, which follow from the sizes (and the device's number of SMs)."""
+    d, need = _capi.PagedAttnDesc(), C.c_size_t()
+    d.n_seqs, d.n_q, d.heads, d.kv_heads, d.head_dim, d.num_blocks, d.block_size, d.width = sizes
+    d.table_stride, d.scale = d.width, 1.0
+    with torch.cuda.device(device):
+        _capi.check(_capi.lib().vla_op_paged_attention_workspace(C.byref(d), C.byref(need)))
+    return need.value
 
 
 def paged_attention(q, cache, block_table, seq_lens, *, scale=None, out=None):
@@ -242,28 +266,27 @@ def paged_attention(q, cache, block_table, seq_lens, *, scale=None, out=None):
     each sees itself and what is before it.  block_table int32 [n, width], seq_lens int32 [n].  scale: head_dim ** -0.5
     unless given.  Returns out, or a new tensor like q; a row that sees nothing is zero."""
     dev = _on_gpu(q, "q")
-    t = q.dtype
-    _refuse(t not in _DTYPES, "q must be bfloat16 or float16, got %s" % t)
+    code = _type(q, "q")
     codes = _cache(cache, dev)
     blocks, kv_heads, block, dim = cache.k.shape
-    pq = _rows(q, "q", dev, t, 4)
+    pq = _rows(q, "q", dev, q.dtype, 4)
     n, tokens, heads, _ = q.shape
-    _refuse(q.shape[3] != dim or block_table.shape[0] != n or seq_lens.shape[0] != n,
-            "q %s, block_table %s, seq_lens %s and cache %s do not fit each other" % (
-                tuple(q.shape), tuple(block_table.shape), tuple(seq_lens.shape), tuple(cache.k.shape)))
+    if q.shape[3] != dim or block_table.shape[0] != n or seq_lens.shape[0] != n:
+        _refuse("q %s, block_table %s, seq_lens %s and cache %s do not fit each other",
+                *(tuple(x.shape) for x in (q, block_table, seq_lens, cache.k)))
     if out is None:
-        out = torch.empty(q.shape, dtype=t, device=dev)
-    po = _rows(out, "out", dev, t, 4)
-    _refuse(out.shape != q.shape, "out must have the shape of q")
-    d = _capi.PagedAttnDesc(pq, po, *q.stride()[:3], *out.stride()[:3], *codes, _whole(block_table, "block_table", dev, 2),
-                            block_table.stride(0) if n > 1 else block_table.shape[1], _whole(seq_lens, "seq_lens", dev),
-                            n, tokens, heads, kv_heads, dim, blocks, block, block_table.shape[1],
-                            dim ** -0.5 if scale is None else scale, _DTYPES[t])
-    need = C.c_size_t()
-    _capi.check(_capi.lib().vla_op_paged_attention_workspace(C.byref(d), C.byref(need)))
-    if need.value:
-        space = torch.empty(need.value, dtype=torch.uint8, device=dev)     # this call's own: the allocator orders its reuse
-        d.workspace, d.workspace_bytes = space.data_ptr(), need.value
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif out.shape != q.shape:
+        _refuse("out must have the shape of q")
+    table = _whole(block_table, "block_table", dev, 2)
+    width = block_table.shape[1]
+    need = _paged_workspace(dev, n, tokens, heads, kv_heads, dim, blocks, block, width)
+    # the workspace is this call's own; the allocator orders its reuse on the stream
+    space = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    d = _capi.PagedAttnDesc(pq, _rows(out, "out", dev, q.dtype, 4), *q.stride()[:3], *out.stride()[:3], *codes, table,
+                            block_table.stride(0) if n > 1 else width, _whole(seq_lens, "seq_lens", dev),
+                            n, tokens, heads, kv_heads, dim, blocks, block, width, dim ** -0.5 if scale is None else scale, code,
+                            space.data_ptr() if need else None, need)
     _enqueue(_capi.lib().vla_op_paged_attention, d, dev)
     return out
 
@@ -276,20 +299,21 @@ def prompt_attention(q, k, v, cu_q, cu_k=None, *, causal=True, scale=None, out=N
     of a sequence sees all its keys, each row before it one less; otherwise every row sees all.  Returns out, or a new
     tensor like q; a row that sees nothing is zero, rows behind the last sequence are not written."""
     dev = _on_gpu(q, "q")
+    code = _type(q, "q")
+    if cu_k is None:
+        cu_k = cu_q
     t = q.dtype
-    _refuse(t not in _DTYPES, "q, k and v must be bfloat16 or float16, got %s" % t)
-    cu_k = cu_q if cu_k is None else cu_k
     pq, pk, pv = _rows(q, "q", dev, t, 3), _rows(k, "k", dev, t, 3), _rows(v, "v", dev, t, 3)
-    _refuse(k.shape != v.shape or k.shape[2] != q.shape[2] or cu_q.shape != cu_k.shape or cu_q.shape[0] < 1,
-            "q %s, k %s, v %s, cu_q %s and cu_k %s do not fit each other" % (
-                tuple(q.shape), tuple(k.shape), tuple(v.shape), tuple(cu_q.shape), tuple(cu_k.shape)))
-    if out is None:
-        out = torch.empty(q.shape, dtype=t, device=dev)
-    po = _rows(out, "out", dev, t, 3)
-    _refuse(out.shape != q.shape, "out must have the shape of q")
     tokens, heads, dim = q.shape
-    d = _capi.PromptAttnDesc(pq, pk, pv, po, _whole(cu_q, "cu_q", dev), _whole(cu_k, "cu_k", dev), cu_q.shape[0] - 1, tokens,
-                             k.shape[0], heads, k.shape[1], dim, *q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *out.stride()[:2],
-                             1 if causal else 0, dim ** -0.5 if scale is None else scale, _DTYPES[t])
+    if k.shape != v.shape or k.shape[2] != dim or cu_q.shape != cu_k.shape or cu_q.shape[0] < 1:
+        _refuse("q %s, k %s, v %s, cu_q %s and cu_k %s do not fit each other", *(tuple(x.shape) for x in (q, k, v, cu_q, cu_k)))
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif out.shape != q.shape:
+        _refuse("out must have the shape of q")
+    d = _capi.PromptAttnDesc(pq, pk, pv, _rows(out, "out", dev, t, 3), _whole(cu_q, "cu_q", dev), _whole(cu_k, "cu_k", dev),
+                             cu_q.shape[0] - 1, tokens, k.shape[0], heads, k.shape[1], dim,
+                             *q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *out.stride()[:2],
+                             1 if causal else 0, dim ** -0.5 if scale is None else scale, code)
     _enqueue(_capi.lib().vla_op_prompt_attention, d, dev)
     return out

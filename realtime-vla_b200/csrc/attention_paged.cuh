@@ -2,27 +2,32 @@
 // layout in cache_pages.cuh).  q[b][i] is token lens[b] - n + i of sequence b and sees the keys j <= lens[b] - n + i; key j is
 // row j % block of page table[b][j / block].  A page id outside the cache is not seen.  A row that sees nothing is zero.
 //
-// Bound by the bytes of the cache: each code is read once and used by the n * heads / kv_heads rows that share it.
-// Codes become fp16 without rounding (e4m3 has 4 bits of significand and 2^-9 .. 448 for a range), so the products run on
-// mma.m16n8k16 with fp16 operands and fp32 sums; at 8 rows per key the tensor work is a few per cent of what even
-// that path can do while the codes stream in.  Keys and values are the 16-wide operand (tokens, then head dims), the rows
-// the 8-wide one, so that 8 rows, the heads of the Gemma prefix, leave nothing idle:
-//     S^T[16 tokens x 8 rows]  = K . Q^T          O^T[head dims x 8 rows] += s_v (V^T . P^T)
-// The page's scale of K multiplies S, that of V the product's fp32 result, both after the sums.
-// A warp works alone on tiles of 16 tokens (never more than one page) with cp.async into its own ring of tiles; the 8
-// warps of a CTA take the tiles of a unit in turn and join their sums at its end.
+// Bound by the bytes of the cache: each code is read once, for the n * heads / kv_heads rows that share it.  The codes go
+// from TMA straight into tcgen05.mma (kind f8f6f4), so no thread ever touches one; what the threads do is the softmax of
+// 8 or 16 numbers per token.  For that, the other operand has to be e4m3 as well, without losing what bf16 or fp16
+// hold: Q and P are each split into three e4m3 numbers, x = x0 + x1 / 16 + x2 / 256, each the rounding of what is left
+// (4 bits a piece, 12 bits in all).  The pieces are further columns of the MMA's N side, which costs nothing that counts:
+//     S[128 tokens x 3R]      = K_tile . (Q0 Q1 Q2)^T       A = K tile, K-major;    R = 8 NT rows
+//     O[128 head dims x 3R]  += V_tile^T . (P0 P1 P2)       A = V tile, MN-major: as the page lies in memory
+// The page's scale of K multiplies S.  That of V goes into the exponent: w = 2^(s + log2 s_v - M), with M the running
+// maximum of that sum, and the softmax's own sum gets w / s_v; so pages of any scales add up in one accumulator, and P
+// has its 12 bits relative to the largest contribution.
 //
-// A unit is (sequence, kv head, block of 8 NT rows).  With few or long sequences the tiles of all units are laid out in one
-// line and cut into equal pieces, one per CTA, whatever the lengths; a unit cut by a piece's border leaves partial sums in
-// the workspace, which a second kernel joins in a fixed order.
+// A unit is (sequence, kv head, block of R rows).  All units are laid out in one line, by groups of 16 tokens with a gap
+// for a unit's fixed cost, and the line is cut into equal pieces, one per CTA, whatever the lengths.  A unit cut by a
+// piece's border leaves partial sums in the workspace, which a second kernel joins in a fixed order.
+// Roles, all walking the same piece on their own: warp 0 pages and TMA, warp 1 MMA, warp 2 Q pieces of the next unit, warps
+// 3..6 softmax, one token (and, at a unit's end, one head dim) per thread.  All mbarrier waits are bounded.  Code that
+// runs once per unit is kept in loops: run straight through, it costs about 8 clocks an instruction to fetch.
 #pragma once
 #include "cache_pages.cuh"
 
 struct PagedAttnParams {
+  CUtensorMap tmK;       // codes [blocks][kv heads * block][head dim], box of `box_rows` rows x 128 (64) bytes
+  CUtensorMap tmV;
   const void* q;
   void* o;
   long long q_seq, q_tok, q_head, o_seq, o_tok, o_head;
-  const uint8_t* kc;
   const uint8_t* vc;
   const float* ks;
   const float* vs;
@@ -31,527 +36,816 @@ struct PagedAttnParams {
   const int* lens;
   int n_seqs, n_q, group, kv_heads;
   int rows;              // n_q * group
-  int row_blocks;        // ceil(rows / (8 NT))
+  int row_blocks;        // ceil(rows / R)
+  int units;             // per sequence: kv_heads * row_blocks
+  uint32_t per_page_inv; // ceil(2^32 / (block / 16)), 0 for blocks of 16: see page_of
   int blocks, block, width;
+  int box_rows;          // 16, 32, 64 or 128 tokens: the largest that divides the block
   float scale_log2e;
-  int split;             // 0: CTA c does unit c; 1: pieces of the line of tiles
-  float* part_o;         // [cta][2][8 NT][D]: sums of a unit's first piece (slot 1) or a later one (slot 0)
-  float2* part_ml;       // [cta][2][8 NT]: maximum and sum
-  int* cut;              // [cta][4]: the unit that starts in this CTA and ends in another: sequence (-1: none), rest, last CTA
+  int whole;             // units are short: pieces are cut between units only, nothing to join
+  float* part_o;         // [cta][2][R][D]: sums of a unit's first part (slot 1) or a later one (slot 0)
+  float2* part_ml;       // [cta][2][R]: maximum and sum
+  int* cut;              // [cta][4]: the unit that starts in this CTA and ends in another: sequence (-1: none), kv head, row block, last CTA
 };
 
-constexpr int PAGED_THREADS = 256;
-constexpr int PAGED_WARPS = PAGED_THREADS / 32;
-constexpr int PAGED_MIN_TILES = 16;      // tiles per CTA, at least
+constexpr int PAGED_THREADS = 224;
+constexpr int PAGED_GAP = 12;            // fixed cost of a unit, in groups of 16 tokens
+constexpr int PAGED_MIN_PIECE = 8;       // groups (with gaps) per CTA, at least
+constexpr int PAGED_WHOLE = 32;          // units of at most this many groups are not cut
 
 template <int D, int NT>
 struct PagedCfg {
-  static constexpr int TILE_BYTES = 16 * D;                            // of K, and of V
-  static constexpr int STAGES = D == 64 ? 4 : 3;
-  static constexpr int RING_BYTES = PAGED_WARPS * STAGES * 2 * TILE_BYTES;
-  static constexpr int RSTRIDE = D + 8;                                // floats per row of a warp's sums
-  static constexpr int JOIN_BYTES = PAGED_WARPS * 8 * NT * RSTRIDE * 4;   // over the ring, once its tiles are used up
-  static constexpr int Q_BYTES = 8 * NT * D * 2;
-  static constexpr int KSTEPS = D / 16;
-  static constexpr bool Q_REGS = D * NT <= 128 || (D == 256 && NT == 1);
+  static constexpr int R = 8 * NT;                    // rows of a unit
+  static constexpr int N = NT == 1 ? 32 : 48;         // MMA columns: three pieces of R rows, a multiple of 16
+  static constexpr int HALVES = D == 256 ? 2 : 1;     // 128-byte column blocks of a tile
+  static constexpr int ROW_BYTES = D == 64 ? 64 : 128;
+  static constexpr int TILE_BYTES = 128 * D;          // 128 tokens of K, or of V
+  static constexpr int BLOCK_BYTES = 128 * ROW_BYTES; // one column block of a tile
+  static constexpr int SLOTS = D == 64 ? 10 : 6;      // ring of tiles: K and V in turn, each with barriers of its own
+  static constexpr int Q_BUFS = D == 128 && NT == 2 ? 1 : 2;
+  static constexpr int Q_BYTES = N * D;
+  static constexpr int P_BYTES = N * 128;
+  static constexpr int SMEM_BYTES = SLOTS * TILE_BYTES + Q_BUFS * Q_BYTES + P_BYTES + 1024;
   static constexpr int PER_SM = D == 256 ? 1 : 2;
-  static constexpr int BODY_BYTES = RING_BYTES > JOIN_BYTES ? RING_BYTES : JOIN_BYTES;
-  static constexpr int SMEM_BYTES = BODY_BYTES + Q_BYTES;
+  static constexpr int S_COL = 0, O_COL = 2 * N;      // two S buffers, then O per column block
+  static constexpr int TMEM_COLS = NT == 1 ? 128 : 256;
+  static constexpr uint64_t LAYOUT = D == 64 ? 4ull : 2ull;                 // 64- or 128-byte swizzle
+  static constexpr uint64_t GROUP_STRIDE = 8 * ROW_BYTES;                   // bytes from 8 rows to the next 8
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
-  const int n = on ? 16 : 0;             // nothing is read where n is 0; the 16 bytes become zeros
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ uint2 lds64(uint32_t a) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
-  return v;
-}
-// two e4m3 codes -> two fp16 values, exact
-__device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t two) {
-  uint32_t h;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)two));
-  return h;
-}
-__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
-  uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
-  return d;
-}
-__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}"
+      ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
 }
-// Byte of 16-byte piece c of row r in a tile of rows of D bytes.  The pieces of a row are exchanged so that the K reads (8
-// rows, every second piece) and the V reads (every second row, 8 pieces) of a warp hit distinct banks.
-template <int D>
-__device__ __forceinline__ int tile_at(int r, int c) {
-  return D == 64 ? r * D + ((c ^ (r >> 1 & 3)) << 4) : r * D + (((c & ~7) | ((c ^ r) & 7)) << 4);
+__device__ __forceinline__ uint64_t paged_desc(uint32_t smem_addr, uint64_t lead_bytes, uint64_t stride_bytes, uint64_t layout) {
+  return (uint64_t)((smem_addr & 0x3FFFF) >> 4) | (lead_bytes >> 4) << 16 | (stride_bytes >> 4) << 32 | 1ull << 46 | layout << 61;
 }
-__device__ __forceinline__ bool has_nan(uint32_t w) {   // any of four e4m3 codes is 0x7f or 0xff
-  return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
+// The three pieces of 8 rows in one lane: columns 0 .. 7 of each of three blocks of `apart` columns.
+__device__ __forceinline__ void paged_tmem_ld(uint32_t taddr, int apart, uint32_t (&v)[24]) {
+#pragma unroll
+  for (int i = 0; i < 3; ++i)
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v[8 * i]), "=r"(v[8 * i + 1]), "=r"(v[8 * i + 2]), "=r"(v[8 * i + 3]), "=r"(v[8 * i + 4]), "=r"(v[8 * i + 5]),
+                   "=r"(v[8 * i + 6]), "=r"(v[8 * i + 7])
+                 : "r"(taddr + i * apart)
+                 : "memory");
+  tmem_ld_wait();
+}
+__device__ __forceinline__ void paged_tmem_st(uint32_t taddr, int apart, const uint32_t (&v)[24]) {
+#pragma unroll
+  for (int i = 0; i < 3; ++i)
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"r"(taddr + i * apart), "r"(v[8 * i]), "r"(v[8 * i + 1]), "r"(v[8 * i + 2]), "r"(v[8 * i + 3]), "r"(v[8 * i + 4]),
+                   "r"(v[8 * i + 5]), "r"(v[8 * i + 6]), "r"(v[8 * i + 7])
+                 : "memory");
+  tmem_st_wait();
+}
+// the number that three pieces stand for
+__device__ __forceinline__ float paged_sum(const uint32_t (&v)[24], int r) {
+  return fmaf(__uint_as_float(v[16 + r]), 0x1p-8f, fmaf(__uint_as_float(v[8 + r]), 0x1p-4f, __uint_as_float(v[r])));
+}
+// mbar_wait with its loop out of line: a kernel of many roles has many waits, and its code has to stay in the caches
+__device__ __noinline__ bool paged_wait_loop(uint32_t bar, uint32_t parity, volatile int* abort_flag) { return mbar_wait(bar, parity, abort_flag); }
+__device__ __forceinline__ bool paged_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  return mbar_try_wait(bar, parity) || paged_wait_loop(bar, parity, abort_flag);
+}
+// whether `on` holds in any of the 128 threads that meet at named barrier `id`
+__device__ __forceinline__ bool barrier_any(int id, bool on) {
+  uint32_t any;
+  asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 q, %1, 0;\n barrier.cta.red.or.pred p, %2, 128, q;\n selp.u32 %0, 1, 0, p;\n}"
+               : "=r"(any) : "r"((uint32_t)on), "r"(id) : "memory");
+  return any != 0;
+}
+// largest value of a warp's lanes
+__device__ __forceinline__ float warp_max_f32(float x) {
+  float y;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float lg2_approx(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Three e4m3 pieces of two numbers of at most 256: a in the low bytes of c[], b in the high ones.
+__device__ __forceinline__ void pieces(float a, float b, uint32_t (&c)[3]) {
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    c[i] = to_e4m3x2(a, b);
+    const float2 f = from_e4m3x2(c[i]);
+    a = (a - f.x) * 16.f;
+    b = (b - f.y) * 16.f;
+  }
+}
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {   // 0x80 in the bytes that are 0x7f or 0xff
+  return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
 }
 
 __device__ __forceinline__ int paged_len(const PagedAttnParams& p, int b) {
   return (int)min(max((long long)p.lens[b], 0ll), (long long)p.width * p.block);
 }
-__device__ __forceinline__ int paged_tiles(const PagedAttnParams& p, int b) { return (paged_len(p, b) + 15) / 16; }
-
+// The page of a sequence that group g of 16 tokens lies in, g / (block / 16): with at most 16 groups a page and g below 2^27,
+// the product's error stays below 1 / 32, less than a step of the quotient.
+__device__ __forceinline__ int page_of(const PagedAttnParams& p, int g) { return p.per_page_inv ? (int)__umulhi((uint32_t)g, p.per_page_inv) : g; }
 // where row rr of (sequence b, kv head h) lies in q / o
 __device__ __forceinline__ long long paged_row(const PagedAttnParams& p, int b, int h, int rr, long long seq, long long tok, long long head) {
   return b * seq + (rr / p.group) * tok + (long long)(h * p.group + rr % p.group) * head;
 }
 
 // Sums over the CTA's threads before this one, and over all of them.
-__device__ __forceinline__ long long block_scan(long long v, long long* all, long long* warp_sum) {
+__device__ __forceinline__ int paged_scan(int v, int* all, int* warp_sum) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long s = v;
+  int s = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long u = __shfl_up_sync(0xffffffffu, s, o);
+    const int u = __shfl_up_sync(0xffffffffu, s, o);
     if (lane >= o) s += u;
   }
   if (lane == 31) warp_sum[warp] = s;
   __syncthreads();
-  long long before = 0, total = 0;
+  int before = 0, total = 0;
 #pragma unroll
-  for (int w = 0; w < PAGED_WARPS; ++w) {
-    if (w < warp) before += warp_sum[w];
-    total += warp_sum[w];
+  for (int w = 0; w < PAGED_THREADS / 32; ++w) {
+    const int n = warp_sum[w];
+    if (w < warp) before += n;
+    total += n;
   }
   __syncthreads();
   *all = total;
   return before + s - v;
 }
 
+// The parts of units in one piece of the line, in order.  Every role walks on its own; the state is a few registers.  The
+// host refuses sizes whose line could pass 2^31.
+struct PagedWalk {
+  int begin, end;        // the piece
+  int at, next_at;       // line position of the unit's first tile, and of the next unit's gap
+  int next_b, next_h, next_rb, len;
+  int b, h, rb, t0, t1, tiles;   // the part at hand: tiles [t0, t1) of `tiles` of row block rb of kv head h of sequence b
+
+  __device__ __forceinline__ bool next(const PagedAttnParams& p) {
+#pragma unroll 1
+    while (next_at < end) {
+      const int groups = (len + 15) >> 4;
+      if (next_h == p.kv_heads || !groups) {   // the line goes on, so there is a further sequence with tokens
+        next_h = 0;
+        len = paged_len(p, ++next_b);
+        continue;
+      }
+      b = next_b;
+      h = next_h;
+      rb = next_rb;
+      if (++next_rb == p.row_blocks) {
+        next_rb = 0;
+        ++next_h;
+      }
+      at = next_at + PAGED_GAP;
+      next_at = at + groups;
+      tiles = (groups + 7) >> 3;
+      // a border inside a tile belongs to the piece where the tile starts
+      t0 = cut(p, begin);
+      t1 = cut(p, end);
+      if (t0 < t1) return true;
+    }
+    return false;
+  }
+  __device__ __forceinline__ int cut(const PagedAttnParams& p, int x) const { return x <= at ? 0 : p.whole ? tiles : min(tiles, (x - at + 7) >> 3); }
+};
+
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) paged_attention_kernel(const PagedAttnParams p) {
+__global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) paged_attention_kernel(const __grid_constant__ PagedAttnParams p) {
   using C = PagedCfg<D, NT>;
-  constexpr int ROWS = 8 * NT;
-  extern __shared__ __align__(128) uint8_t paged_smem[];
-  float* join = reinterpret_cast<float*>(paged_smem);
-  uint2* q_frag = reinterpret_cast<uint2*>(paged_smem + C::BODY_BYTES);   // [NT][KSTEPS][32]
-  __shared__ float q_scale[ROWS];
-  __shared__ float2 warp_ml[PAGED_WARPS][ROWS];
-  __shared__ long long warp_sum[PAGED_WARPS];
-  __shared__ int found_b;
-  __shared__ long long found_base;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const uint32_t ring = smem_u32(paged_smem) + warp * (C::STAGES * 2 * C::TILE_BYTES);
-  const int units = p.kv_heads * p.row_blocks;      // per sequence
+  constexpr int R = C::R;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t bar_mem[2 * C::SLOTS + 8];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_mem, poison_mem[3];          // poison: a hidden value of the unit was NaN (units in turn)
+  __shared__ int found_b, found_base, warp_sum[PAGED_THREADS / 32];
+  // of the 8 groups of a tile, written and handed back with its V: scale of K, log2 and inverse of the scale of V, 0 where
+  // no page is
+  __shared__ float4 page_info[C::SLOTS / 2][8];
+  __shared__ float q_scale[2][R];
+  __shared__ float4 warp_max[R], warp_sums[2][R];   // by row, of the four softmax warps (sums: of odd and even units)
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  const uint32_t pad = (1024u - (raw_addr & 1023u)) & 1023u;
+  const uint32_t sRing = raw_addr + pad, sQ = sRing + C::SLOTS * C::TILE_BYTES, sP = sQ + C::Q_BUFS * C::Q_BYTES;
+  uint8_t* ring = smem_raw + pad;
+  uint8_t* q_mem = ring + C::SLOTS * C::TILE_BYTES;
+  uint8_t* p_mem = q_mem + C::Q_BUFS * C::Q_BYTES;
+  const uint32_t bars = smem_u32(bar_mem);
+  // K of tile c lies in slot 2c, V in slot 2c + 1, modulo the ring; a slot is used for the (c / HALF)-th time
+  constexpr int HALF = C::SLOTS / 2, B0 = 2 * C::SLOTS;
+  auto full = [&](int s) { return bars + 8 * s; };
+  auto empty = [&](int s) { return bars + 8 * (C::SLOTS + s); };
+  auto s_full = [&](int b) { return bars + 8 * (B0 + b); };
+  const uint32_t p_ready = bars + 8 * (B0 + 2), o_done = bars + 8 * (B0 + 3);
+  auto q_ready = [&](int b) { return bars + 8 * (B0 + 4 + b); };
+  auto q_empty = [&](int b) { return bars + 8 * (B0 + 6 + b); };
+  volatile int* abort_flag = &abort_mem;
+  volatile int* poison = poison_mem;
 
-  // ---- one unit's tiles [t0, t1) ----
-  auto segment = [&](int b, int u, int t0, int t1, int part_slot) {
-    const int h = u / p.row_blocks, r0 = (u % p.row_blocks) * ROWS;
-    const int len = paged_len(p, b);
-    const int* table = p.table + b * p.table_ld;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    // tiles of this warp: t0 + warp, + 8, ...; lane i knows the page and scales of the i-th of 32 of them
-    const int mine = max(0, (t1 - t0 - warp + PAGED_WARPS - 1) / PAGED_WARPS);
-    auto look = [&](int first, int& id, float& ks, float& vs) {
-      id = -1;
-      ks = vs = 0.f;
-      if (first + lane < mine) {
-        id = table[(t0 + warp + (first + lane) * PAGED_WARPS) * 16 / p.block];
-        if (id < 0 || id >= p.blocks) id = -1;
-        else {
-          ks = p.ks[(long long)id * p.kv_heads + h];
-          vs = p.vs[(long long)id * p.kv_heads + h];
-        }
-      }
-    };
-    int id_now, id_next;
-    float ks_now, vs_now, ks_next, vs_next;
-    look(0, id_now, ks_now, vs_now);
-    look(32, id_next, ks_next, vs_next);
-    auto issue = [&](int i, int batch) {
-      if (i < mine) {
-        const int id = __shfl_sync(0xffffffffu, i >> 5 == batch ? id_now : id_next, i & 31);
-        const int tok = (t0 + warp + i * PAGED_WARPS) * 16;
-        const long long at = id < 0 ? 0 : (((long long)id * p.kv_heads + h) * p.block + tok % p.block) * D;
-        const uint32_t dst = ring + (i % C::STAGES) * 2 * C::TILE_BYTES;
-#pragma unroll
-        for (int k = 0; k < D / 32; ++k) {
-          const int piece = k * 32 + lane;
-          const uint32_t to = dst + tile_at<D>(piece / (D / 16), piece % (D / 16));
-          cp_async16(to, p.kc + at + piece * 16, id >= 0);
-          cp_async16(to + C::TILE_BYTES, p.vc + at + piece * 16, id >= 0);
-        }
-      }
-      cp_commit();
-    };
-#pragma unroll
-    for (int i = 0; i < C::STAGES - 1; ++i) issue(i, 0);
-
-    // Q as fp16 fragments for all warps.  A row is multiplied by the power of two that brings its largest magnitude to
-    // [2^14, 2^15): bf16's 8 bits fit fp16's 11, and only what is 2^-28 of the row's largest begins to lose bits.
-    // MMA (half a, piece s, word j) pairs K's bytes 4j .. 4j + 3 of piece 8a + 2t + s (D = 64: piece t) with the same head
-    // dims of Q.
-    for (int nt = warp; nt < NT; nt += PAGED_WARPS) {
-      const int rr = r0 + nt * 8 + g;
-      const T* src = reinterpret_cast<const T*>(p.q) + (rr < p.rows ? paged_row(p, b, h, rr, p.q_seq, p.q_tok, p.q_head) : 0);
-      constexpr int PIECES = D / 64;         // 16-element pieces per lane
-      uint32_t w[PIECES][8];
-      float top = 0.f;
-#pragma unroll
-      for (int x = 0; x < PIECES; ++x) {
-        const int d = D == 64 ? 16 * t : 128 * (x >> 1) + 32 * t + 16 * (x & 1);
-        uint4 v0 = make_uint4(0u, 0u, 0u, 0u), v1 = v0;
-        if (rr < p.rows) {
-          v0 = *reinterpret_cast<const uint4*>(src + d);
-          v1 = *reinterpret_cast<const uint4*>(src + d + 8);
-        }
-        const uint32_t vv[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          w[x][e] = vv[e];
-          const float2 f = unpack2<T>(vv[e]);
-          top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
-        }
-      }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int e = (__float_as_int(top) >> 23) - 127 - 14;                       // top in [2^(e+14), 2^(e+15))
-      const bool plain = top == 0.f || !(top < INFINITY) || e < -126 || e > 126;  // zeros, infinities, the edges of the range
-      const float up = plain ? 1.f : __int_as_float((127 - e) << 23);
-      if (t == 0) q_scale[nt * 8 + g] = (plain ? 1.f : __int_as_float((127 + e) << 23)) * p.scale_log2e;
-#pragma unroll
-      for (int x = 0; x < PIECES; ++x)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 f0 = unpack2<T>(w[x][2 * j]), f1 = unpack2<T>(w[x][2 * j + 1]);
-          const __half2 h0 = __floats2half2_rn(f0.x * up, f0.y * up), h1 = __floats2half2_rn(f1.x * up, f1.y * up);
-          q_frag[(nt * C::KSTEPS + x * 4 + j) * 32 + lane] =
-              make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
-        }
+  if (threadIdx.x == 0) {
+#pragma unroll 1
+    for (int s = 0; s < C::SLOTS; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
     }
-    __syncthreads();
-    uint2 qr[C::Q_REGS ? NT * C::KSTEPS : 1];
-    if (C::Q_REGS) {
-#pragma unroll
-      for (int i = 0; i < (C::Q_REGS ? NT * C::KSTEPS : 1); ++i) qr[i] = q_frag[i * 32 + lane];
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(s_full(b), 1);
+      mbar_init(q_ready(b), 1);
+      mbar_init(q_empty(b), 1 + 4);
     }
-    float sc[NT][2];
-    int lim[NT][2];                          // keys that the rows of this lane's columns see
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int r = nt * 8 + 2 * t + c;
-        sc[nt][c] = q_scale[r];
-        lim[nt][c] = r0 + r < p.rows ? len - p.n_q + 1 + (r0 + r) / p.group : len;
-      }
-    const int lim_min = len - p.n_q + 1 + r0 / p.group;
+    mbar_init(p_ready, 128);
+    mbar_init(o_done, 1);
+    abort_mem = 0;
+    poison_mem[0] = poison_mem[1] = poison_mem[2] = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&p.tmK);
+    tma_prefetch_desc(&p.tmV);
+  }
+  if (warp == 1) tmem_alloc(smem_u32(&tmem_slot), C::TMEM_COLS);
+  pdl_wait();
 
-    float o[NT][D / 16][4];                  // [.][(half a, word j, e)]: head dims 128a + 16g + 4j + 2e, + 1 (D = 64: 8g + 4j + 2e)
-    float m[NT][2], l[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-      for (int f = 0; f < D / 16; ++f) o[nt][f][0] = o[nt][f][1] = o[nt][f][2] = o[nt][f][3] = 0.f;
-      m[nt][0] = m[nt][1] = -INFINITY;
-      l[nt][0] = l[nt][1] = 0.f;
+  // rows of sequences without tokens
+#pragma unroll 1
+  for (int b = blockIdx.x; b < p.n_seqs; b += gridDim.x) {
+    if (paged_len(p, b)) continue;
+#pragma unroll 1
+    for (int x = threadIdx.x; x < p.kv_heads * p.rows * D; x += PAGED_THREADS)
+      reinterpret_cast<T*>(p.o)[paged_row(p, b, x / (p.rows * D), x / D % p.rows, p.o_seq, p.o_tok, p.o_head) + x % D] = (T)0.f;
+  }
+  // this CTA's piece of the line, and the sequence it starts in
+  PagedWalk start;
+  start.begin = 0;
+  start.end = 0;
+  int piece = 0, sum = 0;
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    // the first pass forms the length of the line; with one round of sequences it also has each one's place in it
+#pragma unroll 1
+    for (int base = 0, rounds = (p.n_seqs + PAGED_THREADS - 1) / PAGED_THREADS; rounds > 0; --rounds, base += PAGED_THREADS) {
+      const int b = base + threadIdx.x;
+      const int groups = b < p.n_seqs ? (paged_len(p, b) + 15) >> 4 : 0;
+      const int n = groups ? (groups + PAGED_GAP) * p.units : 0;
+      int all;
+      const int at = sum + paged_scan(n, &all, warp_sum);
+      sum += all;
+      if (pass == 0 && rounds == 1) {
+        piece = max((int)((uint32_t)sum / gridDim.x) + 1, PAGED_MIN_PIECE);
+        start.begin = (int)min((long long)blockIdx.x * piece, (long long)sum);
+        start.end = min(start.begin + piece, sum);
+      }
+      if ((pass == 1 || base == 0 && rounds == 1) && at <= start.begin && start.begin < at + n) {
+        found_b = b;
+        found_base = at;
+      }
     }
+    if (p.n_seqs <= PAGED_THREADS) break;
+    sum = 0;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  if (start.begin < start.end) {
+    start.next_b = found_b;
+    start.len = paged_len(p, found_b);
+    const int one = ((start.len + 15) >> 4) + PAGED_GAP, u = (start.begin - found_base) / one;
+    start.next_h = u / p.row_blocks;
+    start.next_rb = u - start.next_h * p.row_blocks;
+    start.next_at = found_base + u * one;
+  } else {
+    start.next_at = start.end;               // no part
+  }
 
-    for (int i = 0; i < mine; ++i) {
-      if (i && (i & 31) == 0) {
-        id_now = id_next; ks_now = ks_next; vs_now = vs_next;
-        look(i + 32, id_next, ks_next, vs_next);
+  if (warp == 0) {
+    // ---- pages and TMA: lane (j, g) looks after group g of the j-th of four tiles.  Ids are fetched one batch ahead,
+    // across units, and scales while the batch before goes out, so that neither latency stands between two loads. ----
+    PagedWalk w = start;
+    struct Batch { int b, h, len, tile, n; int id; float ks, vs; };
+    Batch now, next;
+    now.n = 0;
+    int c = 0, tile = 0;
+    bool ok = true, more = w.next(p);
+    if (more) tile = w.t0;
+    const uint64_t pol = policy_evict_normal();
+    const int per_box = p.box_rows / 16;
+#pragma unroll 1
+    do {
+      next.n = 0;
+      next.id = -1;
+      if (more) {
+        next.b = w.b; next.h = w.h; next.len = w.len; next.tile = tile;
+        next.n = min(4, w.t1 - tile);
+        tile += next.n;
+        if ((lane >> 3) < next.n) {
+          const int group = next.tile * 8 + lane;
+          if (group * 16 < next.len) next.id = p.table[next.b * p.table_ld + page_of(p, group)];
+        }
+        if (tile == w.t1) {
+          more = w.next(p);
+          if (more) tile = w.t0;
+        }
       }
-      cp_wait<C::STAGES - 2>();
+#pragma unroll 1
+      for (int j = 0; j < now.n && ok; ++j, ++c) {
+        const int s = 2 * (c % HALF);
+        const uint32_t freed = (uint32_t)(c / HALF - 1) & 1u;
+        const bool here = lane >> 3 == j;
+        const int g = lane & 7, group = (now.tile + j) * 8 + g;
+        const bool load = here && now.id >= 0 && g % per_box == 0;
+        const int bytes = __popc(__ballot_sync(0xffffffffu, load)) * p.box_rows * D;
+        const int row = now.h * p.block + group * 16 - page_of(p, group) * p.block;
+#pragma unroll 1
+        for (int kv = 0; kv < 2; ++kv) {
+          if (c >= HALF) ok = ok && __all_sync(0xffffffffu, paged_wait(empty(s + kv), freed, abort_flag));
+          if (!ok) break;
+          if (load) {
+            const uint32_t dst = sRing + (s + kv) * C::TILE_BYTES + g * 16 * C::ROW_BYTES;
+#pragma unroll
+            for (int x = 0; x < C::HALVES; ++x)
+              tma_load_3d(dst + x * C::BLOCK_BYTES, kv ? &p.tmV : &p.tmK, full(s + kv), x * 128, row, now.id, pol);
+          }
+          if (kv == 1 && here) {                // the scales may come in later than the loads go out
+            const float v = fmaxf(now.vs, 0x1p-100f);      // a page of zeros may have any scale, zero too; NaN stays
+            page_info[c % HALF][g] = now.id < 0 ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                                : make_float4(now.ks, now.vs != now.vs ? now.vs : lg2_approx(v), now.vs != now.vs ? now.vs : 1.f / v, 1.f);
+          }
+          __syncwarp();                         // page_info goes out with lane 0's arrival
+          if (lane == 0) mbar_expect_tx(full(s + kv), bytes);
+        }
+      }
+      // the batch that is next: its ids are here by now, its scales are asked for
+      now = next;
+      if (now.id >= p.blocks) now.id = -1;
+      if (now.n && now.id >= 0) {
+        now.ks = p.ks[(long long)now.id * p.kv_heads + now.h];
+        now.vs = p.vs[(long long)now.id * p.kv_heads + now.h];
+      }
+    } while (ok && now.n);
+  } else if (warp == 1) {
+    // ---- MMA: S up to one tile ahead of P V, each issued as soon as its operands are there ----
+    if (lane == 0) {
+      const uint32_t idesc = (1u << 4) | ((uint32_t)(C::N / 8) << 17) | (8u << 24);       // e4m3 x e4m3 -> fp32, M = 128
+      const uint32_t idesc_pv = idesc | (1u << 15);                                        // A MN-major
+      PagedWalk w = start;
+      int tile = 0, cs = 0, cp = 0, seg = -1;
+      bool more = true, turn = true;            // turn: the next S is a unit's first
+      // of the tiles whose P V is to come, at most two, even and odd: MMA steps of 32 tokens, negative for a unit's first
+      int steps_of[2] = {0, 0};
+      const uint64_t k_desc = paged_desc(sRing, 16, C::GROUP_STRIDE, C::LAYOUT), q_desc = paged_desc(sQ, 16, C::GROUP_STRIDE, C::LAYOUT);
+      // 64 head dims: M's second half runs on into what lies behind, and is not used
+      const uint64_t v_desc = paged_desc(sRing, D == 64 ? C::TILE_BYTES : 16, C::GROUP_STRIDE, C::LAYOUT), p_desc = paged_desc(sP, 16, 1024, 2);
+      uint64_t t_idle = 0;
+      uint32_t idle = 0;
+#pragma unroll 1
+      for (;;) {
+        bool did = false;
+        if (turn && more) {
+          more = w.next(p);
+          tile = w.t0;
+          ++seg;
+          turn = false;
+        }
+        if (!more && cp == cs) break;
+        if (more && cs <= cp + 1) {            // S of tile cp + 1 goes over that of cp - 1, whose P has been taken
+          const int s = 2 * (cs % HALF), qb = seg % C::Q_BUFS;
+          if (mbar_test(full(s), (uint32_t)(cs / HALF) & 1u) && (tile != w.t0 || mbar_test(q_ready(qb), (uint32_t)(seg / C::Q_BUFS) & 1u))) {
+            tc_fence_after();
+            const uint64_t kd = k_desc + s * (C::TILE_BYTES / 16), qd = q_desc + qb * (C::Q_BYTES / 16);
+#pragma unroll
+            for (int x = 0; x < C::HALVES; ++x)
+#pragma unroll
+              for (int k = 0; k < C::ROW_BYTES / 32; ++k)
+                umma_f8(tmem + C::S_COL + (cs & 1) * C::N, kd + x * (C::BLOCK_BYTES / 16) + 2 * k, qd + x * (C::N * 8) + 2 * k, idesc, (x | k) != 0);
+            umma_commit(empty(s));
+            umma_commit(s_full(cs & 1));
+            const int steps = (min(w.len - tile * 128, 128) + 31) >> 5;
+            steps_of[cs & 1] = tile == w.t0 ? -steps : steps;
+            ++cs;
+            if (++tile == w.t1) {
+              umma_commit(q_empty(qb));        // this unit's Q is no longer read
+              turn = true;
+            }
+            did = true;
+          }
+        }
+        if (cp < cs) {
+          const int s = 2 * (cp % HALF) + 1;
+          if (mbar_test(p_ready, (uint32_t)cp & 1u) && mbar_test(full(s), (uint32_t)(cp / HALF) & 1u)) {
+            tc_fence_after();
+            const uint64_t vd = v_desc + s * (C::TILE_BYTES / 16);
+            const int steps = steps_of[cp & 1];
+#pragma unroll
+            for (int x = 0; x < C::HALVES; ++x)
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                if (k < abs(steps))
+                  umma_f8(tmem + C::O_COL + x * C::N, vd + x * (C::BLOCK_BYTES / 16) + k * (32 * C::ROW_BYTES / 16), p_desc + 2 * k, idesc_pv, steps > 0 || k != 0);
+            umma_commit(empty(s));
+            umma_commit(o_done);
+            ++cp;
+            did = true;
+          }
+        }
+        if (did) {
+          idle = 0;
+        } else if ((++idle & 255) == 0) {      // the clock is read seldom: a look at it costs more than one at the barriers
+          const uint64_t now = globaltimer_ns();
+          if (idle == 256) t_idle = now;
+          if (*abort_flag || now - t_idle > VLA_WAIT_LIMIT_NS) {
+            *abort_flag = 1;
+            break;
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 2) {
+    // ---- Q pieces: each row times the power of two that brings its largest magnitude to [2^7, 2^8) ----
+    PagedWalk w = start;
+#pragma unroll 1
+    for (int seg = 0; w.next(p); ++seg) {
+      const int qb = seg % C::Q_BUFS, h = w.h, r0 = w.rb * R;
+      constexpr int E = D / 64;               // pairs of elements per lane and row
+      uint32_t rows[R][E];                    // all in flight at once; they move up as the loop takes the first
+      const int i0 = r0 ? r0 / p.group : 0;
+      int g = r0 - i0 * p.group;
+      const T* src = reinterpret_cast<const T*>(p.q) + w.b * p.q_seq + i0 * p.q_tok + (long long)(h * p.group + g) * p.q_head + lane * (2 * E);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) rows[r][i] = 0u;
+        if (r0 + r < p.rows) {
+          if (E == 4) {
+            const uint4 v = *reinterpret_cast<const uint4*>(src);
+            rows[r][0] = v.x; rows[r][1 % E] = v.y; rows[r][2 % E] = v.z; rows[r][3 % E] = v.w;
+          } else if (E == 2) {
+            const uint2 v = *reinterpret_cast<const uint2*>(src);
+            rows[r][0] = v.x; rows[r][1 % E] = v.y;
+          } else {
+            rows[r][0] = *reinterpret_cast<const uint32_t*>(src);
+          }
+        }
+        src += p.q_head;
+        if (++g == p.group) {
+          g = 0;
+          src += p.q_tok - p.group * p.q_head;
+        }
+      }
+      if (seg >= C::Q_BUFS && !__all_sync(0xffffffffu, paged_wait(q_empty(qb), (uint32_t)(seg / C::Q_BUFS - 1) & 1u, abort_flag))) break;
+#pragma unroll 1
+      for (int r = 0; r < R; ++r) {
+        float2 f[E];
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          f[i] = unpack2<T>(rows[0][i]);
+          top = fmaxf(top, fmaxf(fabsf(f[i].x), fabsf(f[i].y)));
+#pragma unroll
+          for (int k = 0; k + 1 < R; ++k) rows[k][i] = rows[k + 1][i];
+        }
+        top = warp_max_f32(top);
+        const int e = (__float_as_int(top) >> 23) - 127 - 7;
+        // zeros, the smallest numbers and infinities stay as they are; the scores of a row with an infinity are NaN
+        const bool plain = top == 0.f || !(top < INFINITY) || e < -126;
+        const float up = plain ? 1.f : __int_as_float((127 - e) << 23);
+        if (lane == 0) q_scale[qb][r] = (plain ? 1.f : __int_as_float((127 + e) << 23)) * (top < INFINITY ? p.scale_log2e : NAN);
+        uint32_t c[E][3];
+#pragma unroll
+        for (int i = 0; i < E; ++i) pieces(f[i].x * up, f[i].y * up, c[i]);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+          const int n = k * R + r, at = lane * (2 * E);          // byte of the row
+          uint8_t* dst = q_mem + qb * C::Q_BYTES + (at / 128) * C::N * 128 + n * C::ROW_BYTES +
+                         (((at % 128 / 16) ^ (D == 64 ? n >> 1 & 3 : n & 7)) << 4) + at % 16;
+          if (E == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(c[0][k] | c[1 % E][k] << 16, c[2 % E][k] | c[3 % E][k] << 16);
+          else if (E == 2) *reinterpret_cast<uint32_t*>(dst) = c[0][k] | c[1 % E][k] << 16;
+          else *reinterpret_cast<uint16_t*>(dst) = (uint16_t)c[0][k];
+        }
+      }
+      fence_proxy_async_shared();
       __syncwarp();
-      issue(i + C::STAGES - 1, i >> 5);
-      const int id = __shfl_sync(0xffffffffu, id_now, i & 31);
-      const float ks = __shfl_sync(0xffffffffu, ks_now, i & 31), vs = __shfl_sync(0xffffffffu, vs_now, i & 31);
-      const int tok = (t0 + warp + i * PAGED_WARPS) * 16;
-      const uint32_t sk = ring + (i % C::STAGES) * 2 * C::TILE_BYTES, sv = sk + C::TILE_BYTES;
-
-      float s[NT][4];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
-#pragma unroll
-      for (int x = 0; x < D / 64; ++x) {
-        const int piece = D == 64 ? t : 8 * (x >> 1) + 2 * t + (x & 1);
-        const uint4 a = lds128(sk + tile_at<D>(g, piece)), c = lds128(sk + tile_at<D>(g + 8, piece));
-        const uint32_t wa[4] = {a.x, a.y, a.z, a.w}, wc[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t fr[4] = {e4m3x2_f16x2(wa[j]), e4m3x2_f16x2(wc[j]), e4m3x2_f16x2(wa[j] >> 16), e4m3x2_f16x2(wc[j] >> 16)};
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const uint2 qq = C::Q_REGS ? qr[nt * C::KSTEPS + x * 4 + j] : q_frag[(nt * C::KSTEPS + x * 4 + j) * 32 + lane];
-            mma_f16(s[nt], fr, qq.x, qq.y);
-          }
-        }
-      }
-      const bool edge = tok + 16 > lim_min || id < 0;        // warp-uniform: some row does not see some token
-      bool grow = false;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[nt][e] *= sc[nt][e & 1] * ks;
-          if (edge && (id < 0 || tok + g + 4 * (e & 2) >= lim[nt][e & 1])) s[nt][e] = -INFINITY;
-          grow |= s[nt][e] > m[nt][e & 1] + 8.f;
-        }
-      // The subtracted maximum moves when a score has outgrown it by 2^8: probabilities stay below that, within fp16.
-      if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float top = fmaxf(m[nt][c], fmaxf(s[nt][c], s[nt][c + 2]));
-#pragma unroll
-            for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-            const float a = top == m[nt][c] ? 1.f : ex2_approx(m[nt][c] - top);
-            m[nt][c] = top;
-            l[nt][c] *= a;
-#pragma unroll
-            for (int f = 0; f < D / 16; ++f) {
-              o[nt][f][c] *= a;
-              o[nt][f][c + 2] *= a;
+      if (lane == 0) mbar_arrive(q_ready(qb));
+    }
+  } else {
+    // ---- softmax: thread = token of the tile; at a unit's end, thread = head dim.  A wait that runs out raises the abort
+    // flag and the loop goes on with whatever is there, because the 128 threads meet at barriers. ----
+    const int quarter = warp & 3, tid = quarter * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+      paged_wait(bar, parity, abort_flag);
+      __syncwarp();
+    };
+    // a part, with head, first row, and that row's query and group head
+    struct Part { int b, h, rb, len, t0, t1, tiles, at, r0, i0, g0; };
+    PagedWalk walk = start;
+    auto take = [&](Part& x) {
+      if (!walk.next(p)) return false;
+      x.b = walk.b; x.h = walk.h; x.rb = walk.rb; x.len = walk.len; x.t0 = walk.t0; x.t1 = walk.t1; x.tiles = walk.tiles; x.at = walk.at;
+      x.r0 = x.rb * R;
+      x.i0 = x.r0 ? x.r0 / p.group : 0;
+      x.g0 = x.r0 - x.i0 * p.group;
+      return true;
+    };
+    Part w, w_next;
+    w.t0 = w.t1 = 0;
+    int c = 0, cut_b = -1;
+    // one pass per unit, after a first that only looks up the unit to begin with
+#pragma unroll 1
+    for (int seg = -1;; ++seg) {
+      const int h = w.h, r0 = w.r0, i0 = w.i0, g0 = w.g0;
+      const int lim_min = w.len - p.n_q + 1 + i0;               // the first row sees the fewest keys
+      float qs[R], m[R], l[R];
+#pragma unroll 1
+      for (int tile = w.t0; tile < w.t1; ++tile, ++c) {
+        const int s = 2 * (c % HALF), tok = tile * 128 + tid;
+        wait(full(s + 1), (uint32_t)(c / HALF) & 1u);
+        const float4 info = page_info[c % HALF][tid >> 4];
+        const bool edge = tile * 128 + 128 > lim_min;
+        if (edge || !__all_sync(0xffffffffu, info.w != 0.f)) {
+          // A row of V that no row of this unit sees is cleared; where only some see it, a NaN in it is, and the end of
+          // the unit gives it back: P is zero there, but zero times NaN is NaN.
+          uint8_t* row = ring + (s + 1) * C::TILE_BYTES + tid * C::ROW_BYTES;
+          const bool none = tok >= w.len || info.w == 0.f;
+          if ((none || tok >= lim_min) && tid < (min(w.len - tile * 128, 128) + 31) / 32 * 32) {   // of what P V reads
+#pragma unroll 2
+            for (int x = 0; x < D / 16; ++x) {
+              uint4* at = reinterpret_cast<uint4*>(row + (x / 8) * C::BLOCK_BYTES + (((x & 7) ^ (D == 64 ? tid >> 1 & 3 : tid & 7)) << 4));
+              uint4 v = *at;
+              const uint4 bad = make_uint4(nan_bytes(v.x), nan_bytes(v.y), nan_bytes(v.z), nan_bytes(v.w));
+              if (none) {
+                *at = make_uint4(0u, 0u, 0u, 0u);
+              } else if (bad.x | bad.y | bad.z | bad.w) {
+                v.x &= ~((bad.x >> 7) * 0xffu); v.y &= ~((bad.y >> 7) * 0xffu);     // 0x80 -> 0xff over the byte
+                v.z &= ~((bad.z >> 7) * 0xffu); v.w &= ~((bad.w >> 7) * 0xffu);
+                *at = v;
+                poison[seg % 3] = 1;
+              }
             }
           }
-      }
-      uint32_t pb[NT][2];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float e[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float sub = m[nt][k & 1] == -INFINITY ? 0.f : m[nt][k & 1];
-          e[k] = ex2_approx(s[nt][k] - sub);
-          l[nt][k & 1] += e[k];
+          __syncwarp();
         }
-        const __half2 h0 = __floats2half2_rn(e[0], e[1]), h1 = __floats2half2_rn(e[2], e[3]);
-        pb[nt][0] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&h0));
-        pb[nt][1] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&h1));
-      }
-      // O^T += s_v (V^T P^T), tokens 2t, 2t + 1, 2t + 8, 2t + 9 of each lane.  `seen`: tokens from there on are cleared;
-      // `query` >= 0: only the columns of that query are added.
-      auto pv = [&](auto careful, int seen, int query) {
-        constexpr int VW = D == 64 ? 2 : 4;                  // words per row and lane
-        bool nan = false;
+        wait(s_full(c & 1), (uint32_t)(c >> 1) & 1u);
+        tc_fence_after();
+        if (tile == w.t0) {
+          wait(q_ready(seg % C::Q_BUFS), (uint32_t)(seg / C::Q_BUFS) & 1u);
 #pragma unroll
-        for (int a = 0; a < (D == 256 ? 2 : 1); ++a) {
-          uint32_t w[4][VW];
+          for (int r = 0; r < R; ++r) {
+            qs[r] = q_scale[seg % C::Q_BUFS][r];
+            m[r] = -INFINITY;
+            l[r] = 0.f;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(q_empty(seg % C::Q_BUFS));
+        }
+        float x[R];                              // s + log2 s_v
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int row = 2 * t + (k & 1) + 4 * (k & 2);
-            if (D == 64) {
-              const uint2 v = lds64(sv + tile_at<D>(row, g >> 1) + 8 * (g & 1));
-              w[k][0] = v.x; w[k][1] = v.y;
-            } else {
-              const uint4 v = lds128(sv + tile_at<D>(row, 8 * a + g));
-              w[k][0] = v.x; w[k][1] = v.y; w[k][VW - 2] = v.z; w[k][VW - 1] = v.w;
-            }
-            if (decltype(careful)::value && tok + row >= seen) {
+        for (int r8 = 0; r8 < R; r8 += 8) {
+          uint32_t v[24];
+          paged_tmem_ld(tmem + lane_off + C::S_COL + (c & 1) * C::N + r8, R, v);
 #pragma unroll
-              for (int j = 0; j < VW; ++j) w[k][j] = 0u;
+          for (int r = 0; r < 8; ++r) x[r8 + r] = info.w == 0.f ? -INFINITY : fmaf(paged_sum(v, r), qs[r8 + r] * info.x, info.y);
+        }
+        if (edge) {
+          int lim = min(w.len, lim_min), left = p.group - g0;   // rows of a query follow one another
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            if (tok >= lim) x[r] = -INFINITY;
+            if (--left == 0) {
+              left = p.group;
+              lim = min(w.len, lim + 1);
             }
           }
+        }
+        bool grow = false;
 #pragma unroll
-          for (int j = 0; j < VW; ++j) {
-            if (decltype(careful)::value && query < 0) nan |= has_nan(w[0][j]) || has_nan(w[1][j]) || has_nan(w[2][j]) || has_nan(w[3][j]);
+        for (int r = 0; r < R; ++r) grow |= x[r] > m[r] + 1.f;
+        // The subtracted maximum moves when a token has outgrown it by more than 2: w stays below 2 * 2^7, in e4m3's range.
+        if (tile == w.t0 || barrier_any(1, grow)) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const uint32_t x = __byte_perm(w[0][j], w[1][j], e ? 0x7362 : 0x5140), y = __byte_perm(w[2][j], w[3][j], e ? 0x7362 : 0x5140);
-              const uint32_t fr[4] = {e4m3x2_f16x2(x), e4m3x2_f16x2(x >> 16), e4m3x2_f16x2(y), e4m3x2_f16x2(y >> 16)};
+          for (int r = 0; r < R; ++r) {
+            const float top = warp_max_f32(x[r]);
+            if (lane == 0) reinterpret_cast<float*>(&warp_max[r])[quarter] = top;
+          }
+          if (tile > w.t0) wait(o_done, (uint32_t)(c - 1) & 1u);
+          tc_fence_after();
+          named_barrier_sync(1, 128);
+          float a[R];
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                float c[4] = {0.f, 0.f, 0.f, 0.f};
-                mma_f16(c, fr, pb[nt][0], pb[nt][1]);
-                float* acc = o[nt][a * 8 + j * 2 + e];
+          for (int r = 0; r < R; ++r) {
+            const float4 tops = warp_max[r];
+            const float top = fmaxf(m[r], fmaxf(fmaxf(tops.x, tops.y), fmaxf(tops.z, tops.w)));
+            a[r] = top == m[r] ? 1.f : ex2_approx(m[r] - top);
+            m[r] = top;
+            l[r] *= a[r];
+          }
+          if (tile > w.t0) {
+#pragma unroll 1
+            for (int y = 0; y < C::HALVES; ++y) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                  if (!decltype(careful)::value || query < 0 || (r0 + nt * 8 + 2 * t + (k & 1)) / p.group == query) acc[k] = fmaf(vs, c[k], acc[k]);
+              for (int r8 = 0; r8 < R; r8 += 8) {
+                uint32_t o[24];
+                paged_tmem_ld(tmem + lane_off + C::O_COL + y * C::N + r8, R, o);
+#pragma unroll
+                for (int i = 0; i < 24; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a[r8 + i % 8]);
+                paged_tmem_st(tmem + lane_off + C::O_COL + y * C::N + r8, R, o);
               }
             }
           }
         }
-        return nan;
-      };
-      if (!edge) {
-        pv(std::false_type{}, 0, -1);
-      } else if (p.n_q == 1) {
-        pv(std::true_type{}, len, -1);
-      } else {
-        // Tokens that only later queries see: a NaN among their values would reach the others as 0 * NaN.  Then each
-        // query is multiplied with its own tokens alone.
-        bool nan = false;
-        for (int k = lane; k < D; k += 32) {
-          const int row = k / (D / 16);
-          const uint4 v = lds128(sv + tile_at<D>(row, k % (D / 16)));
-          nan |= tok + row >= lim_min && tok + row < len && (has_nan(v.x) || has_nan(v.y) || has_nan(v.z) || has_nan(v.w));
+        if (c > 0) wait(o_done, (uint32_t)(c - 1) & 1u);   // P of the tile before has been read
+        uint8_t* p_col = p_mem + (tid & 15);
+        const int chunk = tid >> 4;
+#pragma unroll
+        for (int r = 0; r < R; r += 2) {
+          float e[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            e[k] = ex2_approx(x[r + k] - (m[r + k] == -INFINITY ? 0.f : m[r + k]) + 7.f);
+            if (e[k] != 0.f) l[r + k] = fmaf(e[k], info.z, l[r + k]);   // a hidden token's scale may be NaN
+          }
+          uint32_t pc[3];
+          pieces(e[0], e[1], pc);
+#pragma unroll
+          for (int k = 0; k < 3; ++k) {
+            const int n = k * R + r;
+            p_col[n * 128 + ((chunk ^ (n & 7)) << 4)] = (uint8_t)pc[k];
+            p_col[(n + 1) * 128 + ((chunk ^ ((n + 1) & 7)) << 4)] = (uint8_t)(pc[k] >> 8);
+          }
         }
-        if (!__any_sync(0xffffffffu, nan)) {
-          pv(std::true_type{}, len, -1);
-        } else {
-          const int q_end = min((r0 + ROWS - 1) / p.group, p.n_q - 1);
-          for (int query = r0 / p.group; query <= q_end; ++query) pv(std::true_type{}, len - p.n_q + 1 + query, query);
+        fence_proxy_async_shared();
+        tc_fence_before();
+        mbar_arrive(p_ready);
+      }
+
+      // ---- the unit's end: out = O / l ----
+      if (seg >= 0) {
+        // sums over a warp's lanes: each exchange halves the rows a lane looks after, so R + 1 or so exchanges do for all
+#pragma unroll
+        for (int half = R / 2, bit = 16; half >= 1; half >>= 1, bit >>= 1) {
+#pragma unroll
+          for (int r = 0; r < half; ++r) {
+            const bool up = lane & bit;
+            const float give = up ? l[r] : l[r + half], keep = up ? l[r + half] : l[r];
+            l[r] = keep + __shfl_xor_sync(0xffffffffu, give, bit);
+          }
         }
+#pragma unroll
+        for (int bit = 16 / R; bit > 0; bit >>= 1) l[0] += __shfl_xor_sync(0xffffffffu, l[0], bit);
+        if (lane % (32 / R) == 0) reinterpret_cast<float*>(&warp_sums[seg & 1][lane / (32 / R)])[quarter] = l[0];
       }
-    }
-    cp_wait<0>();
-
-    // ---- join the warps' sums: out = sum_w 2^(m_w - M) o_w / sum_w 2^(m_w - M) l_w ----
-    __syncthreads();                         // every warp is through with its ring
+      const bool more = take(w_next);            // while the last P V runs
+      if (seg >= 0) {
+        wait(o_done, (uint32_t)(c - 1) & 1u);
+        tc_fence_after();
+        named_barrier_sync(1, 128);
+        const int slot = w.t0 == 0 ? (w.t1 == w.tiles ? -1 : 1) : 0;
+        // A flag is read here, after this barrier, by all; cleared a unit later, and written two units later at the
+        // earliest: there are barriers between.  The same goes for warp_sums, which two units share in turn.
+        const bool bad = poison[seg % 3] != 0;
+        if (tid == 0) poison[(seg + 2) % 3] = 0;
+        const long long o_at = slot < 0 ? w.b * p.o_seq + i0 * p.o_tok + (long long)(h * p.group + g0) * p.o_head : 0;
+        const long long turn = p.o_tok - (p.group - 1) * p.o_head;     // from a query's last head to the next query's first
+#pragma unroll 1
+        for (int y = 0; y < C::HALVES; ++y) {
+          float val[R];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+          for (int r8 = 0; r8 < R; r8 += 8) {
+            uint32_t o[24];
+            paged_tmem_ld(tmem + lane_off + C::O_COL + y * C::N + r8, R, o);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+            for (int r = 0; r < 8; ++r) val[r8 + r] = paged_sum(o, r);
+          }
+          const int d = y * 128 + tid;
+          if (d >= D) break;
+          uint32_t nans = 0;                       // rows that see a NaN in this head dim
+          if (bad) {
+#pragma unroll 1
+            for (int tok = max(lim_min, w.t0 * 128); tok < min(w.len, w.t1 * 128); ++tok) {
+              const int id = p.table[w.b * p.table_ld + page_of(p, tok >> 4)];
+              if (id >= 0 && id < p.blocks && (p.vc[(((long long)id * p.kv_heads + h) * p.block + tok % p.block) * D + d] & 0x7f) == 0x7f) {
+#pragma unroll 1
+                for (int r = 0; r < R; ++r) nans |= (uint32_t)(tok < w.len - p.n_q + 1 + (r0 + r) / p.group) << r;
+              }
+            }
+          }
+          const int n_rows = min(R, p.rows - r0);
 #pragma unroll
-        for (int x = 4; x < 32; x <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], x);
-        if (g == 0) warp_ml[warp][nt * 8 + 2 * t + c] = make_float2(m[nt][c], l[nt][c]);
-      }
-      if (mine > 0) {
+          for (int r = 0; r < R; ++r)
+            if (nans >> r & 1) val[r] = NAN;
+          if (slot < 0) {
+            T* dst = reinterpret_cast<T*>(p.o) + o_at + d;
+            int left = p.group - g0;
 #pragma unroll
-        for (int f = 0; f < D / 16; ++f)
+            for (int r = 0; r < R; ++r) {
+              const float4 sums = warp_sums[seg & 1][r];
+              const float sum = (sums.x + sums.y) + (sums.z + sums.w);
+              if (r < n_rows) *dst = (T)(sum == 0.f ? 0.f : val[r] * rcp_approx(sum));       // 0: nothing seen
+              --left;
+              dst += left ? p.o_head : turn;
+              left = left ? left : p.group;
+            }
+          } else {
+            float* part = p.part_o + ((long long)blockIdx.x * 2 + slot) * (R * D) + d;
+            float2* part_ml = p.part_ml + ((long long)blockIdx.x * 2 + slot) * R;
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
-            *reinterpret_cast<float2*>(join + (warp * ROWS + nt * 8 + 2 * t + c) * C::RSTRIDE + f * 16 + g * 2) =
-                make_float2(o[nt][f][c], o[nt][f][c + 2]);
-      }
-    }
-    __syncthreads();
-    for (int x = threadIdx.x; x < ROWS * (D / 2); x += PAGED_THREADS) {
-      const int r = x / (D / 2), d = (x % (D / 2)) * 2, rr = r0 + r;
-      if (rr >= p.rows) continue;
-      // head dim d lies at fragment f, lane group gg
-      const int gg = D == 64 ? d / 8 : d % 128 / 16, f = D == 64 ? d % 8 / 2 : d / 128 * 8 + d % 16 / 2;
-      float top = -INFINITY, sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < PAGED_WARPS; ++w) top = fmaxf(top, warp_ml[w][r].x);
-      float2 acc = make_float2(0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < PAGED_WARPS; ++w) {
-        const float2 ml = warp_ml[w][r];
-        if (ml.x != -INFINITY || ml.y != 0.f) {   // otherwise this warp has seen nothing of this row
-          const float a = ml.x == top ? 1.f : ex2_approx(ml.x - top);
-          const float2 v = *reinterpret_cast<const float2*>(join + (w * ROWS + r) * C::RSTRIDE + f * 16 + gg * 2);
-          acc.x = fmaf(a, v.x, acc.x);
-          acc.y = fmaf(a, v.y, acc.y);
-          sum = fmaf(a, ml.y, sum);
+            for (int r = 0; r < R; ++r) {
+              const float4 sums = warp_sums[seg & 1][r];
+              const float sum = (sums.x + sums.y) + (sums.z + sums.w);
+              if (r < n_rows) part[r * D] = sum == 0.f ? 0.f : val[r];
+              if (d == r) part_ml[r] = make_float2(m[r], sum);
+            }
+          }
         }
+        __syncwarp();
+        tc_fence_before();
+        if (slot == 1) cut_b = w.b;                // the piece's last unit
       }
-      if (part_slot < 0) {
-        const float inv = sum != 0.f ? 1.f / sum : 0.f;
-        T* dst = reinterpret_cast<T*>(p.o) + paged_row(p, b, h, rr, p.o_seq, p.o_tok, p.o_head) + d;
-        dst[0] = (T)(acc.x * inv);
-        dst[1] = (T)(acc.y * inv);
-      } else {
-        const long long at = ((long long)blockIdx.x * 2 + part_slot) * ROWS + r;
-        *reinterpret_cast<float2*>(p.part_o + at * D + d) = acc;
-        if (d == 0) p.part_ml[at] = make_float2(top, sum);
-      }
+      if (!more) break;
+      w = w_next;
     }
-    __syncthreads();                         // before the next unit's tiles go over the sums
-  };
-  auto zero = [&](int b, int h0, int h1) {
-    for (int x = threadIdx.x; x < (h1 - h0) * p.rows * D; x += PAGED_THREADS) {
-      const int h = h0 + x / (p.rows * D), rr = x / D % p.rows;
-      reinterpret_cast<T*>(p.o)[paged_row(p, b, h, rr, p.o_seq, p.o_tok, p.o_head) + x % D] = (T)0.f;
-    }
-  };
+    if (tid == 0 && !p.whole)
+      *reinterpret_cast<int4*>(p.cut + 4 * blockIdx.x) = make_int4(cut_b, w.h, w.rb, cut_b < 0 ? 0 : (w.at + 8 * (w.tiles - 1)) / piece);
+  }
 
-  if (!p.split) {
-    const int b = blockIdx.x / units, u = blockIdx.x % units;
-    const int tiles = paged_tiles(p, b);
-    if (tiles) segment(b, u, 0, tiles, -1);
-    else if (u % p.row_blocks == 0) zero(b, u / p.row_blocks, u / p.row_blocks + 1);
-    return;
-  }
-  for (int b = blockIdx.x; b < p.n_seqs; b += gridDim.x)
-    if (paged_tiles(p, b) == 0) zero(b, 0, p.kv_heads);
-
-  // This CTA's piece of the line of tiles, and the sequence it starts in
-  long long total = 0;
-  for (int base = 0; base < p.n_seqs; base += PAGED_THREADS) {
-    const int b = base + threadIdx.x;
-    long long all;
-    block_scan(b < p.n_seqs ? (long long)paged_tiles(p, b) * units : 0, &all, warp_sum);
-    total += all;
-  }
-  const long long piece = max((total + gridDim.x - 1) / gridDim.x, (long long)PAGED_MIN_TILES);
-  const long long begin = blockIdx.x * piece, end = min(begin + piece, total);
-  int cut_b = -1, cut_u = 0, cut_last = 0;
-  if (begin < end) {
-    long long sum = 0;
-    for (int base = 0; base < p.n_seqs && sum <= begin; base += PAGED_THREADS) {
-      const int b = base + threadIdx.x;
-      const long long n = b < p.n_seqs ? (long long)paged_tiles(p, b) * units : 0;
-      long long all;
-      const long long at = sum + block_scan(n, &all, warp_sum);
-      if (at <= begin && begin < at + n) {
-        found_b = b;
-        found_base = at;
-      }
-      sum += all;
-    }
-    __syncthreads();
-    int b = found_b;
-    long long base = found_base, pos = begin;
-    while (pos < end) {
-      const int tiles = paged_tiles(p, b);
-      const long long n = (long long)tiles * units;
-      if (pos >= base + n) {                 // on to the next sequence that has tokens
-        base += n;
-        ++b;
-        continue;
-      }
-      const int u = (int)((pos - base) / tiles), t0 = (int)((pos - base) % tiles);
-      const int t1 = (int)min((long long)tiles, t0 + (end - pos));
-      const long long unit_at = base + (long long)u * tiles;
-      const bool first = unit_at >= begin, last = unit_at + tiles <= end;
-      segment(b, u, t0, t1, first && last ? -1 : first ? 1 : 0);
-      if (first && !last) {
-        cut_b = b;
-        cut_u = u;
-        cut_last = (int)((unit_at + tiles - 1) / piece);
-      }
-      pos += t1 - t0;
-    }
-  }
-  if (threadIdx.x == 0) *reinterpret_cast<int4*>(p.cut + 4 * blockIdx.x) = make_int4(cut_b, cut_u, cut_last, 0);
+  // ---- teardown ----
   pdl_trigger();
+  tc_fence_before();
+  __syncthreads();
+  if (abort_mem) {   // a wait ran out: say so, and let copies in flight land before the shared memory goes to another CTA
+    if (threadIdx.x == 0) atomicOr(&cache_ops_status, VLA_ST_WAIT_TIMEOUT);
+#pragma unroll 1
+    for (int i = 0; i < 32; ++i) __nanosleep(1000);
+  }
+  if (warp == 1) tmem_dealloc(tmem, C::TMEM_COLS);
 }
 
-// Joins the partial sums of the units that were cut: block (c, r) does row r of the unit that starts in piece c, one thread per
-// head dim, the pieces in order.
+// Joins the partial sums of the units that were cut: block (c, y) does two or four rows of the unit that starts in piece c.  A row's
+// parts are dealt out to groups of D / 4 threads, which take four head dims each; the groups' sums are then added in order.
+constexpr int PAGED_JOIN_THREADS = 512;
+template <int D>
+constexpr int PAGED_JOIN_ROWS = D == 256 ? 2 : 4;
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(D) paged_join_kernel(const PagedAttnParams p) {
-  constexpr int ROWS = 8 * NT;
+__global__ void __launch_bounds__(PAGED_JOIN_THREADS) paged_join_kernel(const __grid_constant__ PagedAttnParams p) {
+  constexpr int R = 8 * NT, ROWS = PAGED_JOIN_ROWS<D>, LANES = D / 4, GROUPS = PAGED_JOIN_THREADS / (LANES * ROWS);
+  __shared__ float4 sums[GROUPS][ROWS][LANES];
+  __shared__ float2 group_ml[GROUPS][ROWS];
+  pdl_trigger();
   pdl_wait();
-  const int c = blockIdx.x, r = blockIdx.y, d = threadIdx.x;
+  const int c = blockIdx.x;
   const int4 cut = *reinterpret_cast<const int4*>(p.cut + 4 * c);
   if (cut.x < 0) return;
-  const int h = cut.y / p.row_blocks, rr = (cut.y % p.row_blocks) * ROWS + r;
-  if (rr >= p.rows) return;
-  const int n = cut.z - c + 1;
-  auto at = [&](int i) { return ((long long)(c + i) * 2 + (i == 0 ? 1 : 0)) * ROWS + r; };
-  float top = -INFINITY;
-  for (int i = 0; i < n; ++i) top = fmaxf(top, p.part_ml[at(i)].x);
-  float acc = 0.f, sum = 0.f;
+  const int n = cut.w - c + 1, lane = threadIdx.x % LANES, row = threadIdx.x / LANES % ROWS, group = threadIdx.x / (LANES * ROWS);
+  const int r = blockIdx.y * ROWS + row, rr = cut.z * R + r;
+  const bool on = r < R && rr < p.rows;          // rows of the last block beyond the unit's were not written
+  auto at = [&](int i) { return ((long long)(c + i) * 2 + (i == 0 ? 1 : 0)) * R + r; };
+  auto weight = [](float m, float top) { return m == top ? 1.f : ex2_approx(m - top); };
+  float m = -INFINITY, sum = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-  for (int i = 0; i < n; ++i) {
+  for (int i = group; i < (on ? n : 0); i += GROUPS) {
     const float2 ml = p.part_ml[at(i)];
-    const float v = p.part_o[at(i) * D + d];
-    if (ml.x != -INFINITY || ml.y != 0.f) {
-      const float a = ml.x == top ? 1.f : ex2_approx(ml.x - top);
-      acc = fmaf(a, v, acc);
-      sum = fmaf(a, ml.y, sum);
-    }
+    const float4 v = *reinterpret_cast<const float4*>(p.part_o + at(i) * D + 4 * lane);
+    const float top = fmaxf(m, ml.x), a = weight(m, top), b = weight(ml.x, top);
+    m = top;
+    sum = sum * a + ml.y * b;
+    acc.x = acc.x * a + v.x * b;
+    acc.y = acc.y * a + v.y * b;
+    acc.z = acc.z * a + v.z * b;
+    acc.w = acc.w * a + v.w * b;
   }
-  reinterpret_cast<T*>(p.o)[paged_row(p, cut.x, h, rr, p.o_seq, p.o_tok, p.o_head) + d] = (T)(sum != 0.f ? acc / sum : 0.f);
+  sums[group][row][lane] = acc;
+  if (lane == 0) group_ml[group][row] = make_float2(m, sum);
+  __syncthreads();
+  if (group || !on) return;
+  float top = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < GROUPS; ++k) top = fmaxf(top, group_ml[k][row].x);
+  sum = 0.f;
+  acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int k = 0; k < GROUPS; ++k) {
+    const float2 ml = group_ml[k][row];
+    const float4 v = sums[k][row][lane];
+    const float b = weight(ml.x, top);
+    sum += ml.y * b;
+    acc.x += v.x * b;
+    acc.y += v.y * b;
+    acc.z += v.z * b;
+    acc.w += v.w * b;
+  }
+  const float inv = sum != 0.f ? 1.f / sum : 0.f;
+  uint2* dst = reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.o) + paged_row(p, cut.x, cut.y, rr, p.o_seq, p.o_tok, p.o_head) + 4 * lane);
+  *dst = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
 }

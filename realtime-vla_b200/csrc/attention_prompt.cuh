@@ -15,8 +15,7 @@
 // Roles: warp 0 = tile lookup and TMA producer, warp 1 = MMA issuer and TMEM owner, warps 2..5 = softmax and epilogue.
 // All mbarrier waits are bounded.
 #pragma once
-#include <cuda_fp16.h>
-#include "common.cuh"
+#include "cache_pages.cuh"
 
 struct PromptAttnParams {
   CUtensorMap tmQ;   // [token][kv head][group head][dim], box 64 x G x 1 x tokens of a tile
@@ -33,9 +32,6 @@ struct PromptAttnParams {
   int causal;
   float scale_log2e;
 };
-
-// Bits VLA_ST_* of the operators in this translation unit: a bounded wait that ran out.
-static __device__ int cache_ops_status;
 
 // Up to 128 columns of head dim a CTA needs half an SM (96 KB of shared memory, 256 TMEM columns), and the two CTAs of an
 // SM fill each other's waits between S, softmax and P V.  Wider heads need the whole SM: two S buffers, so that the next

@@ -54,10 +54,12 @@ bool vectors(const void* p, long long a, long long b) { return aligned(p, 16) &&
 
 constexpr long long INT_TOP = 0x7fffffff;
 
-// Tensor map of a 16-bit tensor, innermost dimension first (contiguous); boxes of 64 elements in 128-byte rows, swizzled.
-// The stride of a dimension of size one is free in the caller's tensor and made valid here.
+// Tensor map of a tensor whose innermost dimension, given first, is contiguous (strides in elements of `size` bytes), for
+// boxes of rows of 128 or 64 bytes with the swizzle of that width.  The stride of a dimension of size one is free in the
+// caller's tensor and made valid here.
 template <int N>
-bool head_map(CUtensorMap* tm, const void* base, int dtype, const long long (&dims)[N], const long long (&strides)[N - 1], const int (&box)[N]) {
+bool tensor_map(CUtensorMap* tm, const void* base, int size, CUtensorMapDataType type, const long long (&dims)[N], const long long (&strides)[N - 1],
+                const int (&box)[N]) {
   EncodeTiledFn fn = get_encode_fn();
   if (!fn) return false;
   cuuint64_t gd[N], gs[N - 1];
@@ -66,10 +68,10 @@ bool head_map(CUtensorMap* tm, const void* base, int dtype, const long long (&di
     gd[i] = (cuuint64_t)dims[i];
     bx[i] = (cuuint32_t)box[i];
     es[i] = 1;
-    if (i > 0) gs[i - 1] = dims[i] > 1 ? (cuuint64_t)strides[i - 1] * 2 : (cuuint64_t)dims[0] * 2;
+    if (i > 0) gs[i - 1] = (cuuint64_t)(dims[i] > 1 ? strides[i - 1] : dims[0]) * size;
   }
-  return fn(tm, dtype == VLA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, N, const_cast<void*>(base), gd, gs, bx, es,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+  return fn(tm, type, N, const_cast<void*>(base), gd, gs, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            box[0] * size == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -77,7 +79,8 @@ bool head_map(CUtensorMap* tm, const void* base, int dtype, const long long (&di
 struct PagedShape {
   int rows, nt, row_blocks;
   long long ctas;
-  size_t workspace;        // bytes; 0: one CTA per unit, nothing to join
+  bool whole;              // units are short enough not to be cut
+  size_t workspace;        // bytes; 0: nothing to join
 };
 PagedShape paged_shape(const vla_paged_attn_desc* d) {
   PagedShape s;
@@ -86,16 +89,12 @@ PagedShape paged_shape(const vla_paged_attn_desc* d) {
   s.nt = s.rows > 8 ? 2 : 1;
   s.row_blocks = (int)((rows + 8 * s.nt - 1) / (8 * s.nt));
   const long long units = (long long)d->n_seqs * d->kv_heads * s.row_blocks;
-  const long long tiles = ((long long)d->width * d->block_size + 15) / 16;      // of a unit, at most
-  if (tiles <= 2 * PAGED_MIN_TILES) {
-    s.ctas = units;
-    s.workspace = 0;
-    return s;
-  }
-  s.ctas = (long long)sm_count() * (d->head_dim == 256 ? 1 : 2);
-  if (units < s.ctas) s.ctas = std::min(s.ctas, (units * tiles + PAGED_MIN_TILES - 1) / PAGED_MIN_TILES);
+  const long long groups = (long long)d->width * d->block_size / 16;            // of 16 tokens in a unit, at most
+  const long long room = (long long)sm_count() * (d->head_dim == 256 ? 1 : 2);  // CTAs that run at once
+  s.whole = groups <= PAGED_WHOLE;
+  s.ctas = std::min(room, s.whole ? units : (units * (groups + PAGED_GAP) + PAGED_MIN_PIECE - 1) / PAGED_MIN_PIECE);
   const size_t rows_kept = (size_t)s.ctas * 2 * 8 * s.nt;
-  s.workspace = rows_kept * ((size_t)d->head_dim * sizeof(float) + sizeof(float2)) + (size_t)s.ctas * 4 * sizeof(int);
+  s.workspace = s.whole ? 0 : rows_kept * ((size_t)d->head_dim * sizeof(float) + sizeof(float2)) + (size_t)s.ctas * 4 * sizeof(int);
   return s;
 }
 
@@ -200,21 +199,29 @@ int vla_op_paged_attention(const vla_paged_attn_desc* d, void* stream) {
     if (!vectors(d->q, d->q_seq_stride, d->q_tok_stride) || d->q_head_stride % 8 || !vectors(d->o, d->o_seq_stride, d->o_tok_stride) || d->o_head_stride % 8)
       return refuse(VLA_ERR_SHAPE, "%s: rows of q and o must start on 16 bytes", who);
     const PagedShape s = paged_shape(d);
-    if (s.ctas > INT_TOP) return refuse(VLA_ERR_LIMIT, "%s: too many sequences", who);
+    if ((double)d->n_seqs * d->kv_heads * s.row_blocks * ((double)d->width * d->block_size / 16 + PAGED_GAP) > 2e9)
+      return refuse(VLA_ERR_LIMIT, "%s: more than 2e9 groups of 16 tokens in the table's rows, times key/value heads and blocks of 8 or 16 rows", who);
     if (s.workspace && (!d->workspace || d->workspace_bytes < s.workspace || !aligned(d->workspace, 16)))
       return refuse(VLA_ERR_STATE, "%s: a workspace of %zu bytes on a 16-byte boundary is needed", who, s.workspace);
     PagedAttnParams p;
     p.q = d->q; p.o = d->o;
     p.q_seq = d->q_seq_stride; p.q_tok = d->q_tok_stride; p.q_head = d->q_head_stride;
     p.o_seq = d->o_seq_stride; p.o_tok = d->o_tok_stride; p.o_head = d->o_head_stride;
-    p.kc = reinterpret_cast<const uint8_t*>(d->k_codes); p.vc = reinterpret_cast<const uint8_t*>(d->v_codes);
+    p.vc = reinterpret_cast<const uint8_t*>(d->v_codes);
     p.ks = d->k_scale; p.vs = d->v_scale;
     p.table = d->block_table; p.table_ld = d->table_stride; p.lens = d->seq_lens;
     p.n_seqs = d->n_seqs; p.n_q = d->n_q; p.group = d->heads / d->kv_heads; p.kv_heads = d->kv_heads;
-    p.rows = s.rows; p.row_blocks = s.row_blocks;
+    p.rows = s.rows; p.row_blocks = s.row_blocks; p.units = d->kv_heads * s.row_blocks;
+    p.per_page_inv = d->block_size == 16 ? 0u : (uint32_t)(((1ull << 32) + d->block_size / 16 - 1) / (d->block_size / 16));
     p.blocks = d->num_blocks; p.block = d->block_size; p.width = d->width;
     p.scale_log2e = d->scale * 1.4426950408889634f;
-    p.split = s.workspace != 0;
+    p.whole = s.whole;
+    p.box_rows = d->block_size % 128 == 0 ? 128 : d->block_size % 64 == 0 ? 64 : d->block_size % 32 == 0 ? 32 : 16;
+    const long long dim = d->head_dim, page = (long long)d->kv_heads * d->block_size;
+    const int width = std::min(d->head_dim, 128);
+    if (!tensor_map(&p.tmK, d->k_codes, 1, CU_TENSOR_MAP_DATA_TYPE_UINT8, {dim, page, d->num_blocks}, {dim, page * dim}, {width, p.box_rows, 1}) ||
+        !tensor_map(&p.tmV, d->v_codes, 1, CU_TENSOR_MAP_DATA_TYPE_UINT8, {dim, page, d->num_blocks}, {dim, page * dim}, {width, p.box_rows, 1}))
+      return refuse(VLA_ERR_SHAPE, "%s: the cache cannot be described by a tensor map", who);
     p.part_o = reinterpret_cast<float*>(d->workspace);
     p.part_ml = reinterpret_cast<float2*>(p.part_o + s.ctas * 2 * 8 * s.nt * d->head_dim);
     p.cut = reinterpret_cast<int*>(p.part_ml + s.ctas * 2 * 8 * s.nt);
@@ -224,8 +231,8 @@ int vla_op_paged_attention(const vla_paged_attn_desc* d, void* stream) {
       constexpr int D = decltype(dim)::value, NT = decltype(nt)::value;
       auto kern = paged_attention_kernel<T, D, NT>;
       cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kern), PagedCfg<D, NT>::SMEM_BYTES);
-      if (e == cudaSuccess) e = launch_ex(kern, dim3((unsigned)s.ctas), dim3(PAGED_THREADS), PagedCfg<D, NT>::SMEM_BYTES, st, 1, false, p);
-      if (e == cudaSuccess && p.split) e = launch_ex(paged_join_kernel<T, D, NT>, dim3((unsigned)s.ctas, std::min(8 * NT, s.rows)), dim3(D), 0, st, 1, true, p);
+      if (e == cudaSuccess) e = launch_ex(kern, dim3((unsigned)s.ctas), dim3(PAGED_THREADS), PagedCfg<D, NT>::SMEM_BYTES, st, 1, true, p);
+      if (e == cudaSuccess && !p.whole) e = launch_ex(paged_join_kernel<T, D, NT>, dim3((unsigned)s.ctas, (std::min(8 * NT, s.rows) + PAGED_JOIN_ROWS<D> - 1) / PAGED_JOIN_ROWS<D>), dim3(PAGED_JOIN_THREADS), 0, st, 1, true, p);
       return launched(who, e);
     };
     auto with = [&](auto type, auto dim) -> int {
@@ -268,10 +275,11 @@ int vla_op_prompt_attention(const vla_prompt_attn_desc* d, void* stream) {
     const void* v = d->tokens_k ? d->v : d->q;
     const long long nk = std::max(d->tokens_k, 1), dim = d->head_dim;
     const int box_v = wide ? PromptCfg<true>::V_ROWS : PromptCfg<false>::V_ROWS;
-    bool made = head_map(&p.tmQ, d->q, d->dtype, {dim, p.group, d->kv_heads, d->tokens_q}, {d->q_head_stride, p.group * d->q_head_stride, d->q_tok_stride},
+    const CUtensorMapDataType type = d->dtype == VLA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    bool made = tensor_map(&p.tmQ, d->q, 2, type, {dim, p.group, d->kv_heads, d->tokens_q}, {d->q_head_stride, p.group * d->q_head_stride, d->q_tok_stride},
                          {64, p.group, 1, p.tile_tokens});
-    made = made && head_map(&p.tmK, k, d->dtype, {dim, d->kv_heads, nk}, {d->k_head_stride, d->k_tok_stride}, {64, 1, 128});
-    made = made && head_map(&p.tmV, v, d->dtype, {dim, d->kv_heads, nk}, {d->v_head_stride, d->v_tok_stride}, {64, 1, box_v});
+    made = made && tensor_map(&p.tmK, k, 2, type, {dim, d->kv_heads, nk}, {d->k_head_stride, d->k_tok_stride}, {64, 1, 128});
+    made = made && tensor_map(&p.tmV, v, 2, type, {dim, d->kv_heads, nk}, {d->v_head_stride, d->v_tok_stride}, {64, 1, box_v});
     if (!made) return refuse(VLA_ERR_SHAPE, "%s: the strides of q, k or v cannot be described by a tensor map", who);
     const long long tiles = d->tokens_q / p.tile_tokens + d->n_seqs;     // at most one tile of each sequence is not full
     if (tiles * d->kv_heads > INT_TOP) return refuse(VLA_ERR_LIMIT, "%s: too many tiles", who);

@@ -3,8 +3,10 @@
 // tokens of a head within a page are one contiguous piece; scales fp32 [blocks][kv heads]; value = code * scale.
 #pragma once
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
 #include "common.cuh"
+
+// Bits VLA_ST_* of the operators in this translation unit: a bounded wait that ran out.
+static __device__ int cache_ops_status;
 
 // ---- block tables and slot maps ------------------------------------------------------------------------------------
 // Request b holds ctx[b] tokens in have = ceil(ctx / bs) blocks and gets n[b] more; it takes want - have blocks, want =
@@ -180,13 +182,29 @@ template <>
 __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
   return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<bf16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
 // two floats -> two e4m3 codes (a in the low byte): nearest, ties to even, saturating at 448; NaN stays NaN
 __device__ __forceinline__ uint32_t to_e4m3x2(float a, float b) {
-  return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  uint16_t w;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(w) : "f"(b), "f"(a));
+  return w;
 }
 // two e4m3 codes -> two floats (exact)
-__device__ __forceinline__ float2 from_e4m3x2(uint32_t w) {
-  return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)w, __NV_E4M3)));
+__device__ __forceinline__ float2 from_e4m3x2(uint32_t two) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)two));
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
 // The smallest 2^e >= 2^-60 that brings amax to 448 = 1.75 * 2^8 or less, from amax's own exponent and mantissa.

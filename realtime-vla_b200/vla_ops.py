@@ -176,15 +176,15 @@ def _rows(t, name, device, dtype, dim):
 
 
 def _cache(cache, device):
+    """Addresses of the four tensors of a cache."""
     k, v, ks, vs = cache
-    if k.dim() != 4 or k.shape != v.shape or ks.shape != k.shape[:2] or vs.shape != ks.shape:
-        _refuse("the tensors of the cache do not fit each other: %s, %s, %s, %s", *map(_tell, cache))
-    f8, f32 = torch.float8_e4m3fn, torch.float32
-    if k.dtype is not f8 or v.dtype is not f8 or ks.dtype is not f32 or vs.dtype is not f32:
-        _refuse("a cache is held as float8_e4m3fn with float32 scales: %s, %s, %s, %s", *map(_tell, cache))
-    for t in cache:
-        if t.device != device or not t.is_contiguous():
-            _refuse("the tensors of the cache must be contiguous and on %s; got %s", device, _tell(t))
+    shape, f8, f32 = k.shape, torch.float8_e4m3fn, torch.float32
+    if not (k.dtype is f8 and v.dtype is f8 and ks.dtype is f32 and vs.dtype is f32 and len(shape) == 4 and v.shape == shape
+            and ks.shape == shape[:2] and vs.shape == shape[:2] and k.device == device and v.device == device
+            and ks.device == device and vs.device == device and k.is_contiguous() and v.is_contiguous()
+            and ks.is_contiguous() and vs.is_contiguous()):
+        _refuse("a cache is float8_e4m3fn codes [blocks, kv_heads, block_size, head_dim] twice and float32 scales [blocks, kv_heads] "
+                "twice, all contiguous and on %s; got %s, %s, %s, %s", device, *map(_tell, cache))
     return k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr()
 
 
@@ -196,7 +196,7 @@ def _type(t, name):
 
 
 def _enqueue(fn, desc, device):
-    stream = torch.cuda.current_stream(device).cuda_stream
+    stream = torch._C._cuda_getCurrentRawStream(device.index)      # current_stream(device).cuda_stream in 0.1 instead of 2.2 us
     if torch.cuda.current_device() == device.index:
         rc = fn(C.byref(desc), stream)
     else:
@@ -219,8 +219,12 @@ def block_plan(context_lens, new_lens, block_table, free_blocks, *, block_size, 
         _refuse("context_lens, new_lens, block_table (and first_free) do not fit each other")
     if total_new < 0:
         _refuse("total_new is negative")
-    make = context_lens.new_empty
-    slots, positions, cu, lens, counts = make(total_new), make(total_new), make(n + 1), make(n), make(3)
+    pad = -total_new % 4                   # one allocation, of which slots and positions start on 16 bytes
+    out = context_lens.new_empty(2 * (total_new + pad) + 2 * n + 4)
+    if pad:
+        slots, _, positions, _, cu, lens, counts = out.split_with_sizes([total_new, pad, total_new, pad, n + 1, n, 3])
+    else:
+        slots, positions, cu, lens, counts = out.split_with_sizes([total_new, total_new, n + 1, n, 3])
     d = _capi.BlockPlanDesc(_whole(context_lens, "context_lens", dev), _whole(new_lens, "new_lens", dev), n,
                             _whole(block_table, "block_table", dev, 2), block_table.shape[1],
                             block_table.stride(0) if n > 1 else block_table.shape[1],

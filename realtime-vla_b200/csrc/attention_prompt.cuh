@@ -242,20 +242,24 @@ __global__ void __launch_bounds__(PromptCfg<WIDE>::THREADS, WIDE ? 1 : 2) prompt
       const int k_steps = (p.dim + 15) / 16;
       const uint32_t idesc_o = idesc | (1u << 16) | ((uint32_t)(k_steps * 2) << 17);      // N = head dim, B MN-major
       bool ok = mbar_wait(q_full, 0, abort_flag);
+      // The loops are unrolled over what the tile can hold, with the descriptors as constants from a base: formed step by
+      // step, an MMA took this one thread about 140 clocks to issue, more than twice what it runs for.
+      const uint64_t q_desc = attn_desc_sw128(sQ), k_desc = attn_desc_sw128(sRing), v_desc = prompt_desc_mn(sRing, C::V_ROWS * 128);
       auto issue_s = [&](int c) {
         // the last chunk multiplies only the keys that some row sees, rounded up to 16
         const int keys16 = (min(lim_max - c * 128, 128) + 15) / 16;
-        const uint32_t idesc_s = idesc | ((uint32_t)(keys16 * 2) << 17);
+        const uint32_t idesc_s = idesc | ((uint32_t)(keys16 * 2) << 17), d = tmem + (c % C::AHEAD) * 128;
+#pragma unroll
         for (int u = 0; u < C::UNITS; ++u) {
           const int pos = k_pos(c) + u, s = pos % C::STAGES;
           ok = ok && mbar_wait(full(s), (uint32_t)(pos / C::STAGES) & 1u, abort_flag);
           if (!ok) return;
           tc_fence_after();
-          for (int ks = u * 8; ks < min(k_steps, u * 8 + 8); ++ks) {
-            const uint64_t da = attn_desc_sw128(sQ + (ks >> 2) * C::BOX_BYTES) + 2 * (ks & 3);
-            const uint64_t db = attn_desc_sw128(sRing + s * C::SLOT_BYTES + ((ks >> 2) - 2 * u) * C::BOX_BYTES) + 2 * (ks & 3);
-            umma_bf16(tmem + (c % C::AHEAD) * 128, da, db, idesc_s, ks != 0);
-          }
+          const uint64_t kd = k_desc + s * (C::SLOT_BYTES / 16);
+#pragma unroll
+          for (int ks = 0; ks < 8; ++ks)
+            if (u * 8 + ks < k_steps)
+              umma_bf16(d, q_desc + (u * 2 + ks / 4) * (C::BOX_BYTES / 16) + 2 * (ks % 4), kd + (ks / 4) * (C::BOX_BYTES / 16) + 2 * (ks % 4), idesc_s, (u | ks) != 0);
           umma_commit(empty(s));
         }
         umma_commit(s_full(c % C::AHEAD));
@@ -265,14 +269,17 @@ __global__ void __launch_bounds__(PromptCfg<WIDE>::THREADS, WIDE ? 1 : 2) prompt
         const int buf = c % C::AHEAD;
         ok = mbar_wait(p_ready(buf), (uint32_t)(c / C::AHEAD) & 1u, abort_flag);
         const int keys16 = (min(lim_max - c * 128, 128) + 15) / 16;
+#pragma unroll
         for (int u = 0; u < C::UNITS; ++u) {
           const int pos = v_pos(c) + u, s = pos % C::STAGES;
           ok = ok && mbar_wait(full(s), (uint32_t)(pos / C::STAGES) & 1u, abort_flag);
           if (!ok) break;
           tc_fence_after();
-          const uint64_t db = prompt_desc_mn(sRing + s * C::SLOT_BYTES, C::V_ROWS * 128);
-          for (int kk = 0; kk < min(keys16 - u * (C::V_ROWS / 16), C::V_ROWS / 16); ++kk)
-            umma_ts(tmem + C::O_COL, tmem + buf * 128 + (u * (C::V_ROWS / 16) + kk) * 8, db + 128 * kk, idesc_o, (c | u | kk) != 0);
+          const uint64_t vd = v_desc + s * (C::SLOT_BYTES / 16);
+          const uint32_t p_at = tmem + buf * 128 + u * (C::V_ROWS / 2);
+#pragma unroll
+          for (int kk = 0; kk < C::V_ROWS / 16; ++kk)
+            if (u * (C::V_ROWS / 16) + kk < keys16) umma_ts(tmem + C::O_COL, p_at + kk * 8, vd + 128 * kk, idesc_o, (c | u | kk) != 0);
           umma_commit(empty(s));
         }
         if (!ok) break;

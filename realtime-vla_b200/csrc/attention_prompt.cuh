@@ -5,7 +5,7 @@
 // A row with L_i <= 0 is zero.  heads / kv_heads consecutive query heads share a key/value head.
 //
 // One CTA = one tile of 128 rows: the G = heads / kv_heads query heads of 128 / G consecutive tokens, which share their
-// keys, so that short prompts fill tiles too and a causal tile's diagonal is only 128 / G keys wide.  Chunks of 128 keys:
+// keys, so that short prompts fill tiles too and a causal tile's diagonal is only 128 / G keys wide.  Chunks of 128 (64) keys:
 //     S[128 x 128]  = Q . K_chunk^T       tcgen05.mma, both operands K-major in shared memory
 //     P             = exp2(S scale - m)   one thread per row, straight from TMEM, written back over S as 16-bit pairs
 //     O[128 x dim] += P . V_chunk         tcgen05.mma, A = P in TMEM, B = V as it lies in memory (MN-major), so V needs
@@ -19,7 +19,7 @@
 
 struct PromptAttnParams {
   CUtensorMap tmQ;   // [token][kv head][group head][dim], box 64 x G x 1 x tokens of a tile
-  CUtensorMap tmK;   // [token][kv head][dim], box 64 x 1 x 128
+  CUtensorMap tmK;   // [token][kv head][dim], box 64 x 1 x KEYS
   CUtensorMap tmV;   // the same, box 64 x 1 x V_ROWS
   const void* v;
   void* o;
@@ -33,22 +33,24 @@ struct PromptAttnParams {
   float scale_log2e;
 };
 
-// Up to 128 columns of head dim a CTA needs half an SM (96 KB of shared memory, 256 TMEM columns), and the two CTAs of an
-// SM fill each other's waits between S, softmax and P V.  Wider heads need the whole SM: two S buffers, so that the next
-// chunk's S is there when the softmax has finished a chunk, and K and V in half chunks of 32 KB.
+// Two S buffers, so that the next chunk's S is there when the softmax has finished a chunk.  Up to 128 columns of head dim a
+// CTA takes half an SM (96 KB of shared memory, 256 TMEM columns) with chunks of 64 keys, and the two CTAs of an SM
+// share its tensor core and its exponentials; wider heads need the whole SM, with chunks of 128 keys whose K and V come in
+// halves of 32 KB.
 template <bool WIDE>
 struct PromptCfg {
   static constexpr int BOXES = WIDE ? 4 : 2;              // 64-column boxes of head dim, at most
-  static constexpr int AHEAD = WIDE ? 2 : 1;              // S buffers = chunks of S in flight
+  static constexpr int KEYS = WIDE ? 128 : 64;            // keys per chunk
+  static constexpr int AHEAD = 2;                         // S buffers = chunks of S in flight
   static constexpr int UNITS = WIDE ? 2 : 1;              // ring slots per K or V chunk
-  static constexpr int STAGES = WIDE ? 5 : 2;
-  static constexpr int V_ROWS = 128 / UNITS;
-  static constexpr int BOX_BYTES = 128 * 128;             // 64 columns x 128 rows
-  static constexpr int SLOT_BYTES = 2 * BOX_BYTES;        // K: 2 boxes x 128 keys; V: BOXES boxes x V_ROWS keys
-  static constexpr int Q_BYTES = BOXES * BOX_BYTES;
+  static constexpr int STAGES = WIDE ? 5 : 4;
+  static constexpr int V_ROWS = KEYS / UNITS;
+  static constexpr int Q_BOX = 128 * 128, K_BOX = KEYS * 128, V_BOX = V_ROWS * 128;   // bytes of 64 columns x rows
+  static constexpr int SLOT_BYTES = 2 * K_BOX;            // K: 2 boxes x KEYS; V: BOXES boxes x V_ROWS keys
+  static constexpr int Q_BYTES = BOXES * Q_BOX;
   static constexpr int SMEM_BYTES = Q_BYTES + STAGES * SLOT_BYTES + 256 + 1024;
   static constexpr int TMEM_COLS = WIDE ? 512 : 256;      // S buffers, then O
-  static constexpr int O_COL = AHEAD * 128;
+  static constexpr int O_COL = AHEAD * KEYS;
   static constexpr int THREADS = 192;
 };
 
@@ -71,6 +73,20 @@ __device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64
 // 64 columns `box_bytes` further.
 __device__ __forceinline__ uint64_t prompt_desc_mn(uint32_t smem_addr, uint32_t box_bytes) {
   return (uint64_t)((smem_addr & 0x3FFFF) >> 4) | ((uint64_t)(box_bytes >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// two fp32 operations an instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t&>(d)) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
 }
 
 template <typename T>
@@ -188,7 +204,7 @@ __global__ void __launch_bounds__(PromptCfg<WIDE>::THREADS, WIDE ? 1 : 2) prompt
   const int last_tok = min(tok0 + p.tile_tokens, nq) - 1;
   auto limit_of = [&](int tok) { return p.causal ? min(max(tok + nk - nq + 1, 0), nk) : nk; };
   const int lim_min = seq >= 0 ? limit_of(tok0) : 0, lim_max = seq >= 0 ? limit_of(last_tok) : 0;
-  const int n_chunks = (lim_max + 127) / 128;
+  const int n_chunks = (lim_max + C::KEYS - 1) / C::KEYS;
   const int boxes = (p.dim + 63) / 64;
   // position of a K or V chunk in the ring's order of use: K_0 .. K_{AHEAD-1}, then V_c, K_{c+AHEAD} in turn
   auto k_pos = [&](int c) { return C::UNITS * (c < C::AHEAD ? c : 2 * c - C::AHEAD + 1); };
@@ -198,7 +214,7 @@ __global__ void __launch_bounds__(PromptCfg<WIDE>::THREADS, WIDE ? 1 : 2) prompt
     if (lane == 0 && n_chunks > 0) {
       const int rows = p.group * p.tile_tokens;
       mbar_expect_tx(q_full, boxes * rows * 128);
-      for (int x = 0; x < boxes; ++x) tma_load_4d(sQ + x * C::BOX_BYTES, &p.tmQ, q_full, x * 64, 0, kvh, q0 + tok0);
+      for (int x = 0; x < boxes; ++x) tma_load_4d(sQ + x * C::Q_BOX, &p.tmQ, q_full, x * 64, 0, kvh, q0 + tok0);
       bool ok = true;
       auto slot_free = [&](int pos) {
         return pos < C::STAGES || mbar_wait(empty(pos % C::STAGES), (uint32_t)(pos / C::STAGES - 1) & 1u, abort_flag);
@@ -209,14 +225,10 @@ __global__ void __launch_bounds__(PromptCfg<WIDE>::THREADS, WIDE ? 1 : 2) prompt
           const int pos = k_pos(c) + u, s = pos % C::STAGES;
           ok = slot_free(pos);
           if (!ok) return;
-          const int b0 = u * 2, nb = min(boxes - b0, 2);
-          if (nb <= 0) {                           // heads of at most 128 columns in the wide kernel do not occur
-            mbar_arrive(full(s));
-            continue;
-          }
-          mbar_expect_tx(full(s), nb * C::BOX_BYTES);
+          const int b0 = u * 2, nb = min(boxes - b0, 2);     // at least one: wider heads than 128 have three boxes or four
+          mbar_expect_tx(full(s), nb * C::K_BOX);
           for (int x = 0; x < nb; ++x)
-            tma_load_3d(sRing + s * C::SLOT_BYTES + x * C::BOX_BYTES, &p.tmK, full(s), (b0 + x) * 64, kvh, k0 + c * 128, pol);
+            tma_load_3d(sRing + s * C::SLOT_BYTES + x * C::K_BOX, &p.tmK, full(s), (b0 + x) * 64, kvh, k0 + c * C::KEYS, pol);
         }
       };
       auto load_v = [&](int c) {
@@ -224,9 +236,9 @@ __global__ void __launch_bounds__(PromptCfg<WIDE>::THREADS, WIDE ? 1 : 2) prompt
           const int pos = v_pos(c) + u, s = pos % C::STAGES;
           ok = slot_free(pos);
           if (!ok) return;
-          mbar_expect_tx(full(s), boxes * C::V_ROWS * 128);
+          mbar_expect_tx(full(s), boxes * C::V_BOX);
           for (int x = 0; x < boxes; ++x)
-            tma_load_3d(sRing + s * C::SLOT_BYTES + x * C::V_ROWS * 128, &p.tmV, full(s), x * 64, kvh, k0 + c * 128 + u * C::V_ROWS, pol);
+            tma_load_3d(sRing + s * C::SLOT_BYTES + x * C::V_BOX, &p.tmV, full(s), x * 64, kvh, k0 + c * C::KEYS + u * C::V_ROWS, pol);
         }
       };
       for (int c = 0; c < min(C::AHEAD, n_chunks); ++c) load_k(c);
@@ -244,48 +256,70 @@ __global__ void __launch_bounds__(PromptCfg<WIDE>::THREADS, WIDE ? 1 : 2) prompt
       bool ok = mbar_wait(q_full, 0, abort_flag);
       // The loops are unrolled over what the tile can hold, with the descriptors as constants from a base: formed step by
       // step, an MMA took this one thread about 140 clocks to issue, more than twice what it runs for.
-      const uint64_t q_desc = attn_desc_sw128(sQ), k_desc = attn_desc_sw128(sRing), v_desc = prompt_desc_mn(sRing, C::V_ROWS * 128);
+      const uint64_t q_desc = attn_desc_sw128(sQ), k_desc = attn_desc_sw128(sRing), v_desc = prompt_desc_mn(sRing, C::V_BOX);
+      auto wait_units = [&](int pos0) {
+        for (int u = 0; u < C::UNITS; ++u) {
+          const int pos = pos0 + u;
+          ok = ok && mbar_wait(full(pos % C::STAGES), (uint32_t)(pos / C::STAGES) & 1u, abort_flag);
+        }
+      };
       auto issue_s = [&](int c) {
         // the last chunk multiplies only the keys that some row sees, rounded up to 16
-        const int keys16 = (min(lim_max - c * 128, 128) + 15) / 16;
-        const uint32_t idesc_s = idesc | ((uint32_t)(keys16 * 2) << 17), d = tmem + (c % C::AHEAD) * 128;
+        const int keys16 = (min(lim_max - c * C::KEYS, C::KEYS) + 15) / 16;
+        const uint32_t idesc_s = idesc | ((uint32_t)(keys16 * 2) << 17), d = tmem + (c % C::AHEAD) * C::KEYS;
 #pragma unroll
         for (int u = 0; u < C::UNITS; ++u) {
-          const int pos = k_pos(c) + u, s = pos % C::STAGES;
-          ok = ok && mbar_wait(full(s), (uint32_t)(pos / C::STAGES) & 1u, abort_flag);
-          if (!ok) return;
-          tc_fence_after();
+          const int s = (k_pos(c) + u) % C::STAGES;
           const uint64_t kd = k_desc + s * (C::SLOT_BYTES / 16);
+          const int mine = k_steps - u * 8;     // steps of 16 head dims in this slot
+          auto step = [&](int ks) {
+            umma_bf16(d, q_desc + (u * 2 + ks / 4) * (C::Q_BOX / 16) + 2 * (ks % 4), kd + (ks / 4) * (C::K_BOX / 16) + 2 * (ks % 4), idesc_s, (u | ks) != 0);
+          };
+          if (mine >= 8) {
 #pragma unroll
-          for (int ks = 0; ks < 8; ++ks)
-            if (u * 8 + ks < k_steps)
-              umma_bf16(d, q_desc + (u * 2 + ks / 4) * (C::BOX_BYTES / 16) + 2 * (ks % 4), kd + (ks / 4) * (C::BOX_BYTES / 16) + 2 * (ks % 4), idesc_s, (u | ks) != 0);
+            for (int ks = 0; ks < 8; ++ks) step(ks);
+          } else {
+#pragma unroll 1
+            for (int ks = 0; ks < mine; ++ks) step(ks);
+          }
           umma_commit(empty(s));
         }
         umma_commit(s_full(c % C::AHEAD));
       };
-      for (int c = 0; c < min(C::AHEAD, n_chunks) && ok; ++c) issue_s(c);
+      for (int c = 0; c < min(C::AHEAD, n_chunks) && ok; ++c) {
+        wait_units(k_pos(c));
+        tc_fence_after();
+        if (ok) issue_s(c);
+      }
       for (int c = 0; c < n_chunks && ok; ++c) {
+        // What the loads bring is waited for first, so that nothing but P stands before the MMAs: V of this chunk, and K of
+        // the chunk whose S goes over this one's P (its slot was that of a K whose S is long formed, not of this V).
         const int buf = c % C::AHEAD;
-        ok = mbar_wait(p_ready(buf), (uint32_t)(c / C::AHEAD) & 1u, abort_flag);
-        const int keys16 = (min(lim_max - c * 128, 128) + 15) / 16;
+        const bool more = c + C::AHEAD < n_chunks;
+        wait_units(v_pos(c));
+        if (more) wait_units(k_pos(c + C::AHEAD));
+        ok = ok && mbar_wait(p_ready(buf), (uint32_t)(c / C::AHEAD) & 1u, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        const int keys16 = (min(lim_max - c * C::KEYS, C::KEYS) + 15) / 16;
 #pragma unroll
         for (int u = 0; u < C::UNITS; ++u) {
-          const int pos = v_pos(c) + u, s = pos % C::STAGES;
-          ok = ok && mbar_wait(full(s), (uint32_t)(pos / C::STAGES) & 1u, abort_flag);
-          if (!ok) break;
-          tc_fence_after();
+          const int s = (v_pos(c) + u) % C::STAGES;
           const uint64_t vd = v_desc + s * (C::SLOT_BYTES / 16);
-          const uint32_t p_at = tmem + buf * 128 + u * (C::V_ROWS / 2);
+          const uint32_t p_at = tmem + buf * C::KEYS + u * (C::V_ROWS / 2);
+          auto step = [&](int kk) { umma_ts(tmem + C::O_COL, p_at + kk * 8, vd + 128 * kk, idesc_o, (c | u | kk) != 0); };
+          if (keys16 >= 4 * u + 4) {
 #pragma unroll
-          for (int kk = 0; kk < C::V_ROWS / 16; ++kk)
-            if (u * (C::V_ROWS / 16) + kk < keys16) umma_ts(tmem + C::O_COL, p_at + kk * 8, vd + 128 * kk, idesc_o, (c | u | kk) != 0);
+            for (int kk = 0; kk < 4; ++kk) step(kk);
+          } else {
+#pragma unroll 1
+            for (int kk = 0; kk < keys16 - 4 * u; ++kk) step(kk);
+          }
           umma_commit(empty(s));
         }
-        if (!ok) break;
         umma_commit(o_done(c & 1));
         // S of chunk c + AHEAD goes over P of chunk c: the tensor core takes MMAs in the order of their issue
-        if (c + C::AHEAD < n_chunks) issue_s(c + C::AHEAD);
+        if (more) issue_s(c + C::AHEAD);
       }
     }
     __syncwarp();
@@ -300,61 +334,28 @@ __global__ void __launch_bounds__(PromptCfg<WIDE>::THREADS, WIDE ? 1 : 2) prompt
     bool ok = true;
     for (int c = 0; c < n_chunks && ok; ++c) {
       const int buf = c % C::AHEAD;
-      const int lo = max(lim_min - c * 128, 0), hi = (min(lim_max - c * 128, 128) + 15) / 16 * 16;
-      if (lo < hi) {
-        // Keys that not every row sees (the causal diagonal) or that none does (behind the last key, up to the MMA's
-        // step of 16): their P is zero in the rows that do not see them, but zero times NaN or infinity is NaN.  Such
-        // values are cleared in shared memory; the epilogue gives them back to the rows that see them.
-        for (int u = 0; u < C::UNITS; ++u) {
-          const int pos = v_pos(c) + u, s = pos % C::STAGES;
-          ok = ok && __all_sync(0xffffffffu, mbar_wait(full(s), (uint32_t)(pos / C::STAGES) & 1u, abort_flag));
-          if (!ok) break;
-          const int r0 = max(lo - u * C::V_ROWS, 0), r1 = min(hi - u * C::V_ROWS, C::V_ROWS);
-          const int tail = lim_max - c * 128 - u * C::V_ROWS;      // rows from here on are seen by none
-          for (int x = 0; x < boxes; ++x) {
-            uint8_t* box = ring + s * C::SLOT_BYTES + x * C::V_ROWS * 128;
-            for (int i = r0 * 8 + r; i < r1 * 8; i += 128) {
-              uint4* at = reinterpret_cast<uint4*>(box + i * 16);
-              if (i >= tail * 8) {
-                *at = make_uint4(0u, 0u, 0u, 0u);
-                continue;
-              }
-              const uint4 w4 = *at;
-              uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-              bool bad = false;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                if ((w[e] & H::EXP_LO) == H::EXP_LO) { w[e] &= 0xffff0000u; bad = true; }
-                if ((w[e] >> 16 & H::EXP_LO) == H::EXP_LO) { w[e] &= 0xffffu; bad = true; }
-              }
-              if (bad) {
-                *at = make_uint4(w[0], w[1], w[2], w[3]);
-                *poison = 1;
-              }
-            }
-          }
-        }
-        if (!ok) break;
-        fence_proxy_async_shared();
-      }
       ok = __all_sync(0xffffffffu, mbar_wait(s_full(buf), (uint32_t)(c / C::AHEAD) & 1u, abort_flag));
       if (!ok) break;
       tc_fence_after();
-      const uint32_t ts = tmem + lane_off + buf * 128;
-      float s[128];
+      const uint32_t ts = tmem + lane_off + buf * C::KEYS;
+      float s[C::KEYS];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) tmem_ld32(ts + 32 * g, reinterpret_cast<uint32_t*>(s) + 32 * g);
+      for (int g = 0; g < C::KEYS / 32; ++g) tmem_ld32(ts + 32 * g, reinterpret_cast<uint32_t*>(s) + 32 * g);
       tmem_ld_wait();
-      const int vis = limit - c * 128;
-      if (!__all_sync(0xffffffffu, vis >= 128)) {
+      const int vis = limit - c * C::KEYS;
+      if (!__all_sync(0xffffffffu, vis >= C::KEYS)) {
 #pragma unroll
-        for (int j = 0; j < 128; ++j)
+        for (int j = 0; j < C::KEYS; ++j)
           if (j >= vis) s[j] = -INFINITY;
       }
-      float mx[4] = {s[0], s[1], s[2], s[3]};
+      float mx[8];
 #pragma unroll
-      for (int j = 4; j < 128; ++j) mx[j & 3] = fmaxf(mx[j & 3], s[j]);
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2e;
+      for (int j = 0; j < 8; ++j) mx[j] = s[j];
+#pragma unroll
+      for (int j = 8; j < C::KEYS; j += 16)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) mx[k] = fmaxf(fmaxf(mx[k], s[j + k]), j + 8 + k < C::KEYS ? s[j + 8 + k] : s[j + k]);   // three inputs an instruction
+      const float top = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7]))) * p.scale_log2e;
       // the first chunk sets the maximum; later it moves when a row of this warp has outgrown it by 2^8
       if (__any_sync(0xffffffffu, top > m + 8.f)) {
         const float m_new = fmaxf(m, top);
@@ -377,21 +378,59 @@ __global__ void __launch_bounds__(PromptCfg<WIDE>::THREADS, WIDE ? 1 : 2) prompt
         m = m_new;
       }
       const float sub = m == -INFINITY ? 0.f : m;        // a row that has seen nothing yet
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      const float2 scale2 = make_float2(p.scale_log2e, p.scale_log2e), sub2 = make_float2(-sub, -sub);
+      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
+      for (int g = 0; g < C::KEYS / 64; ++g) {
         uint32_t w[32];
 #pragma unroll
         for (int j = 0; j < 64; j += 2) {
-          const float a = ex2_approx(fmaf(s[64 * g + j], p.scale_log2e, -sub));
-          const float b = ex2_approx(fmaf(s[64 * g + j + 1], p.scale_log2e, -sub));
-          sum[j & 2] += a;
-          sum[(j & 2) + 1] += b;
-          w[j >> 1] = H::pack(a, b);
+          float2 e = fma2(make_float2(s[64 * g + j], s[64 * g + j + 1]), scale2, sub2);
+          e.x = ex2_approx(e.x);
+          e.y = ex2_approx(e.y);
+          sum[j >> 1 & 1] = add2(sum[j >> 1 & 1], e);
+          w[j >> 1] = H::pack(e.x, e.y);
         }
         tmem_st32(ts + 32 * g, w);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+      if ((c + 1) * C::KEYS > lim_min) {
+        // Keys that not every row sees (the causal diagonal) or that none does (behind the last key, up to the MMA's step of
+        // 16): their P is zero in the rows that do not see them, but zero times NaN or infinity is NaN.  Such values are
+        // cleared in shared memory; the epilogue gives them back to the rows that see them.  S of this chunk and the P V
+        // before it are over, so V's slots are past their earlier uses and a look at them cannot take one for this use.
+        // After the exponentials, so that the wait for that P V runs under them.
+        if (c > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_done((c - 1) & 1), (uint32_t)((c - 1) >> 1) & 1u, abort_flag));
+        const int at = v_pos(c), s0 = at % C::STAGES, s1 = (at + C::UNITS - 1) % C::STAGES;
+#pragma unroll
+        for (int u = 0; u < C::UNITS; ++u)
+          ok = ok && __all_sync(0xffffffffu, mbar_wait(full(u ? s1 : s0), (uint32_t)((at + u) / C::STAGES) & 1u, abort_flag));
+        if (!ok) break;
+        const int lo = max(lim_min - c * C::KEYS, 0), tail = lim_max - c * C::KEYS, hi = (min(tail, C::KEYS) + 15) / 16 * 16;
+        constexpr int PIECES = C::BOXES * 8;           // of a key's row, 16 bytes each
+        const int piece = r % PIECES;
+        uint8_t* const column = ring + (piece >> 3) * C::V_BOX + (piece & 7) * 16;
+        if (piece >> 3 < boxes) {
+#pragma unroll 2
+          for (int j = lo + r / PIECES; j < hi; j += 128 / PIECES) {
+            uint4* const w4 = reinterpret_cast<uint4*>(column + (j < C::V_ROWS ? s0 : s1) * C::SLOT_BYTES + j % C::V_ROWS * 128);
+            uint4 w = *w4;
+            // the exponents inverted: a half whose bits were all ones is zero, and taking one from it sets its top bit
+            auto bad = [](uint32_t b) { return ((~b & H::EXP_LO * 0x10001u) - 0x10001u) & 0x80008000u; };
+            if (j >= tail) {
+              *w4 = make_uint4(0u, 0u, 0u, 0u);
+            } else if (bad(w.x) | bad(w.y) | bad(w.z) | bad(w.w)) {
+              auto clean = [](uint32_t b) {
+                return ((b & H::EXP_LO) == H::EXP_LO ? 0u : b & 0xffffu) | ((b >> 16 & H::EXP_LO) == H::EXP_LO ? 0u : b & 0xffff0000u);
+              };
+              *w4 = make_uint4(clean(w.x), clean(w.y), clean(w.z), clean(w.w));
+              *poison = 1;
+            }
+          }
+        }
+        fence_proxy_async_shared();
+        __syncwarp();
+      }
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(p_ready(buf));
@@ -403,7 +442,10 @@ __global__ void __launch_bounds__(PromptCfg<WIDE>::THREADS, WIDE ? 1 : 2) prompt
     if (ok && seq >= 0) {
       const float inv = l != 0.f ? 1.f / l : 0.f;         // nothing seen: O is zero or was never written
       const bool any_poison = *poison != 0;
-      T* orow = reinterpret_cast<T*>(p.o) + (long long)(q0 + tok) * p.o_tok + (long long)(kvh * p.group + r % p.group) * p.o_head;
+      const long long row_at = (long long)(q0 + tok) * p.o_tok + (long long)(kvh * p.group + r % p.group) * p.o_head;
+      const uint32_t rows_ok = __ballot_sync(0xffffffffu, row_ok);
+      // Through Q's shared memory (its last product is over), so that rows leave as whole lines: stored by the thread that
+      // has the row, 16 bytes of 32 rows an instruction, the end of a tile of 256 head dims took 5800 clocks.
 #pragma unroll 1
       for (int d = 0; d < p.dim; d += 32) {
         uint32_t v[32];
@@ -411,26 +453,35 @@ __global__ void __launch_bounds__(PromptCfg<WIDE>::THREADS, WIDE ? 1 : 2) prompt
           tmem_ld32(tmem + lane_off + C::O_COL + d, v);
           tmem_ld_wait();
         }
-        if (row_ok) {
-          float f[32];
+        float f[32];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) f[j] = l != 0.f ? __uint_as_float(v[j]) * inv : 0.f;
-          if (any_poison) {
-            for (int key = lim_min; key < limit; ++key) {
-              const unsigned short* vr = reinterpret_cast<const unsigned short*>(p.v) + (long long)(k0 + key) * p.v_tok + kvh * p.v_head + d;
+        for (int j = 0; j < 32; ++j) f[j] = l != 0.f ? __uint_as_float(v[j]) * inv : 0.f;
+        if (any_poison) {
+#pragma unroll 1
+          for (int key = lim_min; key < limit; ++key) {
+            const unsigned short* vr = reinterpret_cast<const unsigned short*>(p.v) + (long long)(k0 + key) * p.v_tok + kvh * p.v_head + d;
 #pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (d + j < p.dim && (vr[j] & H::EXP_LO) == H::EXP_LO) f[j] += H::value(vr[j]);
-            }
+            for (int j = 0; j < 32; ++j)
+              if (d + j < p.dim && (vr[j] & H::EXP_LO) == H::EXP_LO) f[j] += H::value(vr[j]);
           }
-#pragma unroll
-          for (int j = 0; j < 32; j += 8) {
-            if (d + j < p.dim)
-              *reinterpret_cast<uint4*>(orow + d + j) = make_uint4(H::pack(f[j], f[j + 1]), H::pack(f[j + 2], f[j + 3]),
-                                                                   H::pack(f[j + 4], f[j + 5]), H::pack(f[j + 6], f[j + 7]));
-          }
+          __syncwarp();
         }
-        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 32; j += 8)
+          *reinterpret_cast<uint4*>(smem_raw + pad + ((d + j) >> 6) * C::Q_BOX + r * 128 + ((((d + j) >> 3 & 7) ^ (r & 7)) << 4)) =
+              make_uint4(H::pack(f[j], f[j + 1]), H::pack(f[j + 2], f[j + 3]), H::pack(f[j + 4], f[j + 5]), H::pack(f[j + 6], f[j + 7]));
+      }
+      __syncwarp();
+      constexpr int LANES = C::BOXES * 8;        // per row, 16 bytes each
+      const int piece = lane % LANES;
+      const uint8_t* from = smem_raw + pad + (piece >> 3) * C::Q_BOX;
+#pragma unroll 4
+      for (int k = lane / LANES; k < 32; k += 32 / LANES) {
+        const long long at = __shfl_sync(0xffffffffu, row_at, k);
+        const int rr = quarter * 32 + k;
+        if ((rows_ok >> k & 1) && piece * 8 < p.dim)
+          *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.o) + at + piece * 8) =
+              *reinterpret_cast<const uint4*>(from + rr * 128 + (((piece & 7) ^ (rr & 7)) << 4));
       }
     }
   }

@@ -274,12 +274,11 @@ int vla_op_prompt_attention(const vla_prompt_attn_desc* d, void* stream) {
     const void* k = d->tokens_k ? d->k : d->q;
     const void* v = d->tokens_k ? d->v : d->q;
     const long long nk = std::max(d->tokens_k, 1), dim = d->head_dim;
-    const int box_v = wide ? PromptCfg<true>::V_ROWS : PromptCfg<false>::V_ROWS;
     const CUtensorMapDataType type = d->dtype == VLA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     bool made = tensor_map(&p.tmQ, d->q, 2, type, {dim, p.group, d->kv_heads, d->tokens_q}, {d->q_head_stride, p.group * d->q_head_stride, d->q_tok_stride},
                          {64, p.group, 1, p.tile_tokens});
-    made = made && tensor_map(&p.tmK, k, 2, type, {dim, d->kv_heads, nk}, {d->k_head_stride, d->k_tok_stride}, {64, 1, 128});
-    made = made && tensor_map(&p.tmV, v, 2, type, {dim, d->kv_heads, nk}, {d->v_head_stride, d->v_tok_stride}, {64, 1, box_v});
+    made = made && tensor_map(&p.tmK, k, 2, type, {dim, d->kv_heads, nk}, {d->k_head_stride, d->k_tok_stride}, {64, 1, wide ? PromptCfg<true>::KEYS : PromptCfg<false>::KEYS});
+    made = made && tensor_map(&p.tmV, v, 2, type, {dim, d->kv_heads, nk}, {d->v_head_stride, d->v_tok_stride}, {64, 1, 64});
     if (!made) return refuse(VLA_ERR_SHAPE, "%s: the strides of q, k or v cannot be described by a tensor map", who);
     const long long tiles = d->tokens_q / p.tile_tokens + d->n_seqs;     // at most one tile of each sequence is not full
     if (tiles * d->kv_heads > INT_TOP) return refuse(VLA_ERR_LIMIT, "%s: too many tiles", who);

@@ -129,6 +129,20 @@ def test_prompt_keys_unlike_queries(dim, lens_q, lens_k):
         check_prompts(q, k, v, cq, ck, vla_ops.prompt_attention(q, k, v, cq, ck, causal=causal), causal)
 
 
+@pytest.mark.parametrize("heads,kv,dim", [(16, 8, 128), (8, 8, 64), (8, 4, 256)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_prompt_many_sequences(heads, kv, dim, causal):
+    """Far more tiles than SMs: every CTA takes many, of one chunk and of several, with one live tile and with two."""
+    import vla_ops
+    d = dev()
+    lens = [(37 * i) % 61 for i in range(300)] + [700, 1, 260]
+    keys = [n + (i % 5) * 70 for i, n in enumerate(lens)]
+    q, k, v, cq, ck = prompts(7, lens, keys, heads, kv, dim, torch.bfloat16, d)
+    for _ in range(3):
+        out = vla_ops.prompt_attention(q, k, v, cq, ck, causal=causal)
+    check_prompts(q, k, v, cq, ck, out, causal)
+
+
 @pytest.mark.parametrize("spread", [0.05, 6.0])
 @pytest.mark.parametrize("dim", [64, 256])
 def test_prompt_flat_and_sharp_rows(spread, dim):

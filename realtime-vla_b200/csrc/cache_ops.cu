@@ -168,8 +168,13 @@ int vla_op_cache_append(const vla_cache_append_desc* d, void* stream) {
     p.scale[0] = d->k_scale; p.scale[1] = d->v_scale;
     p.slots = d->slots; p.tokens = d->tokens; p.kv_heads = d->kv_heads; p.block = d->block_size;
     p.n_slots = (long long)d->num_blocks * d->block_size;
-    p.window = d->tokens <= 4096 ? 1 : 16;
-    const dim3 grid((d->tokens + p.window - 1) / p.window);
+    p.block_recip = d->block_size == 16 ? 0 : (uint32_t)(((1ull << 32) + d->block_size / 16 - 1) / (d->block_size / 16));
+    const long long per_cta = APPEND_THREADS / 32, items = 2ll * d->kv_heads;
+    // As many warps as run at once (28 an SM), and no more: a warp whose window starts no run is launched for nothing
+    for (p.window = 1; p.window < APPEND_WINDOW && d->tokens / p.window * items > 28ll * sm_count();) p.window *= 2;
+    const long long jobs = ((long long)d->tokens + p.window - 1) / p.window * items;
+    if (jobs > INT_TOP) return refuse(VLA_ERR_LIMIT, "%s: too many tokens and heads", who);
+    const dim3 grid((unsigned)((jobs + per_cta - 1) / per_cta));
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     auto go = [&](auto kern) { return launched(who, launch_ex(kern, grid, dim3(APPEND_THREADS), 0, st, 1, false, p)); };
     if (d->dtype == VLA_BF16)

@@ -34,6 +34,11 @@ struct PlanParams {
 constexpr int PLAN_THREADS = 512;
 constexpr int PLAN_MAX_SEQS = 8192;   // two sums of 4 bytes per request in shared memory
 
+// ceil(tokens / block).  Lengths are below 2^31 and sums of two below 2^32, so that divisions stay in 32 bits.
+__device__ __forceinline__ unsigned plan_blocks(unsigned tokens, unsigned block) {
+  const unsigned q = tokens / block;
+  return q + (q * block != tokens);
+}
 // Last index i in [0, n) with a[i] <= x (a ascending, a[0] <= x).
 __device__ __forceinline__ int plan_find(const int* a, int n, int x) {
   int lo = 0, hi = n;
@@ -59,13 +64,13 @@ __global__ void __launch_bounds__(PLAN_THREADS) block_plan_kernel(const PlanPara
 
   for (int base = 0; base < p.n_seqs; base += PLAN_THREADS) {
     const int b = base + threadIdx.x;
-    long long ctx = 0, n = 0;
+    unsigned ctx = 0, n = 0;
     if (b < p.n_seqs) {
       ctx = max(p.ctx[b], 0);
       n = max(p.n_new[b], 0);
     }
-    const long long have = (ctx + p.block - 1) / p.block, want = (ctx + n + p.block - 1) / p.block;
-    const long long need = min(want, (long long)p.width) - min(have, (long long)p.width);
+    const unsigned have = plan_blocks(ctx, p.block), want = plan_blocks(ctx + n, p.block), width = p.width;
+    const unsigned need = min(want, width) - min(have, width);
     missing_wide += (want - have) - need;
     long long st = n, sb = need;         // inclusive sums over the warp, then over the CTA
 #pragma unroll
@@ -87,9 +92,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) block_plan_kernel(const PlanPara
       cu[b] = (int)min(t0, TOP);
       off[b] = (int)min(b0, TOP);
       if (blockIdx.x == 0) {
-        const long long granted = min(max((long long)avail - b0, 0ll), need);
+        const long long granted = min(max((long long)avail - b0, 0ll), (long long)need);
         p.cu_new[b] = (int)min(t0, TOP);
-        p.seq_lens[b] = (int)min(min(ctx + n, (min(have, (long long)p.width) + granted) * p.block), TOP);
+        p.seq_lens[b] = (int)min(min((long long)(ctx + n), ((long long)min(have, width) + granted) * p.block), TOP);
       }
     }
     carry_t += all_t;
@@ -120,8 +125,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) block_plan_kernel(const PlanPara
   // new table entries: the j-th block given away
   for (int j = worker; j < given; j += workers) {
     const int b = plan_find(off, p.n_seqs, j);
-    const long long have = ((long long)max(p.ctx[b], 0) + p.block - 1) / p.block;
-    p.table[b * p.table_ld + have + (j - off[b])] = p.free_ids[first + j];
+    p.table[b * p.table_ld + plan_blocks(max(p.ctx[b], 0), p.block) + (j - off[b])] = p.free_ids[first + j];
   }
   // Slot and position of each token row.  An old block's id is read from the table (nothing in this call writes that
   // entry), a new one's from the free list.  Rows behind the last request get slot -1, position 0.
@@ -131,22 +135,29 @@ __global__ void __launch_bounds__(PLAN_THREADS) block_plan_kernel(const PlanPara
     const int t0 = (int)(qd * 4);
     int slot[4] = {-1, -1, -1, -1}, pos[4] = {0, 0, 0, 0};
     int b = t0 < sum_new ? plan_find(cu, p.n_seqs, t0) : p.n_seqs;
+    unsigned ctx = 0, have = 0;
+    bool fresh = true;                   // a request whose length is to be read
+#pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int t = t0 + k;
-      if (t >= sum_new) break;
-      while (t >= cu[b + 1]) ++b;        // requests without new tokens are passed over
-      const int ctx = max(p.ctx[b], 0);
-      const long long at = (long long)ctx + (t - cu[b]);
-      const long long blk = at / p.block;
-      const long long have = ((long long)ctx + p.block - 1) / p.block;
-      int id = -1;
-      if (blk < p.width) {
-        if (blk < have) id = p.table[b * p.table_ld + blk];
-        else if (off[b] + (blk - have) < given) id = p.free_ids[first + off[b] + (blk - have)];
+      if (t < sum_new) {
+        for (; t >= cu[b + 1]; fresh = true) ++b;      // requests without new tokens are passed over
+        if (fresh) {
+          ctx = max(p.ctx[b], 0);
+          have = plan_blocks(ctx, p.block);
+          fresh = false;
+        }
+        const unsigned at = ctx + (unsigned)(t - cu[b]), blk = at / (unsigned)p.block;
+        int id = -1;
+        if (blk < (unsigned)p.width) {
+          const long long nth = (long long)off[b] + (blk - have);
+          if (blk < have) id = p.table[b * p.table_ld + blk];
+          else if (nth < given) id = p.free_ids[first + nth];
+        }
+        const long long s = (long long)id * p.block + (at - blk * p.block);
+        slot[k] = id >= 0 && s <= TOP ? (int)s : -1;
+        pos[k] = (int)min(at, (unsigned)TOP);
       }
-      const long long s = (long long)id * p.block + at % p.block;
-      slot[k] = id >= 0 && s <= TOP ? (int)s : -1;
-      pos[k] = (int)min(at, TOP);
     }
     if (t0 + 3 < p.total) {
       *reinterpret_cast<int4*>(p.slots + t0) = make_int4(slot[0], slot[1], slot[2], slot[3]);

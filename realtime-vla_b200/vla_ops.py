@@ -6,6 +6,7 @@ programs that serve sequences of different lengths: they take torch tensors, enq
 device and return without synchronising, so they can be captured into a CUDA graph.  They run forward only."""
 import ctypes as C
 import functools
+import struct
 from typing import NamedTuple
 
 import torch
@@ -116,6 +117,8 @@ def vit_attention_tc(qkv, *, scale, iters=0):
 
 
 # ---- a key/value cache in pages, held in 8 bits -----------------------------------------------------------------------
+_PLAN, _APPEND = _capi.packer(_capi.BlockPlanDesc), _capi.packer(_capi.CacheAppendDesc)
+_PAGED, _PROMPT = _capi.packer(_capi.PagedAttnDesc), _capi.packer(_capi.PromptAttnDesc)
 _DTYPES = {torch.bfloat16: _capi.VLA_BF16, torch.float16: _capi.VLA_F16}
 
 
@@ -195,13 +198,17 @@ def _type(t, name):
     return code
 
 
-def _enqueue(fn, desc, device):
+def _enqueue(fn, pack, device, *fields):
+    try:
+        desc = pack(*fields)
+    except (struct.error, OverflowError) as e:
+        _refuse("a size is too large (%s)", e)
     stream = torch._C._cuda_getCurrentRawStream(device.index)      # current_stream(device).cuda_stream in 0.1 instead of 2.2 us
-    if torch.cuda.current_device() == device.index:
-        rc = fn(C.byref(desc), stream)
+    if torch._C._cuda_getDevice() == device.index:
+        rc = fn(desc, stream)
     else:
         with torch.cuda.device(device):
-            rc = fn(C.byref(desc), stream)
+            rc = fn(desc, stream)
     if rc:
         _capi.check(rc)
 
@@ -225,13 +232,12 @@ def block_plan(context_lens, new_lens, block_table, free_blocks, *, block_size, 
         slots, _, positions, _, cu, lens, counts = out.split_with_sizes([total_new, pad, total_new, pad, n + 1, n, 3])
     else:
         slots, positions, cu, lens, counts = out.split_with_sizes([total_new, total_new, n + 1, n, 3])
-    d = _capi.BlockPlanDesc(_whole(context_lens, "context_lens", dev), _whole(new_lens, "new_lens", dev), n,
-                            _whole(block_table, "block_table", dev, 2), block_table.shape[1],
-                            block_table.stride(0) if n > 1 else block_table.shape[1],
-                            _whole(free_blocks, "free_blocks", dev), free_blocks.shape[0],
-                            None if first_free is None else _whole(first_free, "first_free", dev), block_size, total_new,
-                            slots.data_ptr(), positions.data_ptr(), cu.data_ptr(), lens.data_ptr(), counts.data_ptr())
-    _enqueue(_capi.lib().vla_op_block_plan, d, dev)
+    _enqueue(_capi.lib().vla_op_block_plan, _PLAN, dev,
+             _whole(context_lens, "context_lens", dev), _whole(new_lens, "new_lens", dev), n, _whole(block_table, "block_table", dev, 2), block_table.shape[1],
+             block_table.stride(0) if n > 1 else block_table.shape[1],
+             _whole(free_blocks, "free_blocks", dev), free_blocks.shape[0],
+             0 if first_free is None else _whole(first_free, "first_free", dev), block_size, total_new,
+             slots.data_ptr(), positions.data_ptr(), cu.data_ptr(), lens.data_ptr(), counts.data_ptr())
     return BlockPlan(slots, positions, cu, lens, counts)
 
 
@@ -247,9 +253,8 @@ def cache_append(k, v, cache, slots):
     pk, pv = _rows(k, "k", dev, k.dtype, 3), _rows(v, "v", dev, k.dtype, 3)
     if k.shape != v.shape or k.shape[1:] != (heads, dim) or slots.shape[0] != k.shape[0]:
         _refuse("k %s, v %s and slots %s do not fit the cache %s", *(tuple(x.shape) for x in (k, v, slots, cache.k)))
-    d = _capi.CacheAppendDesc(pk, pv, _whole(slots, "slots", dev), k.shape[0], *k.stride()[:2], *v.stride()[:2],
-                              *codes, blocks, heads, block, dim, code)
-    _enqueue(_capi.lib().vla_op_cache_append, d, dev)
+    _enqueue(_capi.lib().vla_op_cache_append, _APPEND, dev, pk, pv, _whole(slots, "slots", dev), k.shape[0],
+             *k.stride()[:2], *v.stride()[:2], *codes, blocks, heads, block, dim, code)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -287,11 +292,10 @@ def paged_attention(q, cache, block_table, seq_lens, *, scale=None, out=None):
     need = _paged_workspace(dev, n, tokens, heads, kv_heads, dim, blocks, block, width)
     # the workspace is this call's own; the allocator orders its reuse on the stream
     space = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    d = _capi.PagedAttnDesc(pq, _rows(out, "out", dev, q.dtype, 4), *q.stride()[:3], *out.stride()[:3], *codes, table,
-                            block_table.stride(0) if n > 1 else width, _whole(seq_lens, "seq_lens", dev),
-                            n, tokens, heads, kv_heads, dim, blocks, block, width, dim ** -0.5 if scale is None else scale, code,
-                            space.data_ptr() if need else None, need)
-    _enqueue(_capi.lib().vla_op_paged_attention, d, dev)
+    _enqueue(_capi.lib().vla_op_paged_attention, _PAGED, dev, pq, _rows(out, "out", dev, q.dtype, 4), *q.stride()[:3], *out.stride()[:3],
+             *codes, table, block_table.stride(0) if n > 1 else width, _whole(seq_lens, "seq_lens", dev),
+             n, tokens, heads, kv_heads, dim, blocks, block, width, dim ** -0.5 if scale is None else scale, code,
+             space.data_ptr() if need else 0, need)
     return out
 
 
@@ -315,9 +319,8 @@ def prompt_attention(q, k, v, cu_q, cu_k=None, *, causal=True, scale=None, out=N
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape:
         _refuse("out must have the shape of q")
-    d = _capi.PromptAttnDesc(pq, pk, pv, _rows(out, "out", dev, t, 3), _whole(cu_q, "cu_q", dev), _whole(cu_k, "cu_k", dev),
-                             cu_q.shape[0] - 1, tokens, k.shape[0], heads, k.shape[1], dim,
-                             *q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *out.stride()[:2],
-                             1 if causal else 0, dim ** -0.5 if scale is None else scale, code)
-    _enqueue(_capi.lib().vla_op_prompt_attention, d, dev)
+    _enqueue(_capi.lib().vla_op_prompt_attention, _PROMPT, dev, pq, pk, pv, _rows(out, "out", dev, t, 3),
+             _whole(cu_q, "cu_q", dev), _whole(cu_k, "cu_k", dev), cu_q.shape[0] - 1, tokens, k.shape[0], heads, k.shape[1], dim,
+             *q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *out.stride()[:2],
+             1 if causal else 0, dim ** -0.5 if scale is None else scale, code)
     return out

@@ -108,7 +108,7 @@ __device__ __forceinline__ float paged_sum(const uint32_t (&v)[24], int r) {
   return fmaf(__uint_as_float(v[16 + r]), 0x1p-8f, fmaf(__uint_as_float(v[8 + r]), 0x1p-4f, __uint_as_float(v[r])));
 }
 // mbar_wait with its loop out of line: a kernel of many roles has many waits, and its code has to stay in the caches
-__device__ __noinline__ bool paged_wait_loop(uint32_t bar, uint32_t parity, volatile int* abort_flag) { return mbar_wait(bar, parity, abort_flag); }
+__device__ __noinline__ bool paged_wait_loop(uint32_t bar, uint32_t parity, volatile int* abort_flag) { return mbar_wait_small(bar, parity, abort_flag); }
 __device__ __forceinline__ bool paged_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
   return mbar_try_wait(bar, parity) || paged_wait_loop(bar, parity, abort_flag);
 }

@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(PromptCfg<WIDE>::THREADS, WIDE ? 1 : 2) prompt
       for (int x = 0; x < boxes; ++x) tma_load_4d(sQ + x * C::Q_BOX, &p.tmQ, q_full, x * 64, 0, kvh, q0 + tok0);
       bool ok = true;
       auto slot_free = [&](int pos) {
-        return pos < C::STAGES || mbar_wait(empty(pos % C::STAGES), (uint32_t)(pos / C::STAGES - 1) & 1u, abort_flag);
+        return pos < C::STAGES || mbar_wait_small(empty(pos % C::STAGES), (uint32_t)(pos / C::STAGES - 1) & 1u, abort_flag);
       };
       const uint64_t pol = policy_evict_last();   // other tiles of this sequence read the same keys
       auto load_k = [&](int c) {
@@ -253,14 +253,14 @@ __global__ void __launch_bounds__(PromptCfg<WIDE>::THREADS, WIDE ? 1 : 2) prompt
       const uint32_t idesc = (1u << 4) | (H::MMA_TYPE << 7) | (H::MMA_TYPE << 10) | (8u << 24);
       const int k_steps = (p.dim + 15) / 16;
       const uint32_t idesc_o = idesc | (1u << 16) | ((uint32_t)(k_steps * 2) << 17);      // N = head dim, B MN-major
-      bool ok = mbar_wait(q_full, 0, abort_flag);
+      bool ok = mbar_wait_small(q_full, 0, abort_flag);
       // The loops are unrolled over what the tile can hold, with the descriptors as constants from a base: formed step by
       // step, an MMA took this one thread about 140 clocks to issue, more than twice what it runs for.
       const uint64_t q_desc = attn_desc_sw128(sQ), k_desc = attn_desc_sw128(sRing), v_desc = prompt_desc_mn(sRing, C::V_BOX);
       auto wait_units = [&](int pos0) {
         for (int u = 0; u < C::UNITS; ++u) {
           const int pos = pos0 + u;
-          ok = ok && mbar_wait(full(pos % C::STAGES), (uint32_t)(pos / C::STAGES) & 1u, abort_flag);
+          ok = ok && mbar_wait_small(full(pos % C::STAGES), (uint32_t)(pos / C::STAGES) & 1u, abort_flag);
         }
       };
       auto issue_s = [&](int c) {
@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(PromptCfg<WIDE>::THREADS, WIDE ? 1 : 2) prompt
         const bool more = c + C::AHEAD < n_chunks;
         wait_units(v_pos(c));
         if (more) wait_units(k_pos(c + C::AHEAD));
-        ok = ok && mbar_wait(p_ready(buf), (uint32_t)(c / C::AHEAD) & 1u, abort_flag);
+        ok = ok && mbar_wait_small(p_ready(buf), (uint32_t)(c / C::AHEAD) & 1u, abort_flag);
         if (!ok) break;
         tc_fence_after();
         const int keys16 = (min(lim_max - c * C::KEYS, C::KEYS) + 15) / 16;
@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(PromptCfg<WIDE>::THREADS, WIDE ? 1 : 2) prompt
     bool ok = true;
     for (int c = 0; c < n_chunks && ok; ++c) {
       const int buf = c % C::AHEAD;
-      ok = __all_sync(0xffffffffu, mbar_wait(s_full(buf), (uint32_t)(c / C::AHEAD) & 1u, abort_flag));
+      ok = __all_sync(0xffffffffu, mbar_wait_small(s_full(buf), (uint32_t)(c / C::AHEAD) & 1u, abort_flag));
       if (!ok) break;
       tc_fence_after();
       const uint32_t ts = tmem + lane_off + buf * C::KEYS;
@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(PromptCfg<WIDE>::THREADS, WIDE ? 1 : 2) prompt
       if (__any_sync(0xffffffffu, top > m + 8.f)) {
         const float m_new = fmaxf(m, top);
         if (c > 0) {
-          ok = __all_sync(0xffffffffu, mbar_wait(o_done((c - 1) & 1), (uint32_t)((c - 1) >> 1) & 1u, abort_flag));
+          ok = __all_sync(0xffffffffu, mbar_wait_small(o_done((c - 1) & 1), (uint32_t)((c - 1) >> 1) & 1u, abort_flag));
           if (!ok) break;
           tc_fence_after();
           const float a = m == m_new ? 1.f : ex2_approx(m - m_new);
@@ -400,11 +400,11 @@ __global__ void __launch_bounds__(PromptCfg<WIDE>::THREADS, WIDE ? 1 : 2) prompt
         // cleared in shared memory; the epilogue gives them back to the rows that see them.  S of this chunk and the P V
         // before it are over, so V's slots are past their earlier uses and a look at them cannot take one for this use.
         // After the exponentials, so that the wait for that P V runs under them.
-        if (c > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_done((c - 1) & 1), (uint32_t)((c - 1) >> 1) & 1u, abort_flag));
+        if (c > 0) ok = __all_sync(0xffffffffu, mbar_wait_small(o_done((c - 1) & 1), (uint32_t)((c - 1) >> 1) & 1u, abort_flag));
         const int at = v_pos(c), s0 = at % C::STAGES, s1 = (at + C::UNITS - 1) % C::STAGES;
 #pragma unroll
         for (int u = 0; u < C::UNITS; ++u)
-          ok = ok && __all_sync(0xffffffffu, mbar_wait(full(u ? s1 : s0), (uint32_t)((at + u) / C::STAGES) & 1u, abort_flag));
+          ok = ok && __all_sync(0xffffffffu, mbar_wait_small(full(u ? s1 : s0), (uint32_t)((at + u) / C::STAGES) & 1u, abort_flag));
         if (!ok) break;
         const int lo = max(lim_min - c * C::KEYS, 0), tail = lim_max - c * C::KEYS, hi = (min(tail, C::KEYS) + 15) / 16 * 16;
         constexpr int PIECES = C::BOXES * 8;           // of a key's row, 16 bytes each
@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(PromptCfg<WIDE>::THREADS, WIDE ? 1 : 2) prompt
       mbar_arrive(p_ready(buf));
     }
     if (ok && n_chunks > 0) {
-      ok = __all_sync(0xffffffffu, mbar_wait(o_done((n_chunks - 1) & 1), (uint32_t)((n_chunks - 1) >> 1) & 1u, abort_flag));
+      ok = __all_sync(0xffffffffu, mbar_wait_small(o_done((n_chunks - 1) & 1), (uint32_t)((n_chunks - 1) >> 1) & 1u, abort_flag));
       tc_fence_after();
     }
     if (ok && seq >= 0) {

@@ -2,7 +2,6 @@
 anywhere, but every call needs the compiled library and a B200."""
 import ctypes as C
 import os
-import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libvla_b200.so")
@@ -108,26 +107,16 @@ EXPORTS = {
     "vla_expert_timeline": (C.c_int, [C.c_void_p, C.POINTER(C.c_ulonglong), C.c_int, C.POINTER(C.c_int)]),
     "vla_op_attention": (C.c_int, [C.POINTER(AttnDesc), C.c_void_p]),
     "vla_op_attention_tc": (C.c_int, [C.POINTER(AttnTcDesc), C.c_void_p]),
-    "vla_op_block_plan": (C.c_int, [C.c_void_p, C.c_void_p]),
-    "vla_op_cache_append": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "vla_op_block_plan": (C.c_int, [C.POINTER(BlockPlanDesc), C.c_void_p]),
+    "vla_op_cache_append": (C.c_int, [C.POINTER(CacheAppendDesc), C.c_void_p]),
     "vla_op_paged_attention_workspace": (C.c_int, [C.POINTER(PagedAttnDesc), C.POINTER(C.c_size_t)]),
-    "vla_op_paged_attention": (C.c_int, [C.c_void_p, C.c_void_p]),
-    "vla_op_prompt_attention": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "vla_op_paged_attention": (C.c_int, [C.POINTER(PagedAttnDesc), C.c_void_p]),
+    "vla_op_prompt_attention": (C.c_int, [C.POINTER(PromptAttnDesc), C.c_void_p]),
     "vla_op_cache_status": (C.c_int, [C.POINTER(C.c_int)]),
     "vla_op_norm": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p]),
 }
 
 _lib = None
-
-
-_CODES = {C.c_void_p: "P", C.c_int: "i", C.c_longlong: "q", C.c_float: "f", C.c_size_t: "N"}
-
-
-def packer(desc):
-    """desc's fields in order -> its bytes (a null pointer is 0); a quarter of the time that filling the structure takes."""
-    s = struct.Struct("@" + "".join(_CODES[t] for _, t in desc._fields_) + "0q")
-    assert s.size == C.sizeof(desc)
-    return s.pack
 
 
 def lib():

@@ -1,10 +1,13 @@
-"""Build libvla_b200.so in place with nvcc for sm_100a (cross-compiles without a GPU)."""
+"""Build libvla_b200.so in place with nvcc for sm_100a (cross-compiles without a GPU), and _vla_ops.so, the Python binding of the
+operators that take torch tensors, with g++."""
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB = os.path.join(HERE, "libvla_b200.so")
+BINDING, BINDING_SRC = os.path.join(HERE, "_vla_ops.so"), "csrc/binding.cpp"
 SOURCES = ["csrc/model.cu", "csrc/cache_ops.cu"]
 # headers that only one of the sources includes; the others (common.cuh, host.cuh, the C header) belong to both
 ONLY = {"csrc/cache_ops.cu": {"csrc/attention_paged.cuh", "csrc/attention_prompt.cuh", "csrc/cache_pages.cuh"}}
@@ -26,7 +29,21 @@ def _stale(target, inputs):
 
 
 def needs_build():
-    return _stale(LIB, [os.path.join(HERE, f) for f in SOURCES + HEADERS])
+    return _stale(LIB, [os.path.join(HERE, f) for f in SOURCES + HEADERS]) or _binding_stale()
+
+
+def _binding_stale():
+    return _stale(BINDING, [os.path.join(HERE, f) for f in (BINDING_SRC, "../include/vla_b200.h")])
+
+
+def _binding_command(nvcc):
+    import torch
+    home = os.path.dirname(torch.__file__)
+    include = [os.path.join(home, "include"), os.path.join(home, "include/torch/csrc/api/include"), sysconfig.get_paths()["include"],
+               os.path.join(os.path.dirname(os.path.dirname(nvcc)), "include")]
+    libs = ["torch_python", "torch_cpu", "torch", "c10", "c10_cuda", "vla_b200"]
+    return (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", BINDING_SRC, "-o", BINDING] + ["-I" + d for d in include] +
+            ["-L" + os.path.join(home, "lib"), "-L" + HERE] + ["-l" + x for x in libs] + ["-Wl,-rpath,$ORIGIN"])
 
 
 def build(force=False, verbose=False):
@@ -42,7 +59,10 @@ def build(force=False, verbose=False):
     failed = [s for s, p in zip(todo, running) if p.wait() != 0]
     if failed:
         raise RuntimeError("nvcc failed on " + ", ".join(failed))
-    subprocess.run([nvcc] + flags + ["-shared", "-o", LIB] + [_object(s) for s in SOURCES], cwd=HERE, check=True)
+    if force or _stale(LIB, [_object(s) for s in SOURCES]):
+        subprocess.run([nvcc] + flags + ["-shared", "-o", LIB] + [_object(s) for s in SOURCES], cwd=HERE, check=True)
+    if force or _binding_stale():
+        subprocess.run(_binding_command(nvcc), cwd=HERE, check=True)
     return LIB
 
 

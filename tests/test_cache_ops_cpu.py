@@ -115,3 +115,12 @@ def test_wrappers_refuse_the_cpu():
               lambda: vla_ops.cache_append(q[:, :2], q[:, :2], cache, i), lambda: vla_ops.block_plan(i, i, i[None], i, block_size=16, total_new=0)):
         with pytest.raises(_capi.VlaError, match="no CPU path"):
             f()
+
+
+@needs_library
+def test_wrappers_refuse_what_is_no_tensor():
+    i = torch.zeros(2, dtype=torch.int32)
+    for f in (lambda: vla_ops.prompt_attention(None, i, i, i), lambda: vla_ops.paged_attention([1.0], None, i, i),
+              lambda: vla_ops.cache_append(3, i, None, i), lambda: vla_ops.block_plan("x", i, i, i, block_size=16, total_new=0)):
+        with pytest.raises(_capi.VlaError, match="must be a tensor"):
+            f()

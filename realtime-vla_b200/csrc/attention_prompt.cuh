@@ -137,7 +137,9 @@ __global__ void __launch_bounds__(PromptCfg<WIDE>::THREADS, WIDE ? 1 : 2) prompt
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kvh = blockIdx.x % p.kv_heads;
+  pdl_trigger();
   if (warp == 0) {
+    pdl_wait();
     // Which tile this CTA is: the sequences' tiles are counted from cu_q on the device, 32 sequences at a time.  A
     // causal sequence hands out its last tiles first, because they have the most keys.
     int idx = blockIdx.x / p.kv_heads, seq = -1, at = 0;
@@ -191,6 +193,7 @@ __global__ void __launch_bounds__(PromptCfg<WIDE>::THREADS, WIDE ? 1 : 2) prompt
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int seq = *tile_seq;
+  pdl_wait();
 
   // Lengths, and the limits of the tile's first and last row (every thread: four words from L1 / L2)
   int q0 = 0, nq = 0, k0 = 0, nk = 0;

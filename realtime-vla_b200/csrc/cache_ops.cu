@@ -142,7 +142,7 @@ int vla_op_block_plan(const vla_block_plan_desc* d, void* stream) {
         return launched(who, e);
     const long long rows = std::max<long long>(((long long)d->total_new + 3) / 4, d->n_seqs);
     const int ctas = (int)std::min<long long>(std::max<long long>(1, (rows + PLAN_THREADS - 1) / PLAN_THREADS), 2 * sm_count());
-    return launched(who, launch_ex(block_plan_kernel, dim3(ctas), dim3(PLAN_THREADS), smem, reinterpret_cast<cudaStream_t>(stream), 1, false, p));
+    return launched(who, launch_ex(block_plan_kernel, dim3(ctas), dim3(PLAN_THREADS), smem, reinterpret_cast<cudaStream_t>(stream), 1, true, p));
   });
 }
 
@@ -176,7 +176,7 @@ int vla_op_cache_append(const vla_cache_append_desc* d, void* stream) {
     if (jobs > INT_TOP) return refuse(VLA_ERR_LIMIT, "%s: too many tokens and heads", who);
     const dim3 grid((unsigned)((jobs + per_cta - 1) / per_cta));
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    auto go = [&](auto kern) { return launched(who, launch_ex(kern, grid, dim3(APPEND_THREADS), 0, st, 1, false, p)); };
+    auto go = [&](auto kern) { return launched(who, launch_ex(kern, grid, dim3(APPEND_THREADS), 0, st, 1, true, p)); };
     if (d->dtype == VLA_BF16)
       return d->head_dim == 64 ? go(cache_append_kernel<bf16, 64>) : d->head_dim == 128 ? go(cache_append_kernel<bf16, 128>) : go(cache_append_kernel<bf16, 256>);
     return d->head_dim == 64 ? go(cache_append_kernel<__half, 64>) : d->head_dim == 128 ? go(cache_append_kernel<__half, 128>) : go(cache_append_kernel<__half, 256>);
@@ -290,7 +290,7 @@ int vla_op_prompt_attention(const vla_prompt_attn_desc* d, void* stream) {
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     auto go = [&](auto kern, int smem) -> int {
       if (cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kern), smem); e != cudaSuccess) return launched(who, e);
-      return launched(who, launch_ex(kern, dim3((unsigned)(tiles * d->kv_heads)), dim3(PromptCfg<false>::THREADS), smem, st, 1, false, p));
+      return launched(who, launch_ex(kern, dim3((unsigned)(tiles * d->kv_heads)), dim3(PromptCfg<false>::THREADS), smem, st, 1, true, p));
     };
     if (d->dtype == VLA_BF16)
       return wide ? go(prompt_attention_kernel<bf16, true>, PromptCfg<true>::SMEM_BYTES) : go(prompt_attention_kernel<bf16, false>, PromptCfg<false>::SMEM_BYTES);

@@ -57,6 +57,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) block_plan_kernel(const PlanPara
   int* off = plan_smem + p.n_seqs + 1;   // [n_seqs + 1] first new block of each request
   __shared__ long long warp_sum[2][PLAN_THREADS / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pdl_trigger();
+  pdl_wait();
   const int first = p.first ? min(max(*p.first, 0), p.n_free) : 0;
   const int avail = p.n_free - first;
   long long carry_t = 0, carry_b = 0, missing_wide = 0;
@@ -296,6 +298,8 @@ __global__ void __launch_bounds__(APPEND_THREADS, D == 256 ? 4 : 7) cache_append
     const uint32_t s16 = (uint32_t)slot >> 4;
     return (int)(p.block_recip ? __umulhi(s16, p.block_recip) : s16);
   };
+  pdl_trigger();
+  pdl_wait();
   const int slot_w = slot_at(w0 - 1 + lane), blk_w = block_of(slot_w);     // lane 0: the row before the window
   const int blk_before = __shfl_up_sync(FULL, blk_w, 1);
   uint32_t starts = __ballot_sync(FULL, lane >= 1 && lane <= p.window && blk_w >= 0 && blk_w != blk_before);

@@ -135,13 +135,14 @@ int vla_op_block_plan(const vla_block_plan_desc* d, void* stream) {
     p.table = d->block_table; p.width = d->width; p.table_ld = d->table_stride;
     p.free_ids = d->free_blocks; p.n_free = d->n_free; p.first = d->first_free;
     p.block = d->block_size; p.total = d->total_new;
+    p.block_recip = (unsigned)std::min<unsigned long long>((1ull << 32) / d->block_size, 0xffffffffull);
     p.slots = d->slots; p.positions = d->positions; p.cu_new = d->cu_new; p.seq_lens = d->seq_lens; p.counts = d->counts;
     const size_t smem = (size_t)(2 * d->n_seqs + 2) * sizeof(int);
     if (smem > 40 * 1024)
       if (cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(block_plan_kernel), (2 * PLAN_MAX_SEQS + 2) * (int)sizeof(int)); e != cudaSuccess)
         return launched(who, e);
-    const long long rows = std::max<long long>(((long long)d->total_new + 3) / 4, d->n_seqs);
-    const int ctas = (int)std::min<long long>(std::max<long long>(1, (rows + PLAN_THREADS - 1) / PLAN_THREADS), 2 * sm_count());
+    // one row a thread, or a CTA on each SM: with four rows a thread 140k rows of 512 prompts take 6.4 us instead of 5.0
+    const int ctas = std::min((std::max(std::max(d->total_new, d->n_seqs), 1) - 1) / PLAN_THREADS + 1, sm_count());
     return launched(who, launch_ex(block_plan_kernel, dim3(ctas), dim3(PLAN_THREADS), smem, reinterpret_cast<cudaStream_t>(stream), 1, true, p));
   });
 }

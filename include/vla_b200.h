@@ -312,8 +312,8 @@ int vla_op_block_plan(const vla_block_plan_desc* d, void* stream);
  * of two >= 2^-60 that brings the largest finite magnitude of the call's tokens to 448 or less.  A block whose first
  * slot is written starts anew with that scale; any other block keeps the larger of its scale and that one, and where
  * the scale grows all its codes are rounded again.  Codes are x / scale, nearest even, saturating; NaN stays NaN.
- * The tokens of one block must be consecutive rows of the call (as vla_op_block_plan lays them out); of two consecutive tokens
- * with the same slot the later one is kept.  head_dim 64 | 128 | 256, block_size a multiple of 16 up to 256. */
+ * The tokens of one block must be consecutive rows of the call (as vla_op_block_plan lays them out), with no other or skipped
+ * row between them: else what the block holds afterwards is not defined.  Of two tokens with the same slot the later one is kept.  head_dim 64 | 128 | 256, block_size a multiple of 16 up to 256. */
 typedef struct vla_cache_append_desc {
   const void* k; const void* v; const int32_t* slots; int tokens;
   long long k_tok_stride, k_head_stride, v_tok_stride, v_head_stride;

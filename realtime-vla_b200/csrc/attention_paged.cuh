@@ -273,8 +273,9 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
     tma_prefetch_desc(&p.tmK);
     tma_prefetch_desc(&p.tmV);
   }
-  if (warp == 1) tmem_alloc(smem_u32(&tmem_slot), C::TMEM_COLS);
   pdl_wait();
+  // behind the wait: a CTA of the kernel before this one may yet have to take its own, and this one would hold it up for good
+  if (warp == 1) tmem_alloc(smem_u32(&tmem_slot), C::TMEM_COLS);
 
   // rows of sequences without tokens
 #pragma unroll 1

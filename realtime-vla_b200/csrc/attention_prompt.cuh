@@ -137,7 +137,6 @@ __global__ void __launch_bounds__(PromptCfg<WIDE>::THREADS, WIDE ? 1 : 2) prompt
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kvh = blockIdx.x % p.kv_heads;
-  pdl_trigger();
   if (warp == 0) {
     pdl_wait();
     // Which tile this CTA is: the sequences' tiles are counted from cu_q on the device, 32 sequences at a time.  A
@@ -169,6 +168,7 @@ __global__ void __launch_bounds__(PromptCfg<WIDE>::THREADS, WIDE ? 1 : 2) prompt
       *tile_at = at * p.tile_tokens;
     }
   } else if (warp == 1) {
+    pdl_wait();          // before the TMEM: a CTA of the kernel before this one may yet have to take its own
     tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
   } else if (threadIdx.x == 64) {
     mbar_init(q_full, 1);
@@ -193,6 +193,7 @@ __global__ void __launch_bounds__(PromptCfg<WIDE>::THREADS, WIDE ? 1 : 2) prompt
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int seq = *tile_seq;
+  pdl_trigger();       // the TMEM is there: no CTA of the next kernel can take it first and wait for this one
   pdl_wait();
 
   // Lengths, and the limits of the tile's first and last row (every thread: four words from L1 / L2)

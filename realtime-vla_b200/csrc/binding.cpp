@@ -122,6 +122,8 @@ at::Tensor output(PyObject* o, const at::Tensor& q) {
   if (o == Py_None) return at::empty(q.sizes(), q.options());
   const at::Tensor& t = rows(o, "out", q.device(), q.scalar_type(), (int)q.dim());
   if (t.sizes() != q.sizes()) refuse("out must have the shape of q");
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.stride(i) == 0 && t.size(i) > 1) refuse("out is expanded: several of its elements are one place in memory");
   return t;
 }
 

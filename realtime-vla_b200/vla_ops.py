@@ -162,8 +162,9 @@ def block_plan(context_lens, new_lens, block_table, free_blocks, *, block_size, 
 def cache_append(k, v, cache, slots):
     """Keys and values (bf16 or fp16 [tokens, kv_heads, head_dim]) into the cache at slots (int32 [tokens]), in place.
 
-    Slots outside the cache are skipped; the tokens of one block must be consecutive rows.  A block whose first slot is written
-    starts anew; another block's scale grows where the new tokens need it and its codes are rounded again."""
+    Slots outside the cache are skipped; the tokens of one block must be consecutive rows, with no other or skipped row between
+    them (what such a block holds afterwards is not defined).  A block whose first slot is written starts anew; another
+    block's scale grows where the new tokens need it and its codes are rounded again."""
     _native.cache_append(k, v, cache, slots)
 
 

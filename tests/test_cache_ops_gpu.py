@@ -703,3 +703,41 @@ def test_refusals_on_the_gpu():
         with pytest.raises(_capi.VlaError):
             call()
             raise AssertionError("call %d was not refused" % i)
+
+
+def test_expanded_output_is_refused():
+    import _capi
+    import vla_ops
+    d = dev()
+    q, cache, table, n = pages(38, (20, 30), 1, 8, 2, 128, 16, torch.bfloat16, d)
+    cu = torch.tensor([0, 2], dtype=torch.int32, device=d)
+    for call in (lambda: vla_ops.paged_attention(q, cache, table, n, out=q[:, :, :1].clone().expand(-1, -1, 8, -1)),
+                 lambda: vla_ops.prompt_attention(q[:, 0], q[:, 0], q[:, 0], cu, out=q[:1, 0].clone().expand(2, -1, -1))):
+        with pytest.raises(_capi.VlaError, match="expanded"):
+            call()
+
+
+@pytest.mark.parametrize("block", [1, 3, 7, 16, 48, 1000, 2 ** 20 + 1, 2 ** 31 - 1])
+def test_plan_far_positions(block):
+    """Lengths up to the last that 32 bits hold; the table has room for the first pages only, and no page is free."""
+    import vla_ops
+    d = dev()
+    top, width = 2 ** 31 - 1, 3
+    ctx = [top, top - 5, 2 ** 30, top // block * block, 2 * block - 1 if block < 2 ** 29 else 7]
+    new = [3, 5, 1, 2, 2]
+    table = [[5 * b + i for i in range(width)] for b in range(5)]
+    slots, pos, lens, missing = [], [], [], 0
+    for b, (c, n) in enumerate(zip(ctx, new)):
+        have, want = -(-c // block), -(-(c + n) // block)
+        missing += want - have
+        lens.append(min(c + n, min(have, width) * block, top))
+        for at in range(c, c + n):
+            blk = at // block
+            s = table[b][blk] * block + at % block if blk < min(have, width) else -1
+            slots.append(s if s <= top else -1)
+            pos.append(min(at, top))
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=d)      # noqa: E731
+    tab = i32(table)
+    got = vla_ops.block_plan(i32(ctx), i32(new), tab, i32([]), block_size=block, total_new=sum(new))
+    assert got.slots.tolist() == slots and got.positions.tolist() == pos and got.seq_lens.tolist() == lens
+    assert got.counts.tolist() == [0, missing, sum(new)] and got.cu_new.tolist() == [0, 3, 8, 9, 11, 13] and tab.tolist() == table

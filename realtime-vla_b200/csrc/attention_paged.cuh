@@ -507,34 +507,46 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
         }
       }
       if (seg >= C::Q_BUFS && !__all_sync(0xffffffffu, paged_wait(q_empty(qb), (uint32_t)(seg / C::Q_BUFS - 1) & 1u, abort_flag))) break;
+      // Two rows at a time: a row is a chain of some 450 clocks, and short sequences wait for them.  3 sequences of 69 to 276, 5
+      // tokens each of 64 heads on 8, take 15.1 us instead of 16.3; four at a time 14.9, but more where there are 8 rows.
 #pragma unroll 1
-      for (int r = 0; r < R; ++r) {
-        float2 f[E];
-        float top = 0.f;
+      for (int r = 0; r < R; r += 2) {
+        float2 f[2][E];
+        float top[2];
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-          f[i] = unpack2<T>(rows[0][i]);
-          top = fmaxf(top, fmaxf(fabsf(f[i].x), fabsf(f[i].y)));
+        for (int j = 0; j < 2; ++j) {
+          top[j] = 0.f;
 #pragma unroll
-          for (int k = 0; k + 1 < R; ++k) rows[k][i] = rows[k + 1][i];
+          for (int i = 0; i < E; ++i) {
+            f[j][i] = unpack2<T>(rows[j][i]);
+            top[j] = fmaxf(top[j], fmaxf(fabsf(f[j][i].x), fabsf(f[j][i].y)));
+          }
         }
-        top = warp_max_f32(top);
-        const int e = (__float_as_int(top) >> 23) - 127 - 7;
-        // zeros, the smallest numbers and infinities stay as they are; the scores of a row with an infinity are NaN
-        const bool plain = top == 0.f || !(top < INFINITY) || e < -126;
-        const float up = plain ? 1.f : __int_as_float((127 - e) << 23);
-        if (lane == 0) q_scale[qb][r] = (plain ? 1.f : __int_as_float((127 + e) << 23)) * (top < INFINITY ? p.scale_log2e : NAN);
-        uint32_t c[E][3];
 #pragma unroll
-        for (int i = 0; i < E; ++i) pieces(f[i].x * up, f[i].y * up, c[i]);
+        for (int k = 0; k + 2 < R; ++k)
 #pragma unroll
-        for (int k = 0; k < 3; ++k) {
-          const int n = k * R + r, at = lane * (2 * E);          // byte of the row
-          uint8_t* dst = q_mem + qb * C::Q_BYTES + (at / 128) * C::N * 128 + n * C::ROW_BYTES +
-                         (((at % 128 / 16) ^ (D == 64 ? n >> 1 & 3 : n & 7)) << 4) + at % 16;
-          if (E == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(c[0][k] | c[1 % E][k] << 16, c[2 % E][k] | c[3 % E][k] << 16);
-          else if (E == 2) *reinterpret_cast<uint32_t*>(dst) = c[0][k] | c[1 % E][k] << 16;
-          else *reinterpret_cast<uint16_t*>(dst) = (uint16_t)c[0][k];
+          for (int i = 0; i < E; ++i) rows[k][i] = rows[k + 2][i];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) top[j] = warp_max_f32(top[j]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int e = (__float_as_int(top[j]) >> 23) - 127 - 7;
+          // zeros, the smallest numbers and infinities stay as they are; the scores of a row with an infinity are NaN
+          const bool plain = top[j] == 0.f || !(top[j] < INFINITY) || e < -126;
+          const float up = plain ? 1.f : __int_as_float((127 - e) << 23);
+          if (lane == 0) q_scale[qb][r + j] = (plain ? 1.f : __int_as_float((127 + e) << 23)) * (top[j] < INFINITY ? p.scale_log2e : NAN);
+          uint32_t c[E][3];
+#pragma unroll
+          for (int i = 0; i < E; ++i) pieces(f[j][i].x * up, f[j][i].y * up, c[i]);
+#pragma unroll
+          for (int k = 0; k < 3; ++k) {
+            const int n = k * R + r + j, at = lane * (2 * E);          // byte of the row
+            uint8_t* dst = q_mem + qb * C::Q_BYTES + (at / 128) * C::N * 128 + n * C::ROW_BYTES +
+                           (((at % 128 / 16) ^ (D == 64 ? n >> 1 & 3 : n & 7)) << 4) + at % 16;
+            if (E == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(c[0][k] | c[1 % E][k] << 16, c[2 % E][k] | c[3 % E][k] << 16);
+            else if (E == 2) *reinterpret_cast<uint32_t*>(dst) = c[0][k] | c[1 % E][k] << 16;
+            else *reinterpret_cast<uint16_t*>(dst) = (uint16_t)c[0][k];
+          }
         }
       }
       fence_proxy_async_shared();

@@ -235,6 +235,9 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
   // no page is
   __shared__ float4 page_info[C::SLOTS / 2][8];
   __shared__ float q_scale[2][R];
+  // 16 rows, two CTAs an SM: each softmax warp's copy of the scale of Q and the maximum of each row, the same for all its lanes
+  constexpr bool KEPT = NT == 2 && C::PER_SM == 2;
+  __shared__ float4 row_mem[KEPT ? 4 : 1][2][R / 4];
   __shared__ float4 warp_max[R], warp_sums[2][R];   // by row, of the four softmax warps (sums: of odd and even units)
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t pad = (1024u - (raw_addr & 1023u)) & 1023u;
@@ -575,6 +578,25 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
     };
     Part w, w_next;
     w.t0 = w.t1 = 0;
+    // m and qs are kept there and read where they are needed: in 128 registers a thread they were spilled, and 9 sequences of
+    // 2940 to 16102, 8 tokens each of 28 heads on 4 of 128, took 86 us instead of 72.
+    auto from_mem = [&](int what, float (&v)[R]) {
+      if (!KEPT) return;
+#pragma unroll
+      for (int r = 0; r < R; r += 4) {
+        const float4 f = row_mem[KEPT ? quarter : 0][what][r / 4];
+        v[r] = f.x; v[r + 1] = f.y; v[r + 2] = f.z; v[r + 3] = f.w;
+      }
+    };
+    auto to_mem = [&](int what, const float (&v)[R]) {
+      if (!KEPT) return;
+      __syncwarp();
+      if (lane == 0) {
+#pragma unroll
+        for (int r = 0; r < R; r += 4) row_mem[KEPT ? quarter : 0][what][r / 4] = make_float4(v[r], v[r + 1], v[r + 2], v[r + 3]);
+      }
+      __syncwarp();
+    };
     int c = 0, cut_b = -1;
     // one pass per unit, after a first that only looks up the unit to begin with
 #pragma unroll 1
@@ -621,9 +643,12 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
             m[r] = -INFINITY;
             l[r] = 0.f;
           }
+          to_mem(0, qs);
+          to_mem(1, m);
           __syncwarp();
           if (lane == 0) mbar_arrive(q_empty(seg % C::Q_BUFS));
         }
+        from_mem(0, qs);
         float x[R];                              // s + log2 s_v
 #pragma unroll
         for (int r8 = 0; r8 < R; r8 += 8) {
@@ -643,6 +668,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
             }
           }
         }
+        from_mem(1, m);
         bool grow = false;
 #pragma unroll
         for (int r = 0; r < R; ++r) grow |= x[r] > m[r] + 1.f;
@@ -665,6 +691,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
             m[r] = top;
             l[r] *= a[r];
           }
+          to_mem(1, m);
           if (tile > w.t0) {
 #pragma unroll 1
             for (int y = 0; y < C::HALVES; ++y) {
@@ -680,6 +707,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
           }
         }
         if (c > 0) wait(o_done, (uint32_t)(c - 1) & 1u);   // P of the tile before has been read
+        from_mem(1, m);
         uint8_t* p_col = p_mem + (tid & 15);
         const int chunk = tid >> 4;
 #pragma unroll
@@ -772,6 +800,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
               left = left ? left : p.group;
             }
           } else {
+            from_mem(1, m);
             float* part = p.part_o + ((long long)blockIdx.x * 2 + slot) * (R * D) + d;
             float2* part_ml = p.part_ml + ((long long)blockIdx.x * 2 + slot) * R;
 #pragma unroll

@@ -19,7 +19,7 @@
 // Roles, all walking the same piece on their own: warp 0 pages and TMA, warp 1 MMA, warp 2 Q pieces of the next unit, warps
 // 3..6 softmax, one token (and, at a unit's end, one head dim) per thread.  All mbarrier waits are bounded.  Code that
 // runs once per unit is kept in loops: run straight through, it costs about 8 clocks an instruction to fetch.
-// Measured: 64 sequences of 64 to 8192 tokens, 32 heads on 8 of 128, 48.3 us, 4.5 TB/s of codes and scales; 4 of 90001 to 131071, 8
+// Measured: 64 sequences of 64 to 8192 tokens, 32 heads on 8 of 128, 46.6 us, 4.7 TB/s of codes and scales; 4 of 90001 to 131071, 8
 // heads on 1 of 256, 50.7 us, 4.6 TB/s; one of 809 tokens 8.7 us.
 #pragma once
 #include "cache_pages.cuh"
@@ -235,8 +235,8 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
   // no page is
   __shared__ float4 page_info[C::SLOTS / 2][8];
   __shared__ float q_scale[2][R];
-  // 16 rows, two CTAs an SM: each softmax warp's copy of the scale of Q and the maximum of each row, the same for all its lanes
-  constexpr bool KEPT = NT == 2 && C::PER_SM == 2;
+  // with two CTAs an SM: each softmax warp's copy of the scale of Q and the maximum of each row, the same for all its lanes
+  constexpr bool KEPT = C::PER_SM == 2;
   __shared__ float4 row_mem[KEPT ? 4 : 1][2][R / 4];
   __shared__ float4 warp_max[R], warp_sums[2][R];   // by row, of the four softmax warps (sums: of odd and even units)
   const uint32_t raw_addr = smem_u32(smem_raw);
@@ -579,23 +579,25 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
     Part w, w_next;
     w.t0 = w.t1 = 0;
     // m and qs are kept there and read where they are needed: in 128 registers a thread they were spilled, and 9 sequences of
-    // 2940 to 16102, 8 tokens each of 28 heads on 4 of 128, took 86 us instead of 72.
+    // 2940 to 16102, 8 tokens each of 28 heads on 4 of 128, took 86 us instead of 72 (64 next tokens of 64 to 8192: 48.3, 46.6).
     auto from_mem = [&](int what, float (&v)[R]) {
-      if (!KEPT) return;
+      if constexpr (KEPT) {
 #pragma unroll
-      for (int r = 0; r < R; r += 4) {
-        const float4 f = row_mem[KEPT ? quarter : 0][what][r / 4];
-        v[r] = f.x; v[r + 1] = f.y; v[r + 2] = f.z; v[r + 3] = f.w;
+        for (int r = 0; r < R; r += 4) {
+          const float4 f = row_mem[quarter][what][r / 4];
+          v[r] = f.x; v[r + 1] = f.y; v[r + 2] = f.z; v[r + 3] = f.w;
+        }
       }
     };
     auto to_mem = [&](int what, const float (&v)[R]) {
-      if (!KEPT) return;
-      __syncwarp();
-      if (lane == 0) {
+      if constexpr (KEPT) {
+        __syncwarp();
+        if (lane == 0) {
 #pragma unroll
-        for (int r = 0; r < R; r += 4) row_mem[KEPT ? quarter : 0][what][r / 4] = make_float4(v[r], v[r + 1], v[r + 2], v[r + 3]);
+          for (int r = 0; r < R; r += 4) row_mem[quarter][what][r / 4] = make_float4(v[r], v[r + 1], v[r + 2], v[r + 3]);
+        }
+        __syncwarp();
       }
-      __syncwarp();
     };
     int c = 0, cut_b = -1;
     // one pass per unit, after a first that only looks up the unit to begin with

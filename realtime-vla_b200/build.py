@@ -42,6 +42,7 @@ def _binding_command(nvcc):
     include = [os.path.join(home, "include"), os.path.join(home, "include/torch/csrc/api/include"), sysconfig.get_paths()["include"],
                os.path.join(os.path.dirname(os.path.dirname(nvcc)), "include")]
     libs = ["torch_python", "torch_cpu", "torch", "c10", "c10_cuda", "vla_b200"]
+    # g++ as nvcc finds it: a compiler that links its own libstdc++ does not get on with torch's
     return (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", BINDING_SRC, "-o", BINDING] + ["-I" + d for d in include] +
             ["-L" + os.path.join(home, "lib"), "-L" + HERE] + ["-l" + x for x in libs] + ["-Wl,-rpath,$ORIGIN"])
 

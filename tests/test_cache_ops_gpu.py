@@ -741,3 +741,62 @@ def test_plan_far_positions(block):
     got = vla_ops.block_plan(i32(ctx), i32(new), tab, i32([]), block_size=block, total_new=sum(new))
     assert got.slots.tolist() == slots and got.positions.tolist() == pos and got.seq_lens.tolist() == lens
     assert got.counts.tolist() == [0, missing, sum(new)] and got.cu_new.tolist() == [0, 3, 8, 9, 11, 13] and tab.tolist() == table
+
+
+FIRST_CALLS = """
+import torch, vla_ops
+d = torch.device("cuda", 0)
+q, k = torch.randn(20, 8, 256, device=d).bfloat16(), torch.randn(20, 1, 256, device=d).bfloat16()
+none, new = torch.zeros(1, dtype=torch.int32, device=d), torch.full((1,), 20, dtype=torch.int32, device=d)
+cache, table = vla_ops.kv_cache(300, 1, 16, 256), torch.zeros(1, 200, dtype=torch.int32, device=d)
+free = torch.arange(250, dtype=torch.int32, device=d)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+def run():
+    p = vla_ops.block_plan(none, new, table, free, block_size=16, total_new=20)
+    vla_ops.cache_append(k, k, cache, p.slots)
+    return vla_ops.prompt_attention(q, k, k, p.cu_new), vla_ops.paged_attention(q[None, -1:], cache, table, p.seq_lens)
+with torch.cuda.graph(graph):
+    got = run()
+graph.replay()
+want = run()
+assert all(torch.equal(a, b) for a, b in zip(got, want)) and float(got[0].float().abs().sum()) > 0
+print("same")
+"""
+
+
+def test_first_calls_of_a_process_may_be_captured():
+    import os
+    import subprocess
+    import sys
+
+    import vla_ops
+    env = dict(os.environ, PYTHONPATH=os.path.dirname(os.path.abspath(vla_ops.__file__)))
+    done = subprocess.run([sys.executable, "-c", FIRST_CALLS], env=env, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "same" in done.stdout, done.stderr[-2000:]
+
+
+def test_two_threads():
+    """Each with its own stream and tensors; both get what one alone gets."""
+    import threading
+
+    import vla_ops
+    d = dev()
+    jobs = [pages(40 + i, (3000, 17, 900 + i), 1, 8, 2, 128, 16, torch.bfloat16, d) for i in range(2)]
+    want = [vla_ops.paged_attention(q, cache, table, n) for q, cache, table, n in jobs]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(i):
+        q, cache, table, n = jobs[i]
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[i].append(vla_ops.paged_attention(q, cache, table, n))
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(len(got[i]) == 20 and all(torch.equal(x, want[i]) for x in got[i]) for i in range(2))

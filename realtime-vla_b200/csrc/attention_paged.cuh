@@ -51,7 +51,9 @@ struct PagedAttnParams {
 };
 
 constexpr int PAGED_THREADS = 224;
-constexpr int PAGED_GAP = 12;            // fixed cost of a unit, in groups of 16 tokens
+// Fixed cost of a unit, in groups of 16 tokens.  Measured: 64 sequences of 64 to 8192, heads of 128, with 8, 12, 16, 20: 51.1, 46.6,
+// 46.9, 48.0 us; 83 sequences of 217 to 10009, 3 tokens each, heads of 256: 60.8, 58.2, 54.1, 52.6.
+constexpr int paged_gap(int head_dim) { return head_dim == 256 ? 20 : 12; }
 constexpr int PAGED_MIN_PIECE = 8;       // groups (with gaps) per CTA, at least
 constexpr int PAGED_WHOLE = 32;          // units of at most this many groups are not cut
 
@@ -69,6 +71,7 @@ struct PagedCfg {
   static constexpr int P_BYTES = N * 128;
   static constexpr int SMEM_BYTES = SLOTS * TILE_BYTES + Q_BUFS * Q_BYTES + P_BYTES + 1024;
   static constexpr int PER_SM = D == 256 ? 1 : 2;
+  static constexpr int GAP = paged_gap(D);
   static constexpr int S_COL = 0, O_COL = 2 * N;      // two S buffers, then O per column block
   static constexpr int TMEM_COLS = NT == 1 ? 128 : 256;
   static constexpr uint64_t LAYOUT = D == 64 ? 4ull : 2ull;                 // 64- or 128-byte swizzle
@@ -187,6 +190,7 @@ __device__ __forceinline__ int paged_scan(int v, int* all, int* warp_sum) {
 
 // The parts of units in one piece of the line, in order.  Every role walks on its own; the state is a few registers.  The
 // host refuses sizes whose line could pass 2^31.
+template <int GAP>
 struct PagedWalk {
   int begin, end;        // the piece
   int at, next_at;       // line position of the unit's first tile, and of the next unit's gap
@@ -209,7 +213,7 @@ struct PagedWalk {
         next_rb = 0;
         ++next_h;
       }
-      at = next_at + PAGED_GAP;
+      at = next_at + GAP;
       next_at = at + groups;
       tiles = (groups + 7) >> 3;
       // a border inside a tile belongs to the piece where the tile starts
@@ -291,7 +295,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
       reinterpret_cast<T*>(p.o)[paged_row(p, b, x / (p.rows * D), x / D % p.rows, p.o_seq, p.o_tok, p.o_head) + x % D] = (T)0.f;
   }
   // this CTA's piece of the line, and the sequence it starts in
-  PagedWalk start;
+  PagedWalk<C::GAP> start;
   start.begin = 0;
   start.end = 0;
   int piece = 0, sum = 0;
@@ -302,7 +306,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
     for (int base = 0, rounds = (p.n_seqs + PAGED_THREADS - 1) / PAGED_THREADS; rounds > 0; --rounds, base += PAGED_THREADS) {
       const int b = base + threadIdx.x;
       const int groups = b < p.n_seqs ? (paged_len(p, b) + 15) >> 4 : 0;
-      const int n = groups ? (groups + PAGED_GAP) * p.units : 0;
+      const int n = groups ? (groups + C::GAP) * p.units : 0;
       int all;
       const int at = sum + paged_scan(n, &all, warp_sum);
       sum += all;
@@ -326,7 +330,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
   if (start.begin < start.end) {
     start.next_b = found_b;
     start.len = paged_len(p, found_b);
-    const int one = ((start.len + 15) >> 4) + PAGED_GAP, u = (start.begin - found_base) / one;
+    const int one = ((start.len + 15) >> 4) + C::GAP, u = (start.begin - found_base) / one;
     start.next_h = u / p.row_blocks;
     start.next_rb = u - start.next_h * p.row_blocks;
     start.next_at = found_base + u * one;
@@ -337,7 +341,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
   if (warp == 0) {
     // ---- pages and TMA: lane (j, g) looks after group g of the j-th of four tiles.  Ids are fetched one batch ahead,
     // across units, and scales while the batch before goes out, so that neither latency stands between two loads. ----
-    PagedWalk w = start;
+    PagedWalk<C::GAP> w = start;
     struct Batch { int b, h, len, tile, n; int id; float ks, vs; };
     Batch now, next;
     now.n = 0;
@@ -404,7 +408,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
     if (lane == 0) {
       const uint32_t idesc = (1u << 4) | ((uint32_t)(C::N / 8) << 17) | (8u << 24);       // e4m3 x e4m3 -> fp32, M = 128
       const uint32_t idesc_pv = idesc | (1u << 15);                                        // A MN-major
-      PagedWalk w = start;
+      PagedWalk<C::GAP> w = start;
       int tile = 0, cs = 0, cp = 0, seg = -1;
       bool more = true, turn = true;            // turn: the next S is a unit's first
       // of the tiles whose P V is to come, at most two, even and odd: MMA steps of 32 tokens, negative for a unit's first
@@ -479,7 +483,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
     __syncwarp();
   } else if (warp == 2) {
     // ---- Q pieces: each row times the power of two that brings its largest magnitude to [2^7, 2^8) ----
-    PagedWalk w = start;
+    PagedWalk<C::GAP> w = start;
 #pragma unroll 1
     for (int seg = 0; w.next(p); ++seg) {
       const int qb = seg % C::Q_BUFS, h = w.h, r0 = w.rb * R;
@@ -567,7 +571,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
     };
     // a part, with head, first row, and that row's query and group head
     struct Part { int b, h, rb, len, t0, t1, tiles, at, r0, i0, g0; };
-    PagedWalk walk = start;
+    PagedWalk<C::GAP> walk = start;
     auto take = [&](Part& x) {
       if (!walk.next(p)) return false;
       x.b = walk.b; x.h = walk.h; x.rb = walk.rb; x.len = walk.len; x.t0 = walk.t0; x.t1 = walk.t1; x.tiles = walk.tiles; x.at = walk.at;

@@ -92,7 +92,7 @@ PagedShape paged_shape(const vla_paged_attn_desc* d) {
   const long long groups = (long long)d->width * d->block_size / 16;            // of 16 tokens in a unit, at most
   const long long room = (long long)sm_count() * (d->head_dim == 256 ? 1 : 2);  // CTAs that run at once
   s.whole = groups <= PAGED_WHOLE;
-  s.ctas = std::min(room, s.whole ? units : (units * (groups + PAGED_GAP) + PAGED_MIN_PIECE - 1) / PAGED_MIN_PIECE);
+  s.ctas = std::min(room, s.whole ? units : (units * (groups + paged_gap(d->head_dim)) + PAGED_MIN_PIECE - 1) / PAGED_MIN_PIECE);
   const size_t rows_kept = (size_t)s.ctas * 2 * 8 * s.nt;
   s.workspace = s.whole ? 0 : rows_kept * ((size_t)d->head_dim * sizeof(float) + sizeof(float2)) + (size_t)s.ctas * 4 * sizeof(int);
   return s;
@@ -205,7 +205,7 @@ int vla_op_paged_attention(const vla_paged_attn_desc* d, void* stream) {
     if (!vectors(d->q, d->q_seq_stride, d->q_tok_stride) || d->q_head_stride % 8 || !vectors(d->o, d->o_seq_stride, d->o_tok_stride) || d->o_head_stride % 8)
       return refuse(VLA_ERR_SHAPE, "%s: rows of q and o must start on 16 bytes", who);
     const PagedShape s = paged_shape(d);
-    if ((double)d->n_seqs * d->kv_heads * s.row_blocks * ((double)d->width * d->block_size / 16 + PAGED_GAP) > 2e9)
+    if ((double)d->n_seqs * d->kv_heads * s.row_blocks * ((double)d->width * d->block_size / 16 + paged_gap(d->head_dim)) > 2e9)
       return refuse(VLA_ERR_LIMIT, "%s: more than 2e9 groups of 16 tokens in the table's rows, times key/value heads and blocks of 8 or 16 rows", who);
     if (s.workspace && (!d->workspace || d->workspace_bytes < s.workspace || !aligned(d->workspace, 16)))
       return refuse(VLA_ERR_STATE, "%s: a workspace of %zu bytes on a 16-byte boundary is needed", who, s.workspace);

@@ -324,7 +324,9 @@ int vla_op_cache_append(const vla_cache_append_desc* d, void* stream);
 
 /* O = softmax(scale Q K^T) V of the last n_q tokens of every sequence over the cache: q, o [n_seqs][n_q][heads][head_dim] by
  * strides; query i of sequence b is token seq_lens[b] - n_q + i and sees itself and what is before it (a row before the
- * sequence's start is zero).  Page ids outside the cache are not seen; seq_lens is cut to width * block_size.
+ * sequence's start is zero).  Page ids outside the cache are not seen; seq_lens is cut to width * block_size.  A probability is
+ * held to 2^-12 of itself, and of a row's largest to 2^-25 where the pages' v_scale are alike, 2^-18 (and more slowly
+ * from 2^7 on) where they differ by up to 2^80; what lies further below a row's largest v_scale may be lost.
  * heads is a multiple of kv_heads (consecutive query heads share a key/value head); head_dim 64 | 128 | 256. */
 typedef struct vla_paged_attn_desc {
   const void* q; void* o;

@@ -9,13 +9,17 @@
 // (4 bits a piece, 12 bits in all).  The pieces are further columns of the MMA's N side, which costs nothing that counts:
 //     S[128 tokens x 3R]      = K_tile . (Q0 Q1 Q2)^T       A = K tile, K-major;    R = 8 NT rows
 //     O[128 head dims x 3R]  += V_tile^T . (P0 P1 P2)       A = V tile, MN-major: as the page lies in memory
-// The page's scale of K multiplies S.  That of V goes into the exponent: w = 2^(s + log2 s_v - M), with M the running
-// maximum of that sum, and the softmax's own sum gets w / s_v; so pages of any scales add up in one accumulator, and P
-// has its 12 bits relative to the largest contribution.
+// The page's scale of K multiplies S.  That of V multiplies P: P = 2^(s - m + 7) s_v / 2^L, with m the running maximum of s and
+// 2^L a scale that the unit's pages have at most, and the softmax's own sum gets 2^(s - m + 7).  P is a fixed-point number, 2^8 down
+// to 2^-18, so that only pages whose scales lie close together (PAGED_SPAN) may share one L: else a page that is scaled for one large
+// value, asked for or not, would push the weights of all the others off P's end (with the largest s + log2 s_v as the one
+// reference, a page 2^20 above the rest cost 5% of the result, 2^24 all of it).  A tile with scales further apart is done
+// group by group (apart, below), one P V for each group of scales with a reference of its own; the sums in tensor memory are fp32 and are moved
+// from one reference to the next by whole powers of two.
 //
 // A unit is (sequence, kv head, block of R rows).  All units are laid out in one line, by groups of 16 tokens with a gap
 // for a unit's fixed cost, and the line is cut into equal pieces, one per CTA, whatever the lengths.  A unit cut by a
-// piece's border leaves partial sums in the workspace, which a second kernel joins in a fixed order.
+// piece's border leaves a result for each part in the workspace, which a second kernel joins in a fixed order.
 // Roles, all walking the same piece on their own: warp 0 pages and TMA, warp 1 MMA, warp 2 Q pieces of the next unit, warps
 // 3..6 softmax, one token (and, at a unit's end, one head dim) per thread.  All mbarrier waits are bounded.  Code that
 // runs once per unit is kept in loops: run straight through, it costs about 8 clocks an instruction to fetch.
@@ -45,8 +49,8 @@ struct PagedAttnParams {
   int box_rows;          // 16, 32, 64 or 128 tokens: the largest that divides the block
   float scale_log2e;
   int whole;             // units are short: pieces are cut between units only, nothing to join
-  float* part_o;         // [cta][2][R][D]: sums of a unit's first part (slot 1) or a later one (slot 0)
-  float2* part_ml;       // [cta][2][R]: maximum and sum
+  float* part_o;         // [cta][2][R][D]: result of a unit's first part (slot 1) or a later one (slot 0) by itself
+  float2* part_ml;       // [cta][2][R]: its maximum and sum
   int* cut;              // [cta][4]: the unit that starts in this CTA and ends in another: sequence (-1: none), kv head, row block, last CTA
 };
 
@@ -56,6 +60,14 @@ constexpr int PAGED_THREADS = 224;
 constexpr int paged_gap(int head_dim) { return head_dim == 256 ? 20 : 12; }
 constexpr int PAGED_MIN_PIECE = 8;       // groups (with gaps) per CTA, at least
 constexpr int PAGED_WHOLE = 32;          // units of at most this many groups are not cut
+
+// Scales of V with one reference 2^L: 2^(L - PAGED_SPAN - 1) < s_v <= 2^L, so that the last piece of P ends 2^-18 below the largest
+// probability at the most, and 2^-25 below it where all scales are alike.
+constexpr int PAGED_SPAN = 6;
+// Scales more than 2^80 below the largest that a part has seen share the lowest reference: with 2^8 of P, 2^9 of the codes and 2^17
+// tokens or more, sums relative to less could leave fp32.
+constexpr int PAGED_REACH = 80;
+constexpr int PAGED_NONE = -1000;        // no page with a scale
 
 template <int D, int NT>
 struct PagedCfg {
@@ -99,6 +111,27 @@ __device__ __forceinline__ void paged_tmem_ld(uint32_t taddr, int apart, uint32_
                  : "memory");
   tmem_ld_wait();
 }
+// One of them.
+__device__ __forceinline__ void paged_tmem_ld8(uint32_t taddr, uint32_t (&v)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(taddr) : "memory");
+  tmem_ld_wait();
+}
+__device__ __forceinline__ void paged_tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+  tmem_st_wait();
+}
+// Those of two rows.
+__device__ __forceinline__ float2 paged_tmem_ld2(uint32_t taddr, int apart) {
+  uint32_t v[3][2];
+#pragma unroll
+  for (int i = 0; i < 3; ++i)
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0, %1}, [%2];" : "=r"(v[i][0]), "=r"(v[i][1]) : "r"(taddr + i * apart) : "memory");
+  tmem_ld_wait();
+  auto sum = [&](int r) { return fmaf(__uint_as_float(v[2][r]), 0x1p-8f, fmaf(__uint_as_float(v[1][r]), 0x1p-4f, __uint_as_float(v[0][r]))); };
+  return make_float2(sum(0), sum(1));
+}
 __device__ __forceinline__ void paged_tmem_st(uint32_t taddr, int apart, const uint32_t (&v)[24]) {
 #pragma unroll
   for (int i = 0; i < 3; ++i)
@@ -135,6 +168,14 @@ __device__ __forceinline__ float rcp_approx(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// The smallest L >= -100 with |x| <= 2^L, and 2^L for -126 <= L <= 127.
+__device__ __forceinline__ int scale_level(float x) {
+  const int bits = __float_as_int(x) & 0x7fffffff;
+  return max((bits >> 23) - 127 + ((bits & 0x7fffff) != 0), -100);
+}
+__device__ __forceinline__ float power_of_2(int e) { return __int_as_float((e + 127) << 23); }
+// x / 2^L for L of scale_level
+__device__ __forceinline__ float below_level(float x, int level) { return x * 0.25f * power_of_2(2 - level); }
 __device__ __forceinline__ float lg2_approx(float x) {
   float y;
   asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -226,6 +267,7 @@ struct PagedWalk {
   __device__ __forceinline__ int cut(const PagedAttnParams& p, int x) const { return x <= at ? 0 : p.whole ? tiles : min(tiles, (x - at + 7) >> 3); }
 };
 
+
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) paged_attention_kernel(const __grid_constant__ PagedAttnParams p) {
   using C = PagedCfg<D, NT>;
@@ -234,14 +276,19 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
   __shared__ __align__(8) uint64_t bar_mem[2 * C::SLOTS + 8];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_mem, poison_mem[3];          // poison: a hidden value of the unit was NaN (units in turn)
+  __shared__ int again_mem;                         // this tile has a further P V: apart
   __shared__ int found_b, found_base, warp_sum[PAGED_THREADS / 32];
-  // of the 8 groups of a tile, written and handed back with its V: scale of K, log2 and inverse of the scale of V, 0 where
-  // no page is
+  // of the 8 groups of a tile, written and handed back with its V: scale of K, whether there is a page, scale of V, and highest and lowest
+  // level of the scales of V in the tile (two 16-bit numbers)
   __shared__ float4 page_info[C::SLOTS / 2][8];
   __shared__ float q_scale[2][R];
-  // with two CTAs an SM: each softmax warp's copy of the scale of Q and the maximum of each row, the same for all its lanes
+  // each softmax warp's copy of the scale of Q and the maximum of each row, the same for all its lanes; with two CTAs an SM they are
+  // kept there only
   constexpr bool KEPT = C::PER_SM == 2;
-  __shared__ float4 row_mem[KEPT ? 4 : 1][2][R / 4];
+  __shared__ float4 row_mem[4][2][R / 4];
+  // as well: what O of the part at hand is relative to, O = sum 2^(s - m + 7) s_v / 2^x; the levels from which, y, and up to which, w, x may
+  // follow the scales without a look at the scores; the highest level so far, z
+  __shared__ int4 level_mem[4];
   __shared__ float4 warp_max[R], warp_sums[2][R];   // by row, of the four softmax warps (sums: of odd and even units)
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t pad = (1024u - (raw_addr & 1023u)) & 1023u;
@@ -260,6 +307,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
   auto q_empty = [&](int b) { return bars + 8 * (B0 + 6 + b); };
   volatile int* abort_flag = &abort_mem;
   volatile int* poison = poison_mem;
+  volatile int* again_flag = &again_mem;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -276,7 +324,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
     }
     mbar_init(p_ready, 128);
     mbar_init(o_done, 1);
-    abort_mem = 0;
+    abort_mem = again_mem = 0;
     poison_mem[0] = poison_mem[1] = poison_mem[2] = 0;
     mbar_fence_init();
     tma_prefetch_desc(&p.tmK);
@@ -345,7 +393,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
     struct Batch { int b, h, len, tile, n; int id; float ks, vs; };
     Batch now, next;
     now.n = 0;
-    int c = 0, tile = 0;
+    int c = 0, tile = 0, levels = 0;
     bool ok = true, more = w.next(p);
     if (more) tile = w.t0;
     const uint64_t pol = policy_evict_normal();
@@ -386,10 +434,20 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
             for (int x = 0; x < C::HALVES; ++x)
               tma_load_3d(dst + x * C::BLOCK_BYTES, kv ? &p.tmV : &p.tmK, full(s + kv), x * 128, row, now.id, pol);
           }
-          if (kv == 1 && here) {                // the scales may come in later than the loads go out
-            const float v = fmaxf(now.vs, 0x1p-100f);      // a page of zeros may have any scale, zero too; NaN stays
-            page_info[c % HALF][g] = now.id < 0 ? make_float4(0.f, 0.f, 0.f, 0.f)
-                                                : make_float4(now.ks, now.vs != now.vs ? now.vs : lg2_approx(v), now.vs != now.vs ? now.vs : 1.f / v, 1.f);
+          if (kv == 1) {                        // the scales may come in later than the loads go out
+            const bool on = now.id >= 0, finite = on && fabsf(now.vs) < INFINITY;
+            const float vs = finite ? now.vs : 0.f;
+            if (j == 0) {                       // of every tile of the batch
+              int hi = vs != 0.f ? scale_level(vs) : PAGED_NONE, lo = vs != 0.f ? hi : -PAGED_NONE;
+#pragma unroll
+              for (int o = 1; o < 8; o <<= 1) {
+                hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+                lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+              }
+              levels = hi << 16 | (lo & 0xffff);
+            }
+            // a scale of V that is not finite makes the tokens' scores NaN, and so every row that sees one
+            if (here) page_info[c % HALF][g] = make_float4(!on ? 0.f : finite ? now.ks : NAN, on ? 1.f : 0.f, vs, __int_as_float(levels));
           }
           __syncwarp();                         // page_info goes out with lane 0's arrival
           if (lane == 0) mbar_expect_tx(full(s + kv), bytes);
@@ -409,7 +467,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
       const uint32_t idesc = (1u << 4) | ((uint32_t)(C::N / 8) << 17) | (8u << 24);       // e4m3 x e4m3 -> fp32, M = 128
       const uint32_t idesc_pv = idesc | (1u << 15);                                        // A MN-major
       PagedWalk<C::GAP> w = start;
-      int tile = 0, cs = 0, cp = 0, seg = -1;
+      int tile = 0, cs = 0, cp = 0, pv = 0, seg = -1;     // pv: P V so far, of which a tile has one, or another odd number
       bool more = true, turn = true;            // turn: the next S is a unit's first
       // of the tiles whose P V is to come, at most two, even and odd: MMA steps of 32 tokens, negative for a unit's first
       int steps_of[2] = {0, 0};
@@ -452,8 +510,9 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
         }
         if (cp < cs) {
           const int s = 2 * (cp % HALF) + 1;
-          if (mbar_test(p_ready, (uint32_t)cp & 1u) && mbar_test(full(s), (uint32_t)(cp / HALF) & 1u)) {
+          if (mbar_test(p_ready, (uint32_t)pv & 1u) && mbar_test(full(s), (uint32_t)(cp / HALF) & 1u)) {
             tc_fence_after();
+            const bool again = *again_flag;
             const uint64_t vd = v_desc + s * (C::TILE_BYTES / 16);
             const int steps = steps_of[cp & 1];
 #pragma unroll
@@ -462,9 +521,11 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
               for (int k = 0; k < 4; ++k)
                 if (k < abs(steps))
                   umma_f8(tmem + C::O_COL + x * C::N, vd + x * (C::BLOCK_BYTES / 16) + k * (32 * C::ROW_BYTES / 16), p_desc + 2 * k, idesc_pv, steps > 0 || k != 0);
-            umma_commit(empty(s));
+            if (!again) umma_commit(empty(s));
             umma_commit(o_done);
-            ++cp;
+            ++pv;
+            if (again) steps_of[cp & 1] = abs(steps);
+            else ++cp;
             did = true;
           }
         }
@@ -594,14 +655,148 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
       }
     };
     auto to_mem = [&](int what, const float (&v)[R]) {
-      if constexpr (KEPT) {
-        __syncwarp();
-        if (lane == 0) {
+      __syncwarp();
+      if (lane == 0) {
 #pragma unroll
-          for (int r = 0; r < R; r += 4) row_mem[quarter][what][r / 4] = make_float4(v[r], v[r + 1], v[r + 2], v[r + 3]);
-        }
-        __syncwarp();
+        for (int r = 0; r < R; r += 4) row_mem[quarter][what][r / 4] = make_float4(v[r], v[r + 1], v[r + 2], v[r + 3]);
       }
+      __syncwarp();
+    };
+    const uint32_t o_at = tmem + lane_off + C::O_COL;
+    uint8_t* const p_col = p_mem + (tid & 15);
+    auto put = [&](int r, float a, float b) {      // P of rows r, r + 1
+      uint32_t pc[3];
+      pieces(a, b, pc);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        const int n = k * R + r;
+        p_col[n * 128 + (((tid >> 4) ^ (n & 7)) << 4)] = (uint8_t)pc[k];
+        p_col[(n + 1) * 128 + (((tid >> 4) ^ ((n + 1) & 7)) << 4)] = (uint8_t)(pc[k] >> 8);
+      }
+    };
+    auto move = [&](int by) {                    // O *= 2^by, by that of lane r for row r
+#pragma unroll 1
+      for (int y = 0; y < C::HALVES * 3 * R; y += 8) {         // 8 rows of one piece
+        const uint32_t at = o_at + y / (3 * R) * C::N + y % (3 * R);
+        uint32_t o[8];
+        paged_tmem_ld8(at, o);
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          o[r] = __float_as_uint(__uint_as_float(o[r]) * power_of_2(min(max(__shfl_sync(0xffffffffu, by, y % R + r), -126), 127)));
+        paged_tmem_st8(at, o);
+      }
+    };
+    // The reference follows a tile whose highest scale is somewhat larger.  Lower ones need no move.
+    auto follow = [&](int c, int hi, int lo, bool first) {
+      int4* const lv = &level_mem[quarter];
+      if (lv->y == -PAGED_NONE || hi <= lv->x || hi > lv->w || lo < hi - PAGED_SPAN) return false;
+      const int by = lv->x - hi;
+      if (c > 0) wait(o_done, (uint32_t)(c - 1) & 1u);
+      tc_fence_after();
+      if (!first) move(by);
+      if (lane == 0) *lv = make_int4(hi, hi - PAGED_SPAN, max(lv->z, hi), lv->w);
+      __syncwarp();
+      return true;
+    };
+    // P of a tile whose scales of V lie further apart, or elsewhere than those that the part's reference is made for.  Tokens are
+    // taken by groups of levels, from the highest down, each with a reference that fits the products 2^s s_v of that group alone:
+    // that of row r is 2^(m - g + L), with a whole number g >= 0 in lane r.  P V runs once for each group, over the same V; between
+    // two, O is moved by whole powers of two.  In the end O is relative to 2^(m + x) again, where x is made for the level of a
+    // group that holds next to the largest probabilities in all rows; where there is none and the maxima have just moved, no
+    // level is known to fit, and the next tile comes here as well.  The number of P V is odd, with an empty one if need be, so
+    // that the phases of the barriers stay those of one a tile.  Rare, so that it is kept in loops that need few registers: S is read
+    // again row by row (as a function of its own, with the call in the loop over tiles, all other tiles took half as long again).
+    // 64 sequences of 64 to 8192 tokens, 32 heads on 8 of 128: 49 us with scales within 2^5, 270 with a scale of its own out of 2^9 for
+    // each page, 465 out of 2^60; 4 of 90001 to 131071, 8 heads on 1 of 256: 51, 133 and 255.
+    auto apart = [&](int c, int tok, int len, int lim_min, int g0, bool first, bool moved) {
+      const float4* const infos = page_info[c % HALF];
+      int4* const lv = &level_mem[quarter];
+      auto level_of = [&](float v) { return v != 0.f ? scale_level(v) : PAGED_NONE; };
+      auto highest = [&](int under) {              // of the tile's levels
+        int most = PAGED_NONE;
+#pragma unroll 1
+        for (int k = 0; k < 8; ++k) {
+          const int l = level_of(infos[k].z);
+          if (l < under) most = max(most, l);
+        }
+        return most;
+      };
+      auto scores = [&](int r) {                   // of rows r, r + 1
+        float2 x = paged_tmem_ld2(tmem + lane_off + C::S_COL + (c & 1) * C::N + r, R);
+        const float* qs = reinterpret_cast<const float*>(row_mem[quarter][0]);
+        const float4 info = infos[tid >> 4];
+        x.x *= qs[r] * info.x;
+        x.y *= qs[r + 1] * info.x;
+        if (info.y == 0.f || tok >= min(len, lim_min + (g0 + r) / p.group)) x.x = -INFINITY;
+        if (info.y == 0.f || tok >= min(len, lim_min + (g0 + r + 1) / p.group)) x.y = -INFINITY;
+        return x;
+      };
+      const float* const maxima = reinterpret_cast<const float*>(row_mem[quarter][1]);
+      auto least = [&]() { return lv->z - PAGED_REACH; };          // no reference below 2^(m + least): the sums have to stay within fp32
+      int level = highest(1 - PAGED_NONE), under = 1 - PAGED_NONE, at = lv->x, g = 0, fits = PAGED_NONE, pass = 0;
+      if (lane == 0) lv->z = max(lv->z, level);
+#pragma unroll 1
+      for (;; ++pass) {
+        named_barrier_sync(1, 128);                // warp_max has been read
+        const int from = level - PAGED_SPAN, ref = level == PAGED_NONE ? at : max(level, least());
+        const float vs = infos[tid >> 4].z;
+        const int mine = level_of(vs);
+        const float f = mine < under && mine >= from && mine != PAGED_NONE ? below_level(vs, ref) : 0.f;
+        const float up = f != 0.f ? lg2_approx(fabsf(f)) : -INFINITY;
+#pragma unroll 1
+        for (int r = 0; r < R; r += 2) {
+          const float2 x = scores(r);
+          const float a = warp_max_f32(x.x + up), b = warp_max_f32(x.y + up);
+          if (lane == 0) {
+            reinterpret_cast<float*>(&warp_max[r])[quarter] = a;
+            reinterpret_cast<float*>(&warp_max[r + 1])[quarter] = b;
+          }
+        }
+        const int next = level == PAGED_NONE ? PAGED_NONE : highest(from);
+        const bool again = next != PAGED_NONE || (pass & 1);
+        named_barrier_sync(1, 128);
+        const float4 tops = warp_max[lane % R];
+        const float own_m = maxima[lane % R];
+        const float below = own_m - fmaxf(fmaxf(tops.x, tops.y), fmaxf(tops.z, tops.w));       // NaN: the row has seen nothing
+        const bool near = __all_sync(0xffffffffu, own_m == -INFINITY || below <= PAGED_SPAN + 1.f);
+        if (near && fits == PAGED_NONE) fits = level;
+        int to = below < (float)PAGED_REACH ? max((int)floorf(below) + 1, 0) : below < INFINITY ? PAGED_REACH : 0;
+        to = level == PAGED_NONE ? g : min(to, ref - least());
+        const int by = to - g + at - ref;
+        g = to;
+        at = ref;
+        if (c + pass > 0) wait(o_done, (uint32_t)(c + pass - 1) & 1u);     // the P V before has read P, and O is complete
+        tc_fence_after();
+        if (!(first && pass == 0)) move(by);
+#pragma unroll 1
+        for (int r = 0; r < R; r += 2) {
+          const float2 x = scores(r);
+          const float m0 = maxima[r], m1 = maxima[r + 1];
+          const float up0 = (float)(__shfl_sync(0xffffffffu, g, r) + 7), up1 = (float)(__shfl_sync(0xffffffffu, g, r + 1) + 7);
+          put(r, f * ex2_approx(x.x - (m0 == -INFINITY ? 0.f : m0) + up0), f * ex2_approx(x.y - (m1 == -INFINITY ? 0.f : m1) + up1));
+        }
+        if (tid == 0) *again_flag = again;         // the MMA looks at it behind p_ready
+        fence_proxy_async_shared();
+        tc_fence_before();
+        mbar_arrive(p_ready);
+        if (!again) break;
+        under = from;
+        level = next;
+      }
+      const int home = max(fits != PAGED_NONE ? fits : lv->x, least());
+      if (lane == 0) {                             // the others have read it: barriers
+        if (fits != PAGED_NONE) {
+          lv->y = fits - PAGED_SPAN;
+          lv->w = fits + PAGED_SPAN;
+        } else if (moved) {
+          lv->y = -PAGED_NONE;
+        }
+      }
+      wait(o_done, (uint32_t)(c + pass) & 1u);
+      tc_fence_after();
+      move(at - g - home);
+      if (lane == 0) lv->x = home;
+      __syncwarp();
     };
     int c = 0, cut_b = -1;
     // one pass per unit, after a first that only looks up the unit to begin with
@@ -616,11 +811,11 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
         wait(full(s + 1), (uint32_t)(c / HALF) & 1u);
         const float4 info = page_info[c % HALF][tid >> 4];
         const bool edge = tile * 128 + 128 > lim_min;
-        if (edge || !__all_sync(0xffffffffu, info.w != 0.f)) {
+        if (edge || !__all_sync(0xffffffffu, info.y != 0.f)) {
           // A row of V that no row of this unit sees is cleared; where only some see it, a NaN in it is, and the end of
           // the unit gives it back: P is zero there, but zero times NaN is NaN.
           uint8_t* row = ring + (s + 1) * C::TILE_BYTES + tid * C::ROW_BYTES;
-          const bool none = tok >= w.len || info.w == 0.f;
+          const bool none = tok >= w.len || info.y == 0.f;
           if ((none || tok >= lim_min) && tid < (min(w.len - tile * 128, 128) + 31) / 32 * 32) {   // of what P V reads
 #pragma unroll 2
             for (int x = 0; x < D / 16; ++x) {
@@ -655,13 +850,13 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
           if (lane == 0) mbar_arrive(q_empty(seg % C::Q_BUFS));
         }
         from_mem(0, qs);
-        float x[R];                              // s + log2 s_v
+        float x[R];                              // s
 #pragma unroll
         for (int r8 = 0; r8 < R; r8 += 8) {
           uint32_t v[24];
           paged_tmem_ld(tmem + lane_off + C::S_COL + (c & 1) * C::N + r8, R, v);
 #pragma unroll
-          for (int r = 0; r < 8; ++r) x[r8 + r] = info.w == 0.f ? -INFINITY : fmaf(paged_sum(v, r), qs[r8 + r] * info.x, info.y);
+          for (int r = 0; r < 8; ++r) x[r8 + r] = info.y == 0.f ? -INFINITY : paged_sum(v, r) * (qs[r8 + r] * info.x);
         }
         if (edge) {
           int lim = min(w.len, lim_min), left = p.group - g0;   // rows of a query follow one another
@@ -674,12 +869,17 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
             }
           }
         }
+        if (tile == w.t0 && lane == 0) {         // a part begins with the level of its first tile, if there is one for all of it
+          const int hi = __float_as_int(info.w) >> 16, lo = (int)(short)__float_as_int(info.w), at = max(hi, -100);
+          level_mem[quarter] = make_int4(at, hi - lo <= PAGED_SPAN ? at - PAGED_SPAN : -PAGED_NONE, at, at + PAGED_SPAN);
+        }
         from_mem(1, m);
-        bool grow = false;
+        bool grow = false, moved = false;
 #pragma unroll
         for (int r = 0; r < R; ++r) grow |= x[r] > m[r] + 1.f;
-        // The subtracted maximum moves when a token has outgrown it by more than 2: w stays below 2 * 2^7, in e4m3's range.
+        // The subtracted maximum moves when a token has outgrown it by more than 2: P stays below 2 * 2^7, in e4m3's range.
         if (tile == w.t0 || barrier_any(1, grow)) {
+          moved = true;
 #pragma unroll
           for (int r = 0; r < R; ++r) {
             const float top = warp_max_f32(x[r]);
@@ -712,26 +912,28 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
             }
           }
         }
-        if (c > 0) wait(o_done, (uint32_t)(c - 1) & 1u);   // P of the tile before has been read
         from_mem(1, m);
-        uint8_t* p_col = p_mem + (tid & 15);
-        const int chunk = tid >> 4;
+        // read again instead of kept, and the levels as well: registers are short here
+        const float2 scale = *reinterpret_cast<const float2*>(&page_info[c % HALF][tid >> 4].z);
+        const int2 lv = *reinterpret_cast<const int2*>(&level_mem[quarter]);
+        const int hi = __float_as_int(scale.y) >> 16, lo = (int)(short)__float_as_int(scale.y);       // the same in all threads
+        if (__builtin_expect(hi > lv.x || lo < lv.y, 0) && !follow(c, hi, lo, tile == w.t0)) {
+#pragma unroll
+          for (int r = 0; r < R; ++r) l[r] += ex2_approx(x[r] - (m[r] == -INFINITY ? 0.f : m[r]) + 7.f);
+          apart(c, tok, w.len, lim_min, g0, tile == w.t0, moved);
+          continue;
+        }
+        if (c > 0) wait(o_done, (uint32_t)(c - 1) & 1u);   // P of the tile before has been read
+        const float f = below_level(scale.x, level_mem[quarter].x);
 #pragma unroll
         for (int r = 0; r < R; r += 2) {
           float e[2];
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             e[k] = ex2_approx(x[r + k] - (m[r + k] == -INFINITY ? 0.f : m[r + k]) + 7.f);
-            if (e[k] != 0.f) l[r + k] = fmaf(e[k], info.z, l[r + k]);   // a hidden token's scale may be NaN
+            l[r + k] += e[k];
           }
-          uint32_t pc[3];
-          pieces(e[0], e[1], pc);
-#pragma unroll
-          for (int k = 0; k < 3; ++k) {
-            const int n = k * R + r;
-            p_col[n * 128 + ((chunk ^ (n & 7)) << 4)] = (uint8_t)pc[k];
-            p_col[(n + 1) * 128 + ((chunk ^ ((n + 1) & 7)) << 4)] = (uint8_t)(pc[k] >> 8);
-          }
+          put(r, e[0] * f, e[1] * f);
         }
         fence_proxy_async_shared();
         tc_fence_before();
@@ -790,6 +992,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
             }
           }
           const int n_rows = min(R, p.rows - r0);
+          const float at = power_of_2(level_mem[quarter].x - 2);  // 2^128 is not a number
 #pragma unroll
           for (int r = 0; r < R; ++r)
             if (nans >> r & 1) val[r] = NAN;
@@ -800,7 +1003,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
             for (int r = 0; r < R; ++r) {
               const float4 sums = warp_sums[seg & 1][r];
               const float sum = (sums.x + sums.y) + (sums.z + sums.w);
-              if (r < n_rows) *dst = (T)(sum == 0.f ? 0.f : val[r] * rcp_approx(sum));       // 0: nothing seen
+              if (r < n_rows) *dst = (T)(sum == 0.f ? 0.f : val[r] * rcp_approx(sum) * at * 4.f);       // 0: nothing seen
               --left;
               dst += left ? p.o_head : turn;
               left = left ? left : p.group;
@@ -813,8 +1016,8 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
             for (int r = 0; r < R; ++r) {
               const float4 sums = warp_sums[seg & 1][r];
               const float sum = (sums.x + sums.y) + (sums.z + sums.w);
-              if (r < n_rows) part[r * D] = sum == 0.f ? 0.f : val[r];
-              if (d == r) part_ml[r] = make_float2(m[r], sum);
+              if (r < n_rows) part[r * D] = sum == 0.f ? 0.f : val[r] * rcp_approx(sum) * at * 4.f;
+              if (d == r) part_ml[r] = make_float2(m[r], sum * 0x1p-40f);      // the join's products with it stay finite
             }
           }
         }
@@ -841,7 +1044,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
   if (warp == 1) tmem_dealloc(tmem, C::TMEM_COLS);
 }
 
-// Joins the partial sums of the units that were cut: block (c, y) does two or four rows of the unit that starts in piece c.  A row's
+// Joins the parts of the units that were cut, each with its share of the unit's sum: block (c, y) does two or four rows of the unit that starts in piece c.  A row's
 // parts are dealt out to groups of D / 4 threads, which take four head dims each; the groups' sums are then added in order.
 constexpr int PAGED_JOIN_THREADS = 512;
 template <int D>
@@ -869,11 +1072,12 @@ __global__ void __launch_bounds__(PAGED_JOIN_THREADS) paged_join_kernel(const __
     const float4 v = *reinterpret_cast<const float4*>(p.part_o + at(i) * D + 4 * lane);
     const float top = fmaxf(m, ml.x), a = weight(m, top), b = weight(ml.x, top);
     m = top;
-    sum = sum * a + ml.y * b;
-    acc.x = acc.x * a + v.x * b;
-    acc.y = acc.y * a + v.y * b;
-    acc.z = acc.z * a + v.z * b;
-    acc.w = acc.w * a + v.w * b;
+    const float weigh = ml.y * b;
+    sum = sum * a + weigh;
+    acc.x = acc.x * a + v.x * weigh;
+    acc.y = acc.y * a + v.y * weigh;
+    acc.z = acc.z * a + v.z * weigh;
+    acc.w = acc.w * a + v.w * weigh;
   }
   sums[group][row][lane] = acc;
   if (lane == 0) group_ml[group][row] = make_float2(m, sum);

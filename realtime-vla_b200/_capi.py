@@ -113,6 +113,7 @@ EXPORTS = {
     "vla_op_paged_attention": (C.c_int, [C.POINTER(PagedAttnDesc), C.c_void_p]),
     "vla_op_prompt_attention": (C.c_int, [C.POINTER(PromptAttnDesc), C.c_void_p]),
     "vla_op_cache_status": (C.c_int, [C.POINTER(C.c_int)]),
+    "vla_op_cache_wait_expire": (C.c_int, [C.c_int, C.c_void_p]),
     "vla_op_norm": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p]),
 }
 

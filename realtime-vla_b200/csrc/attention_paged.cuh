@@ -980,7 +980,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
           }
           const int d = y * 128 + tid;
           if (d >= D) break;
-          uint32_t nans = 0;                       // rows that see a NaN in this head dim
+          uint32_t nans = *abort_flag ? ~0u : 0u;  // rows that see a NaN in this head dim, or that a wait left incomplete
           if (bad) {
 #pragma unroll 1
             for (int tok = max(lim_min, w.t0 * 128); tok < min(w.len, w.t1 * 128); ++tok) {
@@ -1003,7 +1003,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
             for (int r = 0; r < R; ++r) {
               const float4 sums = warp_sums[seg & 1][r];
               const float sum = (sums.x + sums.y) + (sums.z + sums.w);
-              if (r < n_rows) *dst = (T)(sum == 0.f ? 0.f : val[r] * rcp_approx(sum) * at * 4.f);       // 0: nothing seen
+              if (r < n_rows) *dst = (T)(sum == 0.f && !(nans >> r & 1) ? 0.f : val[r] * rcp_approx(sum) * at * 4.f);       // 0: nothing seen
               --left;
               dst += left ? p.o_head : turn;
               left = left ? left : p.group;
@@ -1016,7 +1016,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
             for (int r = 0; r < R; ++r) {
               const float4 sums = warp_sums[seg & 1][r];
               const float sum = (sums.x + sums.y) + (sums.z + sums.w);
-              if (r < n_rows) part[r * D] = sum == 0.f ? 0.f : val[r] * rcp_approx(sum) * at * 4.f;
+              if (r < n_rows) part[r * D] = sum == 0.f && !(nans >> r & 1) ? 0.f : val[r] * rcp_approx(sum) * at * 4.f;
               if (d == r) part_ml[r] = make_float2(m[r], sum * 0x1p-40f);      // the join's products with it stay finite
             }
           }

@@ -492,6 +492,10 @@ __global__ void __launch_bounds__(PromptCfg<WIDE>::THREADS, WIDE ? 1 : 2) prompt
           *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.o) + at + piece * 8) =
               *reinterpret_cast<const uint4*>(from + rr * 128 + (((piece & 7) ^ (rr & 7)) << 4));
       }
+    } else if (row_ok) {                         // a wait ran out: no row is left as it was
+      T* const row = reinterpret_cast<T*>(p.o) + (long long)(q0 + tok) * p.o_tok + (long long)(kvh * p.group + r % p.group) * p.o_head;
+#pragma unroll 1
+      for (int d = 0; d < p.dim; ++d) row[d] = (T)NAN;
     }
   }
 

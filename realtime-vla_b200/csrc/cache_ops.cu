@@ -4,6 +4,7 @@
 #include <algorithm>
 #include <cstdarg>
 #include <cstdio>
+#include <mutex>
 #include <type_traits>
 
 #include "../../include/vla_b200.h"
@@ -301,11 +302,26 @@ int vla_op_prompt_attention(const vla_prompt_attn_desc* d, void* stream) {
 
 int vla_op_cache_status(int* out) {
   const char* who = "vla_op_cache_status";
-  if (!out) return refuse(VLA_ERR_STATE, "%s: null argument", who);
-  const int zero = 0;
-  cudaError_t e = cudaMemcpyFromSymbol(out, cache_ops_status, sizeof(int));
-  if (e == cudaSuccess && *out) e = cudaMemcpyToSymbol(cache_ops_status, &zero, sizeof(int));
-  return launched(who, e);
+  return guarded(who, [&]() -> int {
+    if (!out) return refuse(VLA_ERR_STATE, "%s: null argument", who);
+    static std::mutex mu;                  // one look at a time: each has its answer in the same place
+    std::lock_guard<std::mutex> lock(mu);
+    cudaError_t e = cudaDeviceSynchronize();             // streams that do not wait for the default one as well
+    if (e == cudaSuccess) {
+      cache_status_kernel<<<1, 1>>>();
+      e = cudaGetLastError();
+    }
+    if (e == cudaSuccess) e = cudaMemcpyFromSymbol(out, cache_ops_taken, sizeof(int));
+    return launched(who, e);
+  });
+}
+
+int vla_op_cache_wait_expire(int limit_us, void* stream) {
+  const char* who = "vla_op_cache_wait_expire";
+  return guarded(who, [&]() -> int {
+    if (limit_us < 1 || limit_us > 1000000) return refuse(VLA_ERR_LIMIT, "%s: the limit must be 1 to 1000000 microseconds", who);
+    return launched(who, launch_ex(cache_wait_kernel, dim3(1), dim3(1), 0, reinterpret_cast<cudaStream_t>(stream), 1, false, limit_us * 1000ull));
+  });
 }
 
 }  // extern "C"

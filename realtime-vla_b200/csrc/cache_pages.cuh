@@ -7,6 +7,19 @@
 
 // Bits VLA_ST_* of the operators in this translation unit: a bounded wait that ran out.
 static __device__ int cache_ops_status;
+static __device__ int cache_ops_taken;       // what the last look at it found
+
+// Reads and clears in one step: a bit that is set meanwhile stays for the next look.
+static __global__ void cache_status_kernel() { cache_ops_taken = atomicExch(&cache_ops_status, 0); }
+// A wait that nothing ends, as the others are when something goes wrong.
+static __global__ void cache_wait_kernel(unsigned long long limit_ns) {
+  __shared__ __align__(8) uint64_t bar;
+  __shared__ int abort_mem;
+  mbar_init(smem_u32(&bar), 1);
+  mbar_fence_init();
+  abort_mem = 0;
+  if (!mbar_wait_small(smem_u32(&bar), 0, &abort_mem, limit_ns)) atomicOr(&cache_ops_status, VLA_ST_WAIT_TIMEOUT);
+}
 
 // ---- block tables and slot maps ------------------------------------------------------------------------------------
 // Request b holds ctx[b] tokens in have = ceil(ctx / bs) blocks and gets n[b] more; it takes want - have blocks, want =

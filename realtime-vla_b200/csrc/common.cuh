@@ -80,7 +80,7 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 }
 // The same with its polls in a loop: the wait above is 4 KB of code at each of its places, which costs a kernel that runs for a
 // few microseconds more than it saves, while the persistent kernels lose 1% with this one.
-__device__ __forceinline__ bool mbar_wait_small(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+__device__ __forceinline__ bool mbar_wait_small(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint64_t limit_ns = VLA_WAIT_LIMIT_NS) {
   if (mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = globaltimer_ns();
   for (;;) {
@@ -88,7 +88,7 @@ __device__ __forceinline__ bool mbar_wait_small(uint32_t bar, uint32_t parity, v
     for (int i = 0; i < 64; ++i)
       if (mbar_try_wait(bar, parity)) return true;
     if (*abort_flag) return false;
-    if (globaltimer_ns() - t0 > VLA_WAIT_LIMIT_NS) {
+    if (globaltimer_ns() - t0 > limit_ns) {
       *abort_flag = 1;
       return false;
     }

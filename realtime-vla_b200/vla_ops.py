@@ -3,7 +3,8 @@ micro-benchmarks call the kernels through these.
 
 The operators around a key/value cache in pages (block_plan, cache_append, paged_attention, prompt_attention) are for
 programs that serve sequences of different lengths: they take torch tensors, enqueue on the current stream of the tensors'
-device and return without synchronising, so they can be captured into a CUDA graph.  They run forward only."""
+device and return without synchronising, so they can be captured into a CUDA graph.  They run forward only.  Waits inside their
+kernels are bounded; cache_status() says whether one ran out."""
 import ctypes as C
 from typing import NamedTuple
 
@@ -185,3 +186,13 @@ def prompt_attention(q, k, v, cu_q, cu_k=None, *, causal=True, scale=None, out=N
     of a sequence sees all its keys, each row before it one less; otherwise every row sees all.  Returns out, or a new
     tensor like q; a row that sees nothing is zero, rows behind the last sequence are not written."""
     return _native.prompt_attention(q, k, v, cu_q, cu_k, causal, scale, out)
+
+
+def cache_status(device=None):
+    """Whether the operators around the cache have run to their end on a device since the last call of this: 0, or bit 0 set where a
+    bounded wait inside a kernel ran out and the output of some call is not to be trusted.  Waits for all work on the device;
+    a serving loop calls it where it waits anyway, and not while a stream is captured."""
+    word = C.c_int(0)
+    with torch.cuda.device(device):
+        _capi.check(_capi.lib().vla_op_cache_status(C.byref(word)))
+    return word.value

@@ -124,3 +124,11 @@ def test_wrappers_refuse_what_is_no_tensor():
               lambda: vla_ops.cache_append(3, i, None, i), lambda: vla_ops.block_plan("x", i, i, i, block_size=16, total_new=0)):
         with pytest.raises(_capi.VlaError, match="must be a tensor"):
             f()
+
+
+@needs_library
+def test_status_refusals():
+    lib = _capi.lib()
+    assert lib.vla_op_cache_status(None) == STATE and "null" in lib.vla_last_error(None).decode()
+    for limit in (0, -1, 1000001):
+        assert lib.vla_op_cache_wait_expire(limit, None) == LIMIT and "microseconds" in lib.vla_last_error(None).decode()

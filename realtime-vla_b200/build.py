@@ -4,10 +4,13 @@ import os
 import subprocess
 import sys
 import sysconfig
+from importlib import metadata
+from importlib.util import find_spec
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB = os.path.join(HERE, "libvla_b200.so")
 BINDING, BINDING_SRC = os.path.join(HERE, "_vla_ops.so"), "csrc/binding.cpp"
+BINDING_FOR = os.path.join(HERE, "build", "_vla_ops.for")        # see _made_for
 SOURCES = ["csrc/model.cu", "csrc/cache_ops.cu"]
 # headers that only one of the sources includes; the others (common.cuh, host.cuh, the C header) belong to both
 ONLY = {"csrc/cache_ops.cu": {"csrc/attention_paged.cuh", "csrc/attention_prompt.cuh", "csrc/cache_pages.cuh"}}
@@ -32,13 +35,28 @@ def needs_build():
     return _stale(LIB, [os.path.join(HERE, f) for f in SOURCES + HEADERS]) or _binding_stale()
 
 
+def _made_for():
+    """What the binding is linked against: it loads with no other torch or Python."""
+    return "torch %s in %s, %s" % (metadata.version("torch"), _torch_home(), sys.implementation.cache_tag)
+
+
+def _torch_home():
+    return os.path.dirname(find_spec("torch").origin)
+
+
+def _read(path):
+    if not os.path.exists(path):
+        return None
+    with open(path) as f:
+        return f.read()
+
+
 def _binding_stale():
-    return _stale(BINDING, [os.path.join(HERE, f) for f in (BINDING_SRC, "../include/vla_b200.h")])
+    return _stale(BINDING, [os.path.join(HERE, f) for f in (BINDING_SRC, "../include/vla_b200.h")]) or _read(BINDING_FOR) != _made_for()
 
 
 def _binding_command(nvcc):
-    import torch
-    home = os.path.dirname(torch.__file__)
+    home = _torch_home()
     include = [os.path.join(home, "include"), os.path.join(home, "include/torch/csrc/api/include"), sysconfig.get_paths()["include"],
                os.path.join(os.path.dirname(os.path.dirname(nvcc)), "include")]
     libs = ["torch_python", "torch_cpu", "torch", "c10", "c10_cuda", "vla_b200"]
@@ -64,6 +82,8 @@ def build(force=False, verbose=False):
         subprocess.run([nvcc] + flags + ["-shared", "-o", LIB] + [_object(s) for s in SOURCES], cwd=HERE, check=True)
     if force or _binding_stale():
         subprocess.run(_binding_command(nvcc), cwd=HERE, check=True)
+        with open(BINDING_FOR, "w") as f:
+            f.write(_made_for())
     return LIB
 
 

@@ -14,12 +14,15 @@ import _capi
 
 try:
     import _vla_ops as _native          # csrc/binding.cpp
-except ModuleNotFoundError:
+except ImportError as _e:               # not built, or for another torch or Python: the callers through ctypes do without it
     class _NotBuilt:
-        def __getattr__(self, name):
-            raise _capi.VlaError("vla_ops: %s needs the built library (python realtime-vla_b200/build.py); there is no CPU path" % name)
+        def __init__(self, why):
+            self._why = why
 
-    _native = _NotBuilt()
+        def __getattr__(self, name):
+            raise _capi.VlaError("vla_ops: %s needs the built library (python realtime-vla_b200/build.py); there is no CPU path (%s)" % (name, self._why))
+
+    _native = _NotBuilt(str(_e))
 
 
 def _p(t):

@@ -132,3 +132,37 @@ def test_status_refusals():
     assert lib.vla_op_cache_status(None) == STATE and "null" in lib.vla_last_error(None).decode()
     for limit in (0, -1, 1000001):
         assert lib.vla_op_cache_wait_expire(limit, None) == LIMIT and "microseconds" in lib.vla_last_error(None).decode()
+
+
+IMPORTS = """
+import torch, _capi, vla_ops
+assert all(callable(getattr(vla_ops, f)) for f in ("gemm", "attention", "norm", "attention_tc"))
+i = torch.zeros(1, dtype=torch.int32)
+try:
+    vla_ops.block_plan(i, i, i[None], i, block_size=16, total_new=0)
+except _capi.VlaError as e:
+    print("refused:", e)
+"""
+
+
+def test_a_binding_that_does_not_load_leaves_the_rest(tmp_path):
+    """A file of another torch, another Python or half a build: what goes through ctypes alone is still there, and the operators that
+    need the binding say why they are not."""
+    import subprocess
+    import sys
+    (tmp_path / "_vla_ops.so").write_bytes(b"no shared object")
+    package = os.path.dirname(os.path.abspath(vla_ops.__file__))
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join([str(tmp_path), package]))
+    done = subprocess.run([sys.executable, "-c", IMPORTS], env=env, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "refused:" in done.stdout and "_vla_ops.so" in done.stdout, done.stderr[-2000:]
+
+
+def test_the_binding_is_rebuilt_for_another_torch_or_python(monkeypatch):
+    import build
+    made_for = build._made_for()
+    assert made_for and build._made_for() == made_for
+    monkeypatch.setattr(build, "_stale", lambda target, inputs: False)
+    monkeypatch.setattr(build, "_read", lambda path: made_for)
+    assert not build._binding_stale()
+    monkeypatch.setattr(build, "_read", lambda path: made_for.replace("torch", "torch 0 "))
+    assert build._binding_stale()

@@ -1,5 +1,5 @@
 """Build libvla_b200.so in place with nvcc for sm_100a (cross-compiles without a GPU), and _vla_ops.so, the Python binding of the
-operators that take torch tensors, with g++."""
+operators that take torch tensors, with g++ (where torch is installed; --library leaves it out)."""
 import os
 import subprocess
 import sys
@@ -31,8 +31,12 @@ def _stale(target, inputs):
     return not os.path.exists(target) or any(os.path.getmtime(f) > os.path.getmtime(target) for f in inputs)
 
 
-def needs_build():
-    return _stale(LIB, [os.path.join(HERE, f) for f in SOURCES + HEADERS]) or _binding_stale()
+def needs_build(binding=True):
+    return _stale(LIB, [os.path.join(HERE, f) for f in SOURCES + HEADERS]) or binding and _has_torch() and _binding_stale()
+
+
+def _has_torch():
+    return find_spec("torch") is not None
 
 
 def _made_for():
@@ -65,8 +69,9 @@ def _binding_command(nvcc):
             ["-L" + os.path.join(home, "lib"), "-L" + HERE] + ["-l" + x for x in libs] + ["-Wl,-rpath,$ORIGIN"])
 
 
-def build(force=False, verbose=False):
-    if not force and not needs_build():
+def build(force=False, verbose=False, binding=True):
+    """The C library needs nvcc alone; `binding`: the Python binding too, where torch is installed."""
+    if not force and not needs_build(binding):
         return LIB
     nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
     flags = ["-O3", "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-Xcompiler", "-fPIC"]
@@ -80,12 +85,17 @@ def build(force=False, verbose=False):
         raise RuntimeError("nvcc failed on " + ", ".join(failed))
     if force or _stale(LIB, [_object(s) for s in SOURCES]):
         subprocess.run([nvcc] + flags + ["-shared", "-o", LIB] + [_object(s) for s in SOURCES], cwd=HERE, check=True)
-    if force or _binding_stale():
-        subprocess.run(_binding_command(nvcc), cwd=HERE, check=True)
+    if binding and not _has_torch():
+        print("build.py: no torch here, so no _vla_ops.so; libvla_b200.so is complete", file=sys.stderr)
+    elif binding and (force or _binding_stale()):
+        try:
+            subprocess.run(_binding_command(nvcc), cwd=HERE, check=True)
+        except (OSError, subprocess.CalledProcessError) as e:
+            raise RuntimeError("libvla_b200.so is complete, _vla_ops.so could not be built (--library leaves it out): %s" % e) from e
         with open(BINDING_FOR, "w") as f:
             f.write(_made_for())
     return LIB
 
 
 if __name__ == "__main__":
-    print(build(force="--force" in sys.argv, verbose="-v" in sys.argv))
+    print(build(force="--force" in sys.argv, verbose="-v" in sys.argv, binding="--library" not in sys.argv))

@@ -166,3 +166,34 @@ def test_the_binding_is_rebuilt_for_another_torch_or_python(monkeypatch):
     assert not build._binding_stale()
     monkeypatch.setattr(build, "_read", lambda path: made_for.replace("torch", "torch 0 "))
     assert build._binding_stale()
+
+
+def test_building_needs_no_torch_for_the_c_library(monkeypatch, capsys):
+    """Without torch, or when only the C library is asked for, nothing is said to be missing and no binding is tried."""
+    import build
+    ran = []
+    monkeypatch.setattr(build, "_stale", lambda target, inputs: target == build.BINDING)
+    monkeypatch.setattr(build.subprocess, "run", lambda command, **kw: ran.append(command))
+    assert build.needs_build() and not build.needs_build(binding=False)
+    assert build.build(binding=False) == build.LIB and not ran
+    monkeypatch.setattr(build, "find_spec", lambda name: None)
+    assert not build.needs_build()
+    assert build.build() == build.LIB and not ran
+    assert build.build(force=False) == build.LIB
+    monkeypatch.setattr(build, "_stale", lambda target, inputs: True)
+    monkeypatch.setattr(build.subprocess, "Popen", lambda command, **kw: type("Done", (), {"wait": lambda self: 0})())
+    build.build()
+    assert len(ran) == 1 and ran[0][-1].endswith(".o") and "no torch" in capsys.readouterr().err
+
+
+def test_a_binding_that_does_not_compile_names_the_library_that_is_there(monkeypatch):
+    import build
+
+    def run(command, **kw):
+        if command[0] == "g++":
+            raise build.subprocess.CalledProcessError(1, command)
+
+    monkeypatch.setattr(build, "_stale", lambda target, inputs: target == build.BINDING)
+    monkeypatch.setattr(build.subprocess, "run", run)
+    with pytest.raises(RuntimeError, match="libvla_b200.so is complete"):
+        build.build()

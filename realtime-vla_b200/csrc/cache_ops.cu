@@ -61,8 +61,7 @@ constexpr long long INT_TOP = 0x7fffffff;
 template <int N>
 bool tensor_map(CUtensorMap* tm, const void* base, int size, CUtensorMapDataType type, const long long (&dims)[N], const long long (&strides)[N - 1],
                 const int (&box)[N]) {
-  EncodeTiledFn fn = get_encode_fn();
-  if (!fn) return false;
+  EncodeTiledFn fn = get_encode_fn();            // the callers have looked
   cuuint64_t gd[N], gs[N - 1];
   cuuint32_t bx[N], es[N];
   for (int i = 0; i < N; ++i) {
@@ -210,6 +209,7 @@ int vla_op_paged_attention(const vla_paged_attn_desc* d, void* stream) {
       return refuse(VLA_ERR_LIMIT, "%s: more than 2e9 groups of 16 tokens in the table's rows, times key/value heads and blocks of 8 or 16 rows", who);
     if (s.workspace && (!d->workspace || d->workspace_bytes < s.workspace || !aligned(d->workspace, 16)))
       return refuse(VLA_ERR_STATE, "%s: a workspace of %zu bytes on a 16-byte boundary is needed", who, s.workspace);
+    if (!get_encode_fn()) return refuse(VLA_ERR_CUDA, "%s: the CUDA driver that encodes tensor maps is not there", who);
     PagedAttnParams p;
     p.q = d->q; p.o = d->o;
     p.q_seq = d->q_seq_stride; p.q_tok = d->q_tok_stride; p.q_head = d->q_head_stride;
@@ -268,6 +268,7 @@ int vla_op_prompt_attention(const vla_prompt_attn_desc* d, void* stream) {
     if (!vectors(d->q, d->q_tok_stride, d->q_head_stride) || !vectors(d->k, d->k_tok_stride, d->k_head_stride) ||
         !vectors(d->v, d->v_tok_stride, d->v_head_stride) || !vectors(d->o, d->o_tok_stride, d->o_head_stride))
       return refuse(VLA_ERR_SHAPE, "%s: rows of q, k, v and o must start on 16 bytes", who);
+    if (!get_encode_fn()) return refuse(VLA_ERR_CUDA, "%s: the CUDA driver that encodes tensor maps is not there", who);
     PromptAttnParams p;
     p.v = d->v; p.o = d->o; p.cu_q = d->cu_q; p.cu_k = d->cu_k;
     p.n_seqs = d->n_seqs; p.tokens_q = d->tokens_q; p.tokens_k = d->tokens_k;

@@ -197,3 +197,22 @@ def test_a_binding_that_does_not_compile_names_the_library_that_is_there(monkeyp
     monkeypatch.setattr(build.subprocess, "run", run)
     with pytest.raises(RuntimeError, match="libvla_b200.so is complete"):
         build.build()
+
+
+@needs_library
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the addresses are only good where nothing can be launched")
+def test_first_calls_from_several_threads_without_a_driver():
+    """Every one of them says that there is no driver, and none blames the strides."""
+    import threading
+    said = []
+
+    def first():
+        for name, desc in (("vla_op_prompt_attention", prompt_desc()), ("vla_op_paged_attention", paged_desc())):
+            said.append(call(name, desc))
+
+    threads = [threading.Thread(target=first) for _ in range(8)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(said) == 16 and all(rc == 1 and "driver" in text for rc, text in said)

@@ -3,6 +3,7 @@
 // microseconds on the GPU; here the host needs 5 to 9 for each, of which the launch is 3, and through ctypes it needed 11 to 19.
 #include <ATen/ATen.h>
 #include <ATen/core/LegacyTypeDispatch.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -70,12 +71,18 @@ const at::Tensor& whole(PyObject* o, const char* name, c10::Device device, int d
 }
 const int32_t* ints(const at::Tensor& t) { return static_cast<const int32_t*>(t.const_data_ptr()); }
 
+// Neither a gradient nor a tangent of an argument may be lost on the way
+void no_gradient(const at::Tensor& t, const char* name) {
+  if (t.requires_grad() && c10::GradMode::is_enabled()) refuse(name, " requires a gradient; this operator has no backward pass");
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined()) refuse(name, " has a tangent; this operator has no forward-mode gradient");
+}
+
 // A 16-bit tensor of `dim` dimensions on `device` whose last one is contiguous
 const at::Tensor& rows(PyObject* o, const char* name, c10::Device device, at::ScalarType type, int dim) {
   const at::Tensor& t = tensor(o, name);
   if (t.scalar_type() != type || t.dim() != dim || t.device() != device || !rows_contiguous(t))
     refuse(name, " must be ", type, " with ", (int64_t)dim, " dimensions, the last one contiguous, on ", device, "; got ", t);
-  if (t.requires_grad() && c10::GradMode::is_enabled()) refuse(name, " requires a gradient; this operator has no backward pass");
+  no_gradient(t, name);
   return t;
 }
 int type_code(const at::Tensor& t, const char* name) {
@@ -103,6 +110,10 @@ Cache cache_of(PyObject* o, c10::Device device) {
   if (!(part(*c.k, at::kFloat8_e4m3fn, 4) && part(*c.v, at::kFloat8_e4m3fn, 4) && part(*c.ks, at::kFloat, 2) && part(*c.vs, at::kFloat, 2)))
     refuse("a cache is float8_e4m3fn codes [blocks, kv_heads, block_size, head_dim] twice and float32 scales [blocks, kv_heads] twice, "
            "all contiguous and on ", device, "; got ", *c.k, ", ", *c.v, ", ", *c.ks, ", ", *c.vs);
+  no_gradient(*c.k, "cache.k");
+  no_gradient(*c.v, "cache.v");
+  no_gradient(*c.ks, "cache.k_scale");
+  no_gradient(*c.vs, "cache.v_scale");
   return c;
 }
 

@@ -1,0 +1,62 @@
+"""The operators around a key/value cache in pages among torch's own: gradients that they would lose."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def ops():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    import vla_ops
+    return vla_ops
+
+
+def made(ops):
+    g = torch.Generator(device="cuda").manual_seed(61)
+    cache = ops.kv_cache(4, 2, 16, 64)
+    x = torch.randn(20, 2, 64, generator=g, device="cuda").bfloat16()
+    slots = torch.arange(20, dtype=torch.int32, device="cuda")
+    ops.cache_append(x, x, cache, slots)
+    q = torch.randn(1, 1, 8, 64, generator=g, device="cuda").bfloat16()
+    table, lens = torch.arange(4, dtype=torch.int32, device="cuda")[None], torch.full((1,), 20, dtype=torch.int32, device="cuda")
+    return cache, x, slots, q, table, lens
+
+
+def calls(ops, cache, x, slots, q, table, lens):
+    """Each operator with one tensor of its arguments exchanged by f."""
+    cu = torch.tensor([0, 20], dtype=torch.int32, device="cuda")
+    ident = lambda t: t                                                                  # noqa: E731
+    part = lambda name, f: cache._replace(**{name: f(getattr(cache, name))})             # noqa: E731
+    return {
+        "q": lambda f=ident: ops.paged_attention(f(q), cache, table, lens),
+        "k_scale": lambda f=ident: ops.paged_attention(q, part("k_scale", f), table, lens),
+        "v_scale": lambda f=ident: ops.paged_attention(q, part("v_scale", f), table, lens),
+        "append k": lambda f=ident: ops.cache_append(f(x), x, cache, slots),
+        "append v": lambda f=ident: ops.cache_append(x, f(x), cache, slots),
+        "append v_scale": lambda f=ident: ops.cache_append(x, x, part("v_scale", f), slots),
+        "prompt q": lambda f=ident: ops.prompt_attention(f(x), x, x, cu),
+        "prompt k": lambda f=ident: ops.prompt_attention(x, f(x), x, cu),
+        "prompt v": lambda f=ident: ops.prompt_attention(x, x, f(x), cu),
+        "out": lambda f=ident: ops.prompt_attention(x, x, x, cu, out=f(torch.empty_like(x))),
+    }
+
+
+NAMES = ["q", "k_scale", "v_scale", "append k", "append v", "append v_scale", "prompt q", "prompt k", "prompt v", "out"]
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_tangents_and_gradients_are_refused_not_lost(ops, name):
+    import _capi
+    call = calls(ops, *made(ops))[name]
+    call()
+    with fwd.dual_level():
+        with pytest.raises(_capi.VlaError, match="gradient|tangent"):
+            call(lambda t: fwd.make_dual(t, torch.ones_like(t)))
+    grown = lambda t: t.detach().clone().requires_grad_()           # noqa: E731
+    with pytest.raises(_capi.VlaError, match="gradient"):
+        call(grown)
+    with torch.no_grad():
+        call(grown)                                                  # nobody asks for one

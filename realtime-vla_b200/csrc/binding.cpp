@@ -76,6 +76,10 @@ void no_gradient(const at::Tensor& t, const char* name) {
   if (t.requires_grad() && c10::GradMode::is_enabled()) refuse(name, " requires a gradient; this operator has no backward pass");
   if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined()) refuse(name, " has a tangent; this operator has no forward-mode gradient");
 }
+// What an operator has written: autograd's saved copies of it are out of date.  Tensors of inference mode keep no count.
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 
 // A 16-bit tensor of `dim` dimensions on `device` whose last one is contiguous
 const at::Tensor& rows(PyObject* o, const char* name, c10::Device device, at::ScalarType type, int dim) {
@@ -166,6 +170,7 @@ PyObject* block_plan(PyObject* const* a) {      // context_lens, new_lens, block
   int32_t* const base = static_cast<int32_t*>(out.data_ptr());
   d.slots = base; d.positions = base + start[1]; d.cu_new = base + start[2]; d.seq_lens = base + start[3]; d.counts = base + start[4];
   enqueue(vla_op_block_plan, d, dev);
+  written(table);
   const at::AutoDispatchBelowADInplaceOrView plain;     // integers: views that autograd need not know of
   THPObjectPtr result(PyTuple_New(5));
   if (!result) throw Raised{};
@@ -195,6 +200,7 @@ PyObject* cache_append(PyObject* const* a) {    // k, v, cache, slots
   d.num_blocks = number(c.k->size(0), "cache"); d.kv_heads = number(c.k->size(1), "cache");
   d.block_size = number(c.k->size(2), "cache"); d.head_dim = number(c.k->size(3), "cache");
   enqueue(vla_op_cache_append, d, dev);
+  for (const at::Tensor* t : {c.k, c.v, c.ks, c.vs}) written(*t);
   Py_RETURN_NONE;
 }
 
@@ -231,6 +237,7 @@ PyObject* paged_attention(PyObject* const* a) { // q, cache, block_table, seq_le
     }
   }
   enqueue(vla_op_paged_attention, d, dev);      // refuses what the size was refused for, too
+  if (a[5] != Py_None) written(out);
   return THPVariable_Wrap(out);
 }
 
@@ -257,6 +264,7 @@ PyObject* prompt_attention(PyObject* const* a) {        // q, k, v, cu_q, cu_k, 
   d.v_tok_stride = v.stride(0); d.v_head_stride = v.stride(1); d.o_tok_stride = out.stride(0); d.o_head_stride = out.stride(1);
   d.causal = causal; d.scale = scale_of(a[6], q.size(2));
   enqueue(vla_op_prompt_attention, d, dev);
+  if (a[7] != Py_None) written(out);
   return THPVariable_Wrap(out);
 }
 

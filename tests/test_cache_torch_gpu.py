@@ -1,4 +1,4 @@
-"""The operators around a key/value cache in pages among torch's own: gradients that they would lose."""
+"""The operators around a key/value cache in pages among torch's own: gradients that they would lose, and tensors that they change."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
@@ -60,3 +60,41 @@ def test_tangents_and_gradients_are_refused_not_lost(ops, name):
         call(grown)
     with torch.no_grad():
         call(grown)                                                  # nobody asks for one
+
+
+def test_what_is_written_has_a_new_version(ops):
+    cache, x, slots, q, table, lens = made(ops)
+    before = [t._version for t in cache]
+    ops.cache_append(x, x, cache, slots)
+    assert all(t._version > b for t, b in zip(cache, before))
+    before = [t._version for t in (*cache, q, table, lens, x)]
+    out = torch.empty_like(q)
+    version = out._version
+    ops.paged_attention(q, cache, table, lens, out=out)
+    assert out._version > version and [t._version for t in (*cache, q, table, lens, x)] == before
+    wide = torch.empty(20, 2, 2, 64, dtype=torch.bfloat16, device="cuda")
+    version = wide._version
+    ops.prompt_attention(x, x, x, torch.tensor([0, 20], dtype=torch.int32, device="cuda"), out=wide[:, 1])
+    assert wide._version > version                                   # a view's base as well
+    version = table._version
+    ops.block_plan(lens, torch.ones_like(lens), table, torch.zeros(1, dtype=torch.int32, device="cuda"), block_size=16, total_new=1)
+    assert table._version > version
+
+
+def test_a_backward_pass_over_changed_scales_is_refused_by_torch(ops):
+    cache, x, slots, *_ = made(ops)
+    w = torch.ones_like(cache.v_scale).requires_grad_()
+    loss = (w * cache.v_scale).sum()                                 # keeps v_scale
+    ops.cache_append(x * 64, x * 64, cache, slots)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+def test_tensors_of_inference_mode_may_be_written_anywhere(ops):
+    with torch.inference_mode():
+        cache, x, slots, q, table, lens = made(ops)
+        out = torch.empty_like(q)
+        want = ops.paged_attention(q, cache, table, lens).clone()
+    ops.cache_append(x, x, cache, slots)
+    ops.paged_attention(q, cache, table, lens, out=out)
+    assert torch.equal(out, want)

@@ -2,6 +2,7 @@
 // All of them only enqueue work on the caller's stream: no allocation, no synchronisation, nothing kept between calls, so
 // they can be captured into a graph and called from several threads and streams at once.
 #include <algorithm>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <mutex>
@@ -98,7 +99,7 @@ PagedShape paged_shape(const vla_paged_attn_desc* d) {
   return s;
 }
 
-// Sizes and types of a vla_paged_attn_desc
+// Sizes and types of a vla_paged_attn_desc; what passes keeps paged_shape within 64 bits
 int paged_check(const char* who, const vla_paged_attn_desc* d) {
   if (!d) return refuse(VLA_ERR_STATE, "%s: null descriptor", who);
   if (d->n_seqs < 0 || d->n_q < 1 || d->heads < 1 || d->kv_heads < 1 || d->num_blocks < 1 || d->width < 0 || d->table_stride < d->width)
@@ -110,6 +111,10 @@ int paged_check(const char* who, const vla_paged_attn_desc* d) {
     return refuse(VLA_ERR_LIMIT, "%s: more than 2^31 - 17 tokens, or 2^20 rows of a sequence", who);
   if (d->dtype != VLA_BF16 && d->dtype != VLA_F16) return refuse(VLA_ERR_SHAPE, "%s: q must be bf16 or f16", who);
   if (!(d->scale > 0.f) || d->scale > 3e38f) return refuse(VLA_ERR_SHAPE, "%s: scale must be positive and finite", who);
+  // in floating point, because the products may leave 64 bits
+  const double rows = (double)d->n_q * (d->heads / d->kv_heads), row_blocks = std::ceil(rows / (rows > 8 ? 16 : 8));
+  if ((double)d->n_seqs * d->kv_heads * row_blocks * ((double)d->width * d->block_size / 16 + paged_gap(d->head_dim)) > 2e9)
+    return refuse(VLA_ERR_LIMIT, "%s: more than 2e9 groups of 16 tokens in the table's rows, times key/value heads and blocks of 8 or 16 rows", who);
   return VLA_OK;
 }
 
@@ -205,8 +210,6 @@ int vla_op_paged_attention(const vla_paged_attn_desc* d, void* stream) {
     if (!vectors(d->q, d->q_seq_stride, d->q_tok_stride) || d->q_head_stride % 8 || !vectors(d->o, d->o_seq_stride, d->o_tok_stride) || d->o_head_stride % 8)
       return refuse(VLA_ERR_SHAPE, "%s: rows of q and o must start on 16 bytes", who);
     const PagedShape s = paged_shape(d);
-    if ((double)d->n_seqs * d->kv_heads * s.row_blocks * ((double)d->width * d->block_size / 16 + paged_gap(d->head_dim)) > 2e9)
-      return refuse(VLA_ERR_LIMIT, "%s: more than 2e9 groups of 16 tokens in the table's rows, times key/value heads and blocks of 8 or 16 rows", who);
     if (s.workspace && (!d->workspace || d->workspace_bytes < s.workspace || !aligned(d->workspace, 16)))
       return refuse(VLA_ERR_STATE, "%s: a workspace of %zu bytes on a 16-byte boundary is needed", who, s.workspace);
     if (!get_encode_fn()) return refuse(VLA_ERR_CUDA, "%s: the CUDA driver that encodes tensor maps is not there", who);

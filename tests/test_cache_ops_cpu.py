@@ -216,3 +216,15 @@ def test_first_calls_from_several_threads_without_a_driver():
     for t in threads:
         t.join()
     assert len(said) == 16 and all(rc == 1 and "driver" in text for rc, text in said)
+
+
+@needs_library
+@pytest.mark.parametrize("change", [dict(n_seqs=2 ** 31 - 1, n_q=1, heads=2 ** 20, kv_heads=2 ** 20, width=2 ** 20, table_stride=2 ** 20),
+                                    dict(n_seqs=2 ** 31 - 1, n_q=2 ** 13, heads=2 ** 7, kv_heads=2 ** 7, width=2 ** 26, table_stride=2 ** 26),
+                                    dict(n_seqs=2 ** 30, heads=8, kv_heads=8, width=2 ** 26, table_stride=2 ** 26)])
+def test_sizes_whose_products_leave_64_bits(change):
+    """Refused by the question for the workspace as by the call, before any product is formed."""
+    need = C.c_size_t(77)
+    desc = paged_desc(**change)
+    assert _capi.lib().vla_op_paged_attention_workspace(C.byref(desc), C.byref(need)) == LIMIT and need.value == 77
+    assert call("vla_op_paged_attention", desc)[0] == LIMIT

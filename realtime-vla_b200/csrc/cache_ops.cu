@@ -30,7 +30,9 @@ int refuse(int code, const char* fmt, ...) {
 }
 
 int launched(const char* who, cudaError_t e) {
-  return e == cudaSuccess ? VLA_OK : refuse(VLA_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
+  if (e == cudaSuccess) return VLA_OK;
+  (void)cudaGetLastError();            // it has been told; the library's next call must not find it
+  return refuse(VLA_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
 }
 
 // No C++ exception leaves a C entry point.

@@ -56,3 +56,39 @@ def test_replayed_waits_are_seen(ops):
     for _ in range(2):
         graph.replay()
         assert ops.cache_status() == 1
+
+
+REFUSED_LAUNCH = """
+import torch, _capi, vla_ops
+x, slots = torch.ones(4, 1, 64, device="cuda").bfloat16(), torch.arange(4, dtype=torch.int32, device="cuda")
+cache = vla_ops.kv_cache(1, 1, 16, 64)
+torch.cuda.synchronize()
+refused = False
+try:
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        try:
+            torch.cuda.synchronize()                 # ends the capture
+        except RuntimeError:
+            pass
+        try:
+            vla_ops.cache_append(x, x, cache, slots)
+        except _capi.VlaError:
+            refused = True
+except RuntimeError:
+    pass
+assert refused
+assert vla_ops.cache_status() == 0
+vla_ops.cache_append(x, x, cache, slots)
+assert cache.k[0, 0, :4].float().abs().min() > 0
+print("works")
+"""
+
+
+def test_a_launch_that_is_refused_leaves_no_error_behind(ops):
+    """A launch into a capture that has become invalid is refused; the library's next call does not find that error."""
+    import os
+    import subprocess
+    import sys
+    env = dict(os.environ, PYTHONPATH=os.path.dirname(os.path.abspath(ops.__file__)))
+    done = subprocess.run([sys.executable, "-c", REFUSED_LAUNCH], env=env, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "works" in done.stdout, done.stderr[-2000:]

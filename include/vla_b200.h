@@ -347,7 +347,7 @@ int vla_op_paged_attention(const vla_paged_attn_desc* d, void* stream);
 /* O = softmax(scale Q K^T) V over packed prompts: q, o [tokens_q][heads][head_dim], k, v [tokens_k][kv_heads][head_dim] by
  * strides; sequence b owns rows cu_q[b] .. cu_q[b + 1] and cu_k[b] .. cu_k[b + 1] (device memory, ascending).  With causal set, the
  * last query of a sequence sees all its keys, the one before it all but the last, and so on; a row that sees nothing is
- * zero.  Rows of o behind the last sequence are left as they were.  head_dim a multiple of 8 up to 256,
+ * zero.  Rows of o behind the last sequence are left as they were.  o may be q; it overlaps nothing else.  head_dim a multiple of 8 up to 256,
  * heads / kv_heads <= 128. */
 typedef struct vla_prompt_attn_desc {
   const void* q; const void* k; const void* v; void* o;

@@ -132,13 +132,46 @@ void enqueue(int (*fn)(const Desc*, void*), const Desc& d, c10::Device device) {
   }
 }
 
-// out, or a new tensor like q
+// Whether two tensors have an element in common, of which nothing is known only where their layouts do not fit each other.
+bool apart(const at::Tensor& a, const at::Tensor& b) {
+  if (!a.numel() || !b.numel()) return true;
+  // bytes from the first element to behind the last one, of the dimensions whose stride is below `s` bytes
+  auto extent = [](const at::Tensor& t, int64_t s) {
+    int64_t n = t.element_size();
+    for (int64_t i = 0; i < t.dim(); ++i)
+      if (t.size(i) > 1 && t.stride(i) * (int64_t)t.element_size() < s) n += (t.size(i) - 1) * t.stride(i) * t.element_size();
+    return n;
+  };
+  const int64_t at_a = (int64_t)a.const_data_ptr(), at_b = (int64_t)b.const_data_ptr();
+  if (at_a + extent(a, INT64_MAX) <= at_b || at_b + extent(b, INT64_MAX) <= at_a) return true;
+  // parts of rows of s bytes: slices of one buffer
+  for (int64_t i = 0; i < a.dim(); ++i) {
+    const int64_t s = a.stride(i) * a.element_size();
+    if (a.size(i) < 2 || s <= 0) continue;
+    bool rows = true;
+    for (const at::Tensor* t : {&a, &b})
+      for (int64_t k = 0; k < t->dim(); ++k)
+        if (t->size(k) > 1 && t->stride(k) * (int64_t)t->element_size() >= s && t->stride(k) * (int64_t)t->element_size() % s) rows = false;
+    const int64_t from = ((at_b - at_a) % s + s) % s;
+    if (rows && extent(a, s) <= from && from + extent(b, s) <= s) return true;
+  }
+  return false;
+}
+bool same_place(const at::Tensor& a, const at::Tensor& b) {
+  if (a.const_data_ptr() != b.const_data_ptr()) return false;
+  for (int64_t i = 0; i < a.dim(); ++i)
+    if (a.size(i) > 1 && a.stride(i) != b.stride(i)) return false;
+  return true;
+}
+
+// out, or a new tensor like q.  It may be q itself: a row of q has been read by all that read it when it is written.
 at::Tensor output(PyObject* o, const at::Tensor& q) {
   if (o == Py_None) return at::empty(q.sizes(), q.options());
   const at::Tensor& t = rows(o, "out", q.device(), q.scalar_type(), (int)q.dim());
   if (t.sizes() != q.sizes()) refuse("out must have the shape of q");
   for (int64_t i = 0; i < t.dim(); ++i)
     if (t.stride(i) == 0 && t.size(i) > 1) refuse("out is expanded: several of its elements are one place in memory");
+  if (!same_place(t, q) && !apart(t, q)) refuse("out overlaps q without being q");
   return t;
 }
 
@@ -256,6 +289,8 @@ PyObject* prompt_attention(PyObject* const* a) {        // q, k, v, cu_q, cu_k, 
   const int causal = PyObject_IsTrue(a[5]);
   if (causal < 0) throw Raised{};
   const at::Tensor out = output(a[7], q);
+  if (a[7] != Py_None && !apart(out, k)) refuse("out overlaps k");
+  if (a[7] != Py_None && !apart(out, v)) refuse("out overlaps v");
   d.q = q.const_data_ptr(); d.k = k.const_data_ptr(); d.v = v.const_data_ptr(); d.o = out.data_ptr();
   d.cu_q = ints(cu_q); d.cu_k = ints(cu_k);
   d.n_seqs = number(cu_q.size(0) - 1, "cu_q"); d.tokens_q = number(q.size(0), "q"); d.tokens_k = number(k.size(0), "k");

@@ -177,7 +177,7 @@ def paged_attention(q, cache, block_table, seq_lens, *, scale=None, out=None):
 
     q bf16 or fp16 [n, tokens, heads, head_dim]: the last tokens of each sequence, whose keys are in the cache already;
     each sees itself and what is before it.  block_table int32 [n, width], seq_lens int32 [n].  scale: head_dim ** -0.5
-    unless given.  Returns out, or a new tensor like q; a row that sees nothing is zero."""
+    unless given.  Returns out (which may be q), or a new tensor like q; a row that sees nothing is zero."""
     return _native.paged_attention(q, cache, block_table, seq_lens, scale, out)
 
 
@@ -186,8 +186,8 @@ def prompt_attention(q, k, v, cu_q, cu_k=None, *, causal=True, scale=None, out=N
 
     q bf16 or fp16 [tokens, heads, head_dim], k and v [keys, kv_heads, head_dim]; sequence b owns rows cu_q[b] .. cu_q[b + 1] of
     q and cu_k[b] .. cu_k[b + 1] of k and v (int32 [n + 1] on the device, ascending; cu_k: as cu_q unless given).  causal: the last row
-    of a sequence sees all its keys, each row before it one less; otherwise every row sees all.  Returns out, or a new
-    tensor like q; a row that sees nothing is zero, rows behind the last sequence are not written."""
+    of a sequence sees all its keys, each row before it one less; otherwise every row sees all.  Returns out (which may be q
+    but must not overlap k or v), or a new tensor like q; a row that sees nothing is zero, rows behind the last sequence are not written."""
     return _native.prompt_attention(q, k, v, cu_q, cu_k, causal, scale, out)
 
 

@@ -98,3 +98,40 @@ def test_tensors_of_inference_mode_may_be_written_anywhere(ops):
     ops.cache_append(x, x, cache, slots)
     ops.paged_attention(q, cache, table, lens, out=out)
     assert torch.equal(out, want)
+
+
+def test_out_may_be_q_and_nothing_else_that_is_read(ops):
+    """Written over q an output is what it is elsewhere; over k or v, or across q, it is refused: other rows still read those."""
+    import _capi
+    g = torch.Generator(device="cuda").manual_seed(62)
+    q, k, v = (torch.randn(700, 4, 128, generator=g, device="cuda").bfloat16() for _ in range(3))
+    cu = torch.tensor([0, 300, 301, 700], dtype=torch.int32, device="cuda")
+    want = ops.prompt_attention(q, k, v, cu)
+    for out in (k, v, k.view(-1).view(700, 4, 128)):
+        with pytest.raises(_capi.VlaError, match="overlap"):
+            ops.prompt_attention(q, k, v, cu, out=out)
+    wide = torch.empty(701, 4, 128, device="cuda", dtype=torch.bfloat16)
+    wide[:700] = q
+    with pytest.raises(_capi.VlaError, match="overlap"):
+        ops.prompt_attention(wide[:700], k, v, cu, out=wide[1:])
+    fused = torch.cat([q, k, v], 1)                      # [700, 12, 128]: one projection's output, written over its own q
+    fq, fk, fv = fused[:, :4], fused[:, 4:8], fused[:, 8:]
+    for out in (fk, fv, fused[:, 2:6], fused[:, 7:11]):
+        with pytest.raises(_capi.VlaError, match="overlap"):
+            ops.prompt_attention(fq, fk, fv, cu, out=out)
+    assert torch.equal(ops.prompt_attention(fq, fk, fv, cu, out=fq), want) and torch.equal(fk, k) and torch.equal(fv, v)
+    got = q.clone()
+    assert torch.equal(ops.prompt_attention(got, k, v, cu, out=got), want)
+    # attention over a cache: units that are cut between CTAs read q several times
+    cache = ops.kv_cache(600, 2, 16, 128)
+    x = torch.randn(9000, 2, 128, generator=g, device="cuda").bfloat16()
+    ops.cache_append(x, x, cache, torch.arange(9000, dtype=torch.int32, device="cuda"))
+    table = torch.arange(600, dtype=torch.int32, device="cuda")[None].expand(3, -1).contiguous()
+    lens = torch.tensor([9000, 40, 0], dtype=torch.int32, device="cuda")
+    q = torch.randn(3, 3, 8, 128, generator=g, device="cuda").bfloat16()
+    want = ops.paged_attention(q, cache, table, lens)
+    got = q.clone()
+    assert torch.equal(ops.paged_attention(got, cache, table, lens, out=got), want)
+    wide = torch.zeros(4, 3, 8, 128, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(_capi.VlaError, match="overlap"):
+        ops.paged_attention(wide[:3], cache, table, lens, out=wide[1:])

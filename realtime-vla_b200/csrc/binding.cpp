@@ -60,6 +60,8 @@ float scale_of(PyObject* o, int64_t dim) {
   if (x == -1.0 && PyErr_Occurred()) throw Raised{};
   return (float)x;
 }
+// the stride of a dimension of one element, which may be anything, is never used
+int64_t step(const at::Tensor& t, int64_t i) { return t.size(i) > 1 ? t.stride(i) : 0; }
 bool rows_contiguous(const at::Tensor& t) { return t.stride(-1) == 1 || t.size(-1) <= 1; }
 
 // An int32 tensor of `dim` dimensions on `device` with contiguous rows
@@ -227,7 +229,7 @@ PyObject* cache_append(PyObject* const* a) {    // k, v, cache, slots
   if (k.sizes() != v.sizes() || k.size(1) != c.k->size(1) || k.size(2) != c.k->size(3) || slots.size(0) != k.size(0))
     refuse("k ", k.sizes(), ", v ", v.sizes(), " and slots ", slots.sizes(), " do not fit the cache ", c.k->sizes());
   d.k = k.const_data_ptr(); d.v = v.const_data_ptr(); d.slots = ints(slots); d.tokens = number(k.size(0), "k");
-  d.k_tok_stride = k.stride(0); d.k_head_stride = k.stride(1); d.v_tok_stride = v.stride(0); d.v_head_stride = v.stride(1);
+  d.k_tok_stride = step(k, 0); d.k_head_stride = step(k, 1); d.v_tok_stride = step(v, 0); d.v_head_stride = step(v, 1);
   d.k_codes = c.k->data_ptr(); d.v_codes = c.v->data_ptr();
   d.k_scale = static_cast<float*>(c.ks->data_ptr()); d.v_scale = static_cast<float*>(c.vs->data_ptr());
   d.num_blocks = number(c.k->size(0), "cache"); d.kv_heads = number(c.k->size(1), "cache");
@@ -250,8 +252,8 @@ PyObject* paged_attention(PyObject* const* a) { // q, cache, block_table, seq_le
     refuse("q ", q.sizes(), ", block_table ", table.sizes(), ", seq_lens ", lens.sizes(), " and cache ", c.k->sizes(), " do not fit each other");
   const at::Tensor out = output(a[5], q);
   d.q = q.const_data_ptr(); d.o = out.data_ptr();
-  d.q_seq_stride = q.stride(0); d.q_tok_stride = q.stride(1); d.q_head_stride = q.stride(2);
-  d.o_seq_stride = out.stride(0); d.o_tok_stride = out.stride(1); d.o_head_stride = out.stride(2);
+  d.q_seq_stride = step(q, 0); d.q_tok_stride = step(q, 1); d.q_head_stride = step(q, 2);
+  d.o_seq_stride = step(out, 0); d.o_tok_stride = step(out, 1); d.o_head_stride = step(out, 2);
   d.k_codes = c.k->const_data_ptr(); d.v_codes = c.v->const_data_ptr();
   d.k_scale = static_cast<const float*>(c.ks->const_data_ptr()); d.v_scale = static_cast<const float*>(c.vs->const_data_ptr());
   d.block_table = ints(table); d.width = number(table.size(1), "block_table"); d.table_stride = q.size(0) > 1 ? table.stride(0) : table.size(1);
@@ -295,8 +297,8 @@ PyObject* prompt_attention(PyObject* const* a) {        // q, k, v, cu_q, cu_k, 
   d.cu_q = ints(cu_q); d.cu_k = ints(cu_k);
   d.n_seqs = number(cu_q.size(0) - 1, "cu_q"); d.tokens_q = number(q.size(0), "q"); d.tokens_k = number(k.size(0), "k");
   d.heads = number(q.size(1), "q"); d.kv_heads = number(k.size(1), "k"); d.head_dim = number(q.size(2), "q");
-  d.q_tok_stride = q.stride(0); d.q_head_stride = q.stride(1); d.k_tok_stride = k.stride(0); d.k_head_stride = k.stride(1);
-  d.v_tok_stride = v.stride(0); d.v_head_stride = v.stride(1); d.o_tok_stride = out.stride(0); d.o_head_stride = out.stride(1);
+  d.q_tok_stride = step(q, 0); d.q_head_stride = step(q, 1); d.k_tok_stride = step(k, 0); d.k_head_stride = step(k, 1);
+  d.v_tok_stride = step(v, 0); d.v_head_stride = step(v, 1); d.o_tok_stride = step(out, 0); d.o_head_stride = step(out, 1);
   d.causal = causal; d.scale = scale_of(a[6], q.size(2));
   enqueue(vla_op_prompt_attention, d, dev);
   if (a[7] != Py_None) written(out);

@@ -135,3 +135,23 @@ def test_out_may_be_q_and_nothing_else_that_is_read(ops):
     wide = torch.zeros(4, 3, 8, 128, device="cuda", dtype=torch.bfloat16)
     with pytest.raises(_capi.VlaError, match="overlap"):
         ops.paged_attention(wide[:3], cache, table, lens, out=wide[1:])
+
+
+def test_strides_of_dimensions_of_one_do_not_matter(ops):
+    """A single token, sequence or head out of a tensor of odd width: nothing is ever that stride away from it."""
+    cache, x, slots, q, table, lens = made(ops)
+    cu = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    odd = lambda t: torch.cat([t.flatten(), t.new_zeros(3)]).as_strided(t.shape, [1003 if n == 1 else s for n, s in zip(t.shape, t.stride())])   # noqa: E731
+    one = x[:1].contiguous()
+    assert odd(one).stride(0) == 1003 and torch.equal(odd(one), one)
+    want = ops.prompt_attention(one, one, one, cu)
+    assert torch.equal(ops.prompt_attention(odd(one), odd(one), odd(one), cu, out=odd(torch.empty_like(one))), want)
+    single = x[:20, :1].contiguous()
+    cu20 = torch.tensor([0, 20], dtype=torch.int32, device="cuda")
+    assert torch.equal(ops.prompt_attention(odd(single), odd(single), odd(single), cu20), ops.prompt_attention(single, single, single, cu20))
+    want = ops.paged_attention(q, cache, table, lens)
+    assert torch.equal(ops.paged_attention(odd(q), cache, table, lens, out=odd(torch.empty_like(q))), want)
+    a, b = ops.kv_cache(4, 2, 16, 64), ops.kv_cache(4, 2, 16, 64)
+    ops.cache_append(one, one, a, slots[:1])
+    ops.cache_append(odd(one), odd(one), b, slots[:1])
+    assert all(torch.equal(s.float(), t.float()) for s, t in zip(a, b))

@@ -3,7 +3,8 @@
 With p_j the probabilities, v_j = code_j * scale_j the values that a row sees and A = sum_j p_j |v_j|:
   * a probability is held in three e4m3 pieces of 4 bits each, so it is off by at most 2^-12 of itself;
   * the last piece ends at 2^-18 (and what is smaller is off by itself at most) where the largest is at least 2^7, and the scales
-    of the values that are summed up with one reference differ by 2^7 at most: sum_j min(p_j, 2^-18 max p) |v_j|;
+    of the values that are summed up with one reference differ by 2^7 at most: sum_j min(p_j, 2^-18 max p) |v_j|, and 2^-25 where all
+    scales are one;
   * fp32 scores are off by at most ds_j = (dim + 8) 2^-24 scale sum|q||k|, which moves a probability by that relatively: the
     numerator by sum_j p_j ds_j |v_j|, the denominator by sum_j p_j ds_j of itself;
   * exponentials are off by 2^-22 of themselves, a product with the scale by 2^-24: 2^-20 * A for those above and below;
@@ -29,7 +30,7 @@ def values(codes, scale, ids):
     return x.transpose(1, 2).reshape(-1, codes.shape[1], codes.shape[3])
 
 
-def attend(q, k, v, vis, scale):
+def attend(q, k, v, vis, scale, end):
     """q [n, heads, dim], k, v [m, kv, dim] in 64 bits, vis [n, m] -> (o, bound)."""
     n, heads, dim = q.shape
     m, kv = k.shape[:2]
@@ -44,12 +45,12 @@ def attend(q, k, v, vis, scale):
     weigh = lambda w, x: torch.einsum("hgnm,mhd->nhgd", w, x)      # noqa: E731
     o, a = weigh(p, v), weigh(p, v.abs())
     t = q.dtype
-    bound = a * (2.0 ** -12 + 2.0 ** -20 + (m / 32 + 40) * 2.0 ** -23) + weigh(torch.minimum(p, 2.0 ** -18 * p.amax(-1, keepdim=True)), v.abs())
+    bound = a * (2.0 ** -12 + 2.0 ** -20 + (m / 32 + 40) * 2.0 ** -23) + weigh(torch.minimum(p, end * p.amax(-1, keepdim=True)), v.abs())
     bound += weigh(p * ds, v.abs()) + a * (p * ds).sum(-1).permute(2, 0, 1)[..., None] + torch.finfo(t).eps / 2 * o.abs()
     return o.reshape(n, heads, dim), (bound + (2.0 ** -25 if t == torch.float16 else 0.0)).reshape(n, heads, dim)
 
 
-def check(q, cache, table, lens, out, scale=None):
+def check(q, cache, table, lens, out, scale=None, end=2.0 ** -18):
     scale = q.shape[3] ** -0.5 if scale is None else scale
     block, n = cache.k.shape[2], q.shape[1]
     worst = 0.0
@@ -60,7 +61,7 @@ def check(q, cache, table, lens, out, scale=None):
         ids = table[b, :(m + block - 1) // block].long()
         k, v = values(cache.k, cache.k_scale, ids)[:m], values(cache.v, cache.v_scale, ids)[:m]
         vis = torch.arange(m, device=q.device)[None] <= m - n + torch.arange(n, device=q.device)[:, None]
-        want, bound = attend(q[b], k, v, vis, scale)
+        want, bound = attend(q[b], k, v, vis, scale, end)
         got = out[b].double()
         assert torch.isfinite(got).all()
         off = (got - want).abs()
@@ -196,3 +197,118 @@ def test_not_a_number_in_a_far_scale():
         got = vla_ops.paged_attention(q, c, table, n)
         assert not torch.isfinite(got[1].double()).any()
         check(q[:1], c, table[:1], n[:1], got[:1])
+
+
+# ---- every token once -------------------------------------------------------------------------------------------------------
+
+def one_hot(cache, table, lens):
+    """V of a token is one number, in the head dim that its tile of 128 has: a result is the probability of each tile."""
+    blocks, kv, block, dim = cache.v.shape
+    raw(cache.v)[:] = 0
+    for b, m in enumerate(lens.tolist()):
+        t = torch.arange(m, device=table.device)
+        page = table[b, t // block].long()
+        raw(cache.v)[page[:, None], torch.arange(kv, device=page.device)[None], (t % block)[:, None], (t // 128 % dim)[:, None]] = 0x38     # 1
+    cache.v_scale.fill_(2.0 ** -3)
+
+
+@pytest.mark.parametrize("lens", [(20000,), (9000, 131, 4097, 1, 12800), (300, 513, 129, 0, 1025, 511, 512)])
+@pytest.mark.parametrize("heads,kv,dim,queries", LAYOUTS + [(16, 16, 64, 1), (28, 4, 128, 8)])
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float16])
+def test_every_tile_counts_once(lens, heads, kv, dim, queries, t):
+    """A tile that a piece's border loses, or that two pieces take, shows in its own head dim (or in one it shares with few others)."""
+    import vla_ops
+    q, cache, table, n = pages(57, lens, queries, heads, kv, dim, 16, t)
+    one_hot(cache, table, n)
+    check(q, cache, table, n, vla_ops.paged_attention(q, cache, table, n), end=2.0 ** -25)
+
+
+@pytest.mark.parametrize("heads,kv,dim,queries,t", [(8, 1, 256, 1, torch.bfloat16), (8, 1, 256, 3, torch.float16), (8, 2, 128, 1, torch.float16)])
+def test_every_tile_counts_once_in_long_contexts(heads, kv, dim, queries, t):
+    import vla_ops
+    q, cache, table, n = pages(58, (131071, 90001), queries, heads, kv, dim, 64, t)
+    one_hot(cache, table, n)
+    check(q, cache, table, n, vla_ops.paged_attention(q, cache, table, n), end=2.0 ** -25)
+
+
+@pytest.mark.parametrize("ahead", [10, 17, 22])
+def test_many_faint_tokens_beside_a_loud_one(ahead):
+    """One key stands 2^ahead above the largest of 60000 others, which together still count."""
+    import vla_ops
+    q, cache, table, n = pages(59, (60000,), 1, 8, 1, 128, 16, torch.float16)
+    far(q, cache, 60.0)
+    one_hot(cache, table, n)
+    page = int(table[0, 1000])
+    raw(cache.k)[page, 0, 3] = raw(torch.zeros(1, device=q.device).to(F8))
+    raw(cache.k)[page, 0, 3, 0] = raw(torch.tensor([(ahead + 4) * 16.733], device=q.device).to(F8))      # as above, the other way
+    check(q, cache, table, n, vla_ops.paged_attention(q, cache, table, n), end=2.0 ** -25)
+
+
+@pytest.mark.parametrize("block", [16, 32, 48, 64, 80, 96, 112, 128, 144, 176, 192, 208, 240, 256])
+@pytest.mark.parametrize("heads,kv,dim,queries", [(8, 1, 256, 1), (8, 2, 128, 3), (16, 4, 64, 5)])
+def test_pages_of_every_size(block, heads, kv, dim, queries):
+    """Pages that end inside a tile and boxes of 16, 32, 64 and 128 rows."""
+    import vla_ops
+    lens = (block - 1, block, block + 1, 3 * block + 5, 2000)
+    q, cache, table, n = pages(60, lens, queries, heads, kv, dim, block, torch.bfloat16, 3)
+    check(q, cache, table, n, vla_ops.paged_attention(q, cache, table, n))
+    one_hot(cache, table, n)
+    check(q, cache, table, n, vla_ops.paged_attention(q, cache, table, n), end=2.0 ** -25)
+
+
+# ---- refusals ---------------------------------------------------------------------------------------------------------------
+
+def test_each_refusal_says_why():
+    """Every call with one thing wrong, and the words for it."""
+    import _capi
+    import vla_ops
+    q, cache, table, n = pages(61, (20, 30), 1, 8, 2, 128, 16, torch.bfloat16)
+    x = q[:, 0]
+    k = torch.zeros(2, 2, 128, dtype=torch.bfloat16, device=q.device)
+    slots, cu = torch.arange(2, dtype=torch.int32, device=q.device), torch.tensor([0, 1, 2], dtype=torch.int32, device=q.device)
+    odd = torch.zeros(2 * 8 * 128 + 1, dtype=torch.bfloat16, device=q.device)[1:].view(2, 1, 8, 128)
+    paged, prompt, append, plan = vla_ops.paged_attention, vla_ops.prompt_attention, vla_ops.cache_append, vla_ops.block_plan
+    paged(q, cache, table, n)
+    prompt(x, k, k, cu)
+    append(k, k, cache, slots)
+    plan(n, n, table.clone(), n, block_size=16, total_new=50)
+    for words, call in [
+            ("bfloat16 or float16", lambda: paged(q.float(), cache, table, n)),
+            ("multiple of kv_heads", lambda: paged(q[:, :, :7], cache, table, n)),
+            ("do not fit", lambda: paged(q[..., :64], cache, table, n)),
+            ("last one contiguous", lambda: paged(q.transpose(2, 3), cache, table, n)),
+            ("block_table must be int32", lambda: paged(q, cache, table.long(), n)),
+            ("do not fit", lambda: paged(q, cache, table, n[:1])),
+            ("seq_lens must be int32", lambda: paged(q, cache, table, n.cpu())),
+            ("scale must be", lambda: paged(q, cache, table, n, scale=-1.0)),
+            ("scale must be", lambda: paged(q, cache, table, n, scale=float("nan"))),
+            ("a cache is", lambda: paged(q, cache._replace(k=cache.k.float()), table, n)),
+            ("a cache is", lambda: paged(q, cache._replace(v_scale=cache.v_scale[:, :1]), table, n)),
+            ("cache must be", lambda: paged(q, list(cache), table, n)),
+            ("out must be", lambda: paged(q, cache, table, n, out=q.float())),
+            ("shape of q", lambda: paged(q, cache, table, n, out=torch.empty(2, 1, 7, 128, dtype=q.dtype, device=q.device))),
+            ("requires a gradient", lambda: paged(q.detach().clone().requires_grad_(), cache, table, n)),
+            ("start on 16 bytes", lambda: paged(odd, cache, table, n)),
+            ("multiple of kv_heads", lambda: prompt(x[:, :7], k, k, cu)),
+            ("multiple of kv_heads", lambda: prompt(x, torch.zeros(2, 3, 128, dtype=q.dtype, device=q.device), torch.zeros(2, 3, 128, dtype=q.dtype, device=q.device), cu)),
+            ("head_dim must be", lambda: prompt(x[..., :4], k[..., :4], k[..., :4], cu)),
+            ("k must be", lambda: prompt(x, k.half(), k, cu)),
+            ("do not fit", lambda: prompt(x, k, k[:1], cu)),
+            ("do not fit", lambda: prompt(x, k, k, cu, cu[:2])),
+            ("cu_q must be int32", lambda: prompt(x, k, k, cu.float())),
+            ("start on 16 bytes", lambda: prompt(odd[:, 0], k, k, cu)),
+            ("requires a gradient", lambda: prompt(x, k.clone().requires_grad_(), k, cu)),
+            ("do not fit the cache", lambda: append(x, x, cache, slots)),
+            ("do not fit the cache", lambda: append(k, k, cache, slots[:1])),
+            ("slots must be int32", lambda: append(k, k, cache, slots.long())),
+            ("k must be bfloat16", lambda: append(k.float(), k.float(), cache, slots)),
+            ("v must be", lambda: append(k, k.half(), cache, slots)),
+            ("requires a gradient", lambda: append(k.clone().requires_grad_(), k, cache, slots)),
+            ("free_blocks must be int32", lambda: plan(n, n, table, table, block_size=16, total_new=3)),
+            ("do not fit", lambda: plan(n, n[:1], table, n, block_size=16, total_new=3)),
+            ("negative size", lambda: plan(n, n, table, n, block_size=0, total_new=3)),
+            ("total_new is negative", lambda: plan(n, n, table, n, block_size=16, total_new=-1)),
+            ("too large", lambda: plan(n, n, table, n, block_size=16, total_new=2 ** 31)),
+            ("one element", lambda: plan(n, n, table, n, block_size=16, total_new=3, first_free=n))]:
+        with pytest.raises(_capi.VlaError, match=words):
+            call()

@@ -178,8 +178,10 @@ int vla_op_cache_append(const vla_cache_append_desc* d, void* stream) {
     p.n_slots = (long long)d->num_blocks * d->block_size;
     p.block_recip = d->block_size == 16 ? 0 : (uint32_t)(((1ull << 32) + d->block_size / 16 - 1) / (d->block_size / 16));
     const long long per_cta = APPEND_THREADS / 32, items = 2ll * d->kv_heads;
-    // As many warps as run at once (28 an SM), and no more: a warp whose window starts no run is launched for nothing
-    for (p.window = 1; p.window < APPEND_WINDOW && d->tokens / p.window * items > 28ll * sm_count();) p.window *= 2;
+    // As many warps as run at once, and no more: a warp whose window starts no run is launched for
+    // nothing.  16,000 tokens of a head of 256 take 4.6 us; with room for 28 warps an SM, which are not there, 6.3.
+    const long long at_once = (long long)append_ctas(d->head_dim) * per_cta * sm_count();
+    for (p.window = 1; p.window < APPEND_WINDOW && d->tokens / p.window * items > at_once;) p.window *= 2;
     const long long jobs = ((long long)d->tokens + p.window - 1) / p.window * items;
     if (jobs > INT_TOP) return refuse(VLA_ERR_LIMIT, "%s: too many tokens and heads", who);
     const dim3 grid((unsigned)((jobs + per_cta - 1) / per_cta));

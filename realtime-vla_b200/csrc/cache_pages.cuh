@@ -285,6 +285,7 @@ __device__ __forceinline__ float block_scale(float amax) {
 }
 
 constexpr int APPEND_THREADS = 128;
+constexpr int append_ctas(int head_dim) { return head_dim == 256 ? 4 : 7; }      // on an SM at once
 constexpr int APPEND_WINDOW = 16;        // token rows a warp looks for runs in, when there are many
 
 // One warp writes the runs (the consecutive token rows of one block) that start in its window of token rows, for one head,
@@ -299,7 +300,7 @@ constexpr int APPEND_WINDOW = 16;        // token rows a warp looks for runs in,
 // Measured (8 heads of 128, keys and values): 64 new tokens 3.2 us; 16k tokens of prompts 22 us, 4.4 TB/s of what must be
 // read and written; 32k tokens of heads of 256 70 us, 5.7 TB/s.
 template <typename T, int D>
-__global__ void __launch_bounds__(APPEND_THREADS, D == 256 ? 4 : 7) cache_append_kernel(const __grid_constant__ AppendParams p) {
+__global__ void __launch_bounds__(APPEND_THREADS, append_ctas(D)) cache_append_kernel(const __grid_constant__ AppendParams p) {
   constexpr int LPR = D / 8;              // lanes per row: 8 elements (16 bytes) each
   constexpr int RPI = 32 / LPR;           // rows per warp instruction
   constexpr int N = 16 / RPI;             // registers of 16 bytes for 16 rows

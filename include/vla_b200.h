@@ -281,7 +281,7 @@ int vla_op_norm(const float* x, void* y, int rows, int D, int mode, const float*
  * k_scale / v_scale [num_blocks][kv_heads]; a value is code * scale.  block_table [n_seqs][width] (row stride
  * table_stride, int32) names each sequence's pages in order.  A step of a serving loop is: vla_op_block_plan (pages and slots for
  * the new tokens), vla_op_cache_append (their keys and values), then vla_op_prompt_attention (new prompts among
- * themselves) or vla_op_paged_attention (the newest tokens over the whole cache).
+ * themselves, which sees no cache) or vla_op_paged_attention (the newest tokens over the whole cache).
  *
  * These calls only enqueue work on `stream` (asynchronous, no allocation, nothing kept from one call to the next), on the
  * current device, which must be the one the pointers belong to; they may be captured into a graph and issued from several

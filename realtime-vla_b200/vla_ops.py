@@ -176,13 +176,13 @@ def paged_attention(q, cache, block_table, seq_lens, *, scale=None, out=None):
     """Attention of the newest tokens of every sequence over the cache.
 
     q bf16 or fp16 [n, tokens, heads, head_dim]: the last tokens of each sequence, whose keys are in the cache already;
-    each sees itself and what is before it.  block_table int32 [n, width], seq_lens int32 [n].  scale: head_dim ** -0.5
+    each sees itself and what is before it.  Fewer new tokens than that: they stand at the end of the row.  block_table int32 [n, width], seq_lens int32 [n].  scale: head_dim ** -0.5
     unless given.  Returns out (which may be q), or a new tensor like q; a row that sees nothing is zero."""
     return _native.paged_attention(q, cache, block_table, seq_lens, scale, out)
 
 
 def prompt_attention(q, k, v, cu_q, cu_k=None, *, causal=True, scale=None, out=None):
-    """Attention over packed prompts of different lengths.
+    """Attention over packed prompts of different lengths.  It sees k and v alone: tokens behind a cached context take paged_attention.
 
     q bf16 or fp16 [tokens, heads, head_dim], k and v [keys, kv_heads, head_dim]; sequence b owns rows cu_q[b] .. cu_q[b + 1] of
     q and cu_k[b] .. cu_k[b + 1] of k and v (int32 [n + 1] on the device, ascending; cu_k: as cu_q unless given).  causal: the last row

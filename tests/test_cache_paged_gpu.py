@@ -312,3 +312,36 @@ def test_each_refusal_says_why():
             ("one element", lambda: plan(n, n, table, n, block_size=16, total_new=3, first_free=n))]:
         with pytest.raises(_capi.VlaError, match=words):
             call()
+
+
+# ---- a second turn ------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("heads,kv,dim", [(8, 1, 256), (8, 2, 128)])
+def test_second_turn_of_different_lengths(heads, kv, dim):
+    """Prompts, then further tokens behind them, a different number for each sequence: plan, append, and attention over the cache with
+    the queries of each sequence at the end of its row, as the documentation lays it out.  Every token sees its sequence's cache
+    up to itself."""
+    import vla_ops
+    g = torch.Generator(device=dev()).manual_seed(63)
+    first, then, block = (40, 1, 129, 17), (5, 33, 0, 12), 16
+    cache = vla_ops.kv_cache(40, kv, block, dim)
+    table = torch.full((4, 12), -1, dtype=torch.int32, device="cuda")
+    free = torch.randperm(40, generator=g, device="cuda").to(torch.int32)
+    lens, taken = torch.zeros(4, dtype=torch.int32, device="cuda"), None
+    for turn in (first, then):
+        new = torch.tensor(turn, dtype=torch.int32, device="cuda")
+        q = torch.randn(sum(turn), heads, dim, generator=g, device="cuda").bfloat16()
+        k, v = torch.randn(2, sum(turn), kv, dim, generator=g, device="cuda").bfloat16().unbind(0)
+        plan = vla_ops.block_plan(lens, new, table, free, block_size=block, total_new=sum(turn), first_free=taken)
+        vla_ops.cache_append(k, v, cache, plan.slots)
+        lens, taken = plan.seq_lens, plan.counts[:1]
+    most = max(then)
+    row = plan.cu_new[1:, None] - most + torch.arange(most, device="cuda")                  # [sequences, most]; negative: padding
+    out = vla_ops.paged_attention(q[row.clamp_min(0)], cache, table, plan.seq_lens)
+    out = out[torch.arange(most, device="cuda") >= most - new[:, None]]                     # [sum of new tokens, heads, dim]
+    assert out.shape == q.shape and plan.seq_lens.tolist() == [a + b for a, b in zip(first, then)]
+    cu = plan.cu_new.tolist()
+    for b in range(4):
+        if then[b]:
+            one = slice(b, b + 1)
+            check(q[None, cu[b]:cu[b + 1]], cache, table[one], plan.seq_lens[one], out[None, cu[b]:cu[b + 1]])

@@ -15,6 +15,7 @@
 // Roles: warp 0 = tile lookup and TMA producer, warp 1 = MMA issuer and TMEM owner, warps 2..5 = softmax and epilogue.
 // All mbarrier waits are bounded.
 #pragma once
+#include <type_traits>
 #include "cache_pages.cuh"
 
 struct PromptAttnParams {
@@ -94,33 +95,10 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return d;
 }
 
-template <typename T>
-struct Half16;   // what differs between the two 16-bit types
-template <>
-struct Half16<bf16> {
-  static constexpr uint32_t MMA_TYPE = 1u;
-  static constexpr uint32_t EXP_LO = 0x7f80u;
-  static __device__ __forceinline__ uint32_t pack(float a, float b) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-  static __device__ __forceinline__ float value(uint32_t bits) { return __uint_as_float(bits << 16); }
-};
-template <>
-struct Half16<__half> {
-  static constexpr uint32_t MMA_TYPE = 0u;
-  static constexpr uint32_t EXP_LO = 0x7c00u;
-  static __device__ __forceinline__ uint32_t pack(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-  static __device__ __forceinline__ float value(uint32_t bits) { return __half2float(__ushort_as_half((unsigned short)bits)); }
-};
-
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(PromptCfg<WIDE>::THREADS, WIDE ? 1 : 2) prompt_attention_kernel(const __grid_constant__ PromptAttnParams p) {
   using C = PromptCfg<WIDE>;
-  using H = Half16<T>;
+  constexpr uint32_t EXP = Bits16<T>::EXP;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t pad = (1024u - (raw_addr & 1023u)) & 1023u;
@@ -259,7 +237,8 @@ __global__ void __launch_bounds__(PromptCfg<WIDE>::THREADS, WIDE ? 1 : 2) prompt
     __syncwarp();
   } else if (warp == 1) {
     if (lane == 0 && n_chunks > 0) {
-      const uint32_t idesc = (1u << 4) | (H::MMA_TYPE << 7) | (H::MMA_TYPE << 10) | (8u << 24);
+      constexpr uint32_t TYPE = std::is_same<T, bf16>::value ? 1u : 0u;      // both operands bf16, or both fp16
+      const uint32_t idesc = (1u << 4) | (TYPE << 7) | (TYPE << 10) | (8u << 24);
       const int k_steps = (p.dim + 15) / 16;
       const uint32_t idesc_o = idesc | (1u << 16) | ((uint32_t)(k_steps * 2) << 17);      // N = head dim, B MN-major
       bool ok = mbar_wait_small(q_full, 0, abort_flag);
@@ -398,7 +377,7 @@ __global__ void __launch_bounds__(PromptCfg<WIDE>::THREADS, WIDE ? 1 : 2) prompt
           e.x = ex2_approx(e.x);
           e.y = ex2_approx(e.y);
           sum[j >> 1 & 1] = add2(sum[j >> 1 & 1], e);
-          w[j >> 1] = H::pack(e.x, e.y);
+          w[j >> 1] = pack2<T>(e.x, e.y);
         }
         tmem_st32(ts + 32 * g, w);
       }
@@ -425,12 +404,12 @@ __global__ void __launch_bounds__(PromptCfg<WIDE>::THREADS, WIDE ? 1 : 2) prompt
             uint4* const w4 = reinterpret_cast<uint4*>(column + (j < C::V_ROWS ? s0 : s1) * C::SLOT_BYTES + j % C::V_ROWS * 128);
             uint4 w = *w4;
             // the exponents inverted: a half whose bits were all ones is zero, and taking one from it sets its top bit
-            auto bad = [](uint32_t b) { return ((~b & H::EXP_LO * 0x10001u) - 0x10001u) & 0x80008000u; };
+            auto bad = [](uint32_t b) { return ((~b & EXP * 0x10001u) - 0x10001u) & 0x80008000u; };
             if (j >= tail) {
               *w4 = make_uint4(0u, 0u, 0u, 0u);
             } else if (bad(w.x) | bad(w.y) | bad(w.z) | bad(w.w)) {
               auto clean = [](uint32_t b) {
-                return ((b & H::EXP_LO) == H::EXP_LO ? 0u : b & 0xffffu) | ((b >> 16 & H::EXP_LO) == H::EXP_LO ? 0u : b & 0xffff0000u);
+                return ((b & EXP) == EXP ? 0u : b & 0xffffu) | ((b >> 16 & EXP) == EXP ? 0u : b & 0xffff0000u);
               };
               *w4 = make_uint4(clean(w.x), clean(w.y), clean(w.z), clean(w.w));
               *poison = 1;
@@ -471,14 +450,14 @@ __global__ void __launch_bounds__(PromptCfg<WIDE>::THREADS, WIDE ? 1 : 2) prompt
             const unsigned short* vr = reinterpret_cast<const unsigned short*>(p.v) + (long long)(k0 + key) * p.v_tok + kvh * p.v_head + d;
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-              if (d + j < p.dim && (vr[j] & H::EXP_LO) == H::EXP_LO) f[j] += H::value(vr[j]);
+              if (d + j < p.dim && (vr[j] & EXP) == EXP) f[j] += Bits16<T>::value(vr[j]);
           }
           __syncwarp();
         }
 #pragma unroll
         for (int j = 0; j < 32; j += 8)
           *reinterpret_cast<uint4*>(smem_raw + pad + ((d + j) >> 6) * C::Q_BOX + r * 128 + ((((d + j) >> 3 & 7) ^ (r & 7)) << 4)) =
-              make_uint4(H::pack(f[j], f[j + 1]), H::pack(f[j + 2], f[j + 3]), H::pack(f[j + 4], f[j + 5]), H::pack(f[j + 6], f[j + 7]));
+              make_uint4(pack2<T>(f[j], f[j + 1]), pack2<T>(f[j + 2], f[j + 3]), pack2<T>(f[j + 4], f[j + 5]), pack2<T>(f[j + 6], f[j + 7]));
       }
       __syncwarp();
       constexpr int LANES = C::BOXES * 8;        // per row, 16 bytes each

@@ -359,7 +359,7 @@ typedef struct vla_prompt_attn_desc {
 int vla_op_prompt_attention(const vla_prompt_attn_desc* d, void* stream);
 
 /* Status word of the calls above on the current device: bit 0 = a bounded wait inside a kernel ran out (none does unless something is
- * wrong), and the output of a call since the last look is not to be trusted; where it is known to be incomplete it is NaN.  Waits for all work on the device, on every stream,
+ * wrong), and the output of a call since the last look is not to be trusted; rows that are known to be incomplete are NaN.  Waits for all work on the device, on every stream,
  * returns the word and clears it.  Not while a stream is captured. */
 int vla_op_cache_status(int* out);
 /* Enqueues a wait that nothing ends, for limit_us microseconds (1 to 1000000), which then raises bit 0 as the waits of the calls above

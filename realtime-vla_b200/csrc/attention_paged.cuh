@@ -279,11 +279,11 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
   __shared__ int again_mem;                         // this tile has a further P V: apart
   __shared__ int found_b, found_base, warp_sum[PAGED_THREADS / 32];
   // of the 8 groups of a tile, written and handed back with its V: scale of K, whether there is a page, scale of V, and highest and lowest
-  // level of the scales of V in the tile (two 16-bit numbers)
+  // level of the scales of V in this tile and up to three beside it (two 16-bit numbers)
   __shared__ float4 page_info[C::SLOTS / 2][8];
   __shared__ float q_scale[2][R];
-  // each softmax warp's copy of the scale of Q and the maximum of each row, the same for all its lanes; with two CTAs an SM they are
-  // kept there only
+  // each softmax warp's copy of the scale of Q and the maximum of each row, the same for all its lanes: with two CTAs an SM they are
+  // kept there only, with one they are put there for `apart`
   constexpr bool KEPT = C::PER_SM == 2;
   __shared__ float4 row_mem[4][2][R / 4];
   // as well: what O of the part at hand is relative to, O = sum 2^(s - m + 7) s_v / 2^x; the levels from which, y, and up to which, w, x may
@@ -437,14 +437,9 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
           if (kv == 1) {                        // the scales may come in later than the loads go out
             const bool on = now.id >= 0, finite = on && fabsf(now.vs) < INFINITY;
             const float vs = finite ? now.vs : 0.f;
-            if (j == 0) {                       // of every tile of the batch
-              int hi = vs != 0.f ? scale_level(vs) : PAGED_NONE, lo = vs != 0.f ? hi : -PAGED_NONE;
-#pragma unroll
-              for (int o = 1; o < 8; o <<= 1) {
-                hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-                lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-              }
-              levels = hi << 16 | (lo & 0xffff);
+            if (j == 0) {                       // over the batch, which is quicker than each tile's own and does as well
+              const int level = scale_level(vs), hi = __reduce_max_sync(0xffffffffu, vs != 0.f ? level : PAGED_NONE);
+              levels = hi << 16 | (__reduce_min_sync(0xffffffffu, vs != 0.f ? level : -PAGED_NONE) & 0xffff);
             }
             // a scale of V that is not finite makes the tokens' scores NaN, and so every row that sees one
             if (here) page_info[c % HALF][g] = make_float4(!on ? 0.f : finite ? now.ks : NAN, on ? 1.f : 0.f, vs, __int_as_float(levels));
@@ -844,8 +839,10 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
             m[r] = -INFINITY;
             l[r] = 0.f;
           }
-          to_mem(0, qs);
-          to_mem(1, m);
+          if (KEPT) {
+            to_mem(0, qs);
+            to_mem(1, m);
+          }
           __syncwarp();
           if (lane == 0) mbar_arrive(q_empty(seg % C::Q_BUFS));
         }
@@ -897,7 +894,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
             m[r] = top;
             l[r] *= a[r];
           }
-          to_mem(1, m);
+          if (KEPT) to_mem(1, m);
           if (tile > w.t0) {
 #pragma unroll 1
             for (int y = 0; y < C::HALVES; ++y) {
@@ -920,6 +917,10 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
         if (__builtin_expect(hi > lv.x || lo < lv.y, 0) && !follow(c, hi, lo, tile == w.t0)) {
 #pragma unroll
           for (int r = 0; r < R; ++r) l[r] += ex2_approx(x[r] - (m[r] == -INFINITY ? 0.f : m[r]) + 7.f);
+          if (!KEPT) {
+            to_mem(0, qs);
+            to_mem(1, m);
+          }
           apart(c, tok, w.len, lim_min, g0, tile == w.t0, moved);
           continue;
         }
@@ -954,7 +955,8 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
         }
 #pragma unroll
         for (int bit = 16 / R; bit > 0; bit >>= 1) l[0] += __shfl_xor_sync(0xffffffffu, l[0], bit);
-        if (lane % (32 / R) == 0) reinterpret_cast<float*>(&warp_sums[seg & 1][lane / (32 / R)])[quarter] = l[0];
+        // a quarter of the sum: see `at`; NaN where a wait has run out
+        if (lane % (32 / R) == 0) reinterpret_cast<float*>(&warp_sums[seg & 1][lane / (32 / R)])[quarter] = *abort_flag ? NAN : l[0] * 0.25f;
       }
       const bool more = take(w_next);            // while the last P V runs
       if (seg >= 0) {
@@ -980,7 +982,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
           }
           const int d = y * 128 + tid;
           if (d >= D) break;
-          uint32_t nans = *abort_flag ? ~0u : 0u;  // rows that see a NaN in this head dim, or that a wait left incomplete
+          uint32_t nans = *abort_flag ? ~0u : 0u;  // rows that see a NaN in this head dim, or that the last wait left incomplete
           if (bad) {
 #pragma unroll 1
             for (int tok = max(lim_min, w.t0 * 128); tok < min(w.len, w.t1 * 128); ++tok) {
@@ -992,7 +994,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
             }
           }
           const int n_rows = min(R, p.rows - r0);
-          const float at = power_of_2(level_mem[quarter].x - 2);  // 2^128 is not a number
+          const float at = power_of_2(level_mem[quarter].x - 2);  // 2^x / 4, because x may be 128
 #pragma unroll
           for (int r = 0; r < R; ++r)
             if (nans >> r & 1) val[r] = NAN;
@@ -1003,7 +1005,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
             for (int r = 0; r < R; ++r) {
               const float4 sums = warp_sums[seg & 1][r];
               const float sum = (sums.x + sums.y) + (sums.z + sums.w);
-              if (r < n_rows) *dst = (T)(sum == 0.f && !(nans >> r & 1) ? 0.f : val[r] * rcp_approx(sum) * at * 4.f);       // 0: nothing seen
+              if (r < n_rows) *dst = (T)(sum == 0.f ? 0.f : val[r] * (rcp_approx(sum) * at));       // 0: nothing seen
               --left;
               dst += left ? p.o_head : turn;
               left = left ? left : p.group;
@@ -1016,8 +1018,8 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
             for (int r = 0; r < R; ++r) {
               const float4 sums = warp_sums[seg & 1][r];
               const float sum = (sums.x + sums.y) + (sums.z + sums.w);
-              if (r < n_rows) part[r * D] = sum == 0.f && !(nans >> r & 1) ? 0.f : val[r] * rcp_approx(sum) * at * 4.f;
-              if (d == r) part_ml[r] = make_float2(m[r], sum * 0x1p-40f);      // the join's products with it stay finite
+              if (r < n_rows) part[r * D] = sum == 0.f ? 0.f : val[r] * (rcp_approx(sum) * at);
+              if (d == r) part_ml[r] = make_float2(m[r], sum * 0x1p-38f);      // the join's products with it stay finite
             }
           }
         }

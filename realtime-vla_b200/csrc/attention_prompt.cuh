@@ -427,7 +427,8 @@ __global__ void __launch_bounds__(PromptCfg<WIDE>::THREADS, WIDE ? 1 : 2) prompt
       ok = __all_sync(0xffffffffu, mbar_wait_small(o_done((n_chunks - 1) & 1), (uint32_t)((n_chunks - 1) >> 1) & 1u, abort_flag));
       tc_fence_after();
     }
-    if (ok && seq >= 0) {
+    if (!ok) l = NAN;                            // a wait ran out: no row is left as it was
+    if (seq >= 0) {
       const float inv = l != 0.f ? 1.f / l : 0.f;         // nothing seen: O is zero or was never written
       const bool any_poison = *poison != 0;
       const long long row_at = (long long)(q0 + tok) * p.o_tok + (long long)(kvh * p.group + r % p.group) * p.o_head;
@@ -471,10 +472,6 @@ __global__ void __launch_bounds__(PromptCfg<WIDE>::THREADS, WIDE ? 1 : 2) prompt
           *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.o) + at + piece * 8) =
               *reinterpret_cast<const uint4*>(from + rr * 128 + (((piece & 7) ^ (rr & 7)) << 4));
       }
-    } else if (row_ok) {                         // a wait ran out: no row is left as it was
-      T* const row = reinterpret_cast<T*>(p.o) + (long long)(q0 + tok) * p.o_tok + (long long)(kvh * p.group + r % p.group) * p.o_head;
-#pragma unroll 1
-      for (int d = 0; d < p.dim; ++d) row[d] = (T)NAN;
     }
   }
 

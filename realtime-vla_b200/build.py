@@ -41,7 +41,11 @@ def _has_torch():
 
 def _made_for():
     """What the binding is linked against: it loads with no other torch or Python."""
-    return "torch %s in %s, %s" % (metadata.version("torch"), _torch_home(), sys.implementation.cache_tag)
+    try:
+        version = metadata.version("torch")
+    except metadata.PackageNotFoundError:      # a torch that runs from its source tree
+        version = "unknown"
+    return "torch %s in %s, %s" % (version, _torch_home(), sys.implementation.cache_tag)
 
 
 def _torch_home():

@@ -23,8 +23,8 @@
 // Roles, all walking the same piece on their own: warp 0 pages and TMA, warp 1 MMA, warp 2 Q pieces of the next unit, warps
 // 3..6 softmax, one token (and, at a unit's end, one head dim) per thread.  All mbarrier waits are bounded.  Code that
 // runs once per unit is kept in loops: run straight through, it costs about 8 clocks an instruction to fetch.
-// Measured: 64 sequences of 64 to 8192 tokens, 32 heads on 8 of 128, 46.6 us, 4.7 TB/s of codes and scales; 4 of 90001 to 131071, 8
-// heads on 1 of 256, 50.7 us, 4.6 TB/s; one of 809 tokens 8.7 us.
+// Measured: 64 sequences of 64 to 8192 tokens, 32 heads on 8 of 128, 48.3 us, 4.5 TB/s of codes and scales; 4 of 90001 to 131071, 8
+// heads on 1 of 256, 51.8 us, 4.5 TB/s; one of 809 tokens 9.4 us.
 #pragma once
 #include "cache_pages.cuh"
 
@@ -55,11 +55,17 @@ struct PagedAttnParams {
 };
 
 constexpr int PAGED_THREADS = 224;
-// Fixed cost of a unit, in groups of 16 tokens.  Measured: 64 sequences of 64 to 8192, heads of 128, with 8, 12, 16, 20: 51.1, 46.6,
-// 46.9, 48.0 us; 83 sequences of 217 to 10009, 3 tokens each, heads of 256: 60.8, 58.2, 54.1, 52.6.
+// Fixed cost of a unit, in groups of 16 tokens.  Measured with 8, 12, 16, 20: 200 sequences of 100 to 1500 tokens, 32 heads on 8 of 128,
+// 85.8, 82.3, 81.1, 81.1 us; the same with 16 heads on 4 of 64, 43.2, 41.0, 40.5, 41.3; 64 of 64 to 8192 of these, 56.5, 57.0, 57.0, 57.9.
+// Heads of 256 with 12, 16, 20, 24: 83 sequences of 217 to 10009, 3 tokens each, 102.1, 102.0, 102.0, 103.7.
 constexpr int paged_gap(int head_dim) { return head_dim == 256 ? 20 : 12; }
-constexpr int PAGED_MIN_PIECE = 8;       // groups (with gaps) per CTA, at least
-constexpr int PAGED_WHOLE = 32;          // units of at most this many groups are not cut
+// Groups (with gaps) per CTA, at least.  With less a piece could hold no tile's start, which the join counts on.  With 8, 16, 32: one
+// sequence of 809 tokens, heads of 256, 9.3, 10.6, 13.5 us; 16 of 100 to 4001, 13.9, 13.4, 15.9; of 700 to 900, heads of 64, 12.0, 12.0, 13.8.
+constexpr int PAGED_MIN_PIECE = 8;
+// Units of at most this many groups are not cut, which spares the join.  512 tokens (32 groups) uncut and cut: 300 sequences of 300, 32 heads
+// on 8 of 128, 60.0 and 74.7 us, 64 of 512 20.1 and 23.0, but one of 512 9.4 and 8.9, and with 8 heads on 1 of 256 12.5 and 9.2.  1024 tokens:
+// 64 sequences 31.8 and 33.1, 8 of them 23.8 and 12.2, one of 256 head dims 19.5 and 9.5.
+constexpr int PAGED_WHOLE = 32;
 
 // Scales of V with one reference 2^L: 2^(L - PAGED_SPAN - 1) < s_v <= 2^L, so that the last piece of P ends 2^-18 below the largest
 // probability at the most, and 2^-25 below it where all scales are alike.
@@ -571,7 +577,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
       }
       if (seg >= C::Q_BUFS && !__all_sync(0xffffffffu, paged_wait(q_empty(qb), (uint32_t)(seg / C::Q_BUFS - 1) & 1u, abort_flag))) break;
       // Two rows at a time: a row is a chain of some 450 clocks, and short sequences wait for them.  3 sequences of 69 to 276, 5
-      // tokens each of 64 heads on 8, take 15.1 us instead of 16.3; four at a time 14.9, but more where there are 8 rows.
+      // tokens each of 64 heads on 8, took 1.2 us less than with one; four at a time 0.2 less again, but more where there are 8 rows.
 #pragma unroll 1
       for (int r = 0; r < R; r += 2) {
         float2 f[2][E];
@@ -638,8 +644,8 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
     };
     Part w, w_next;
     w.t0 = w.t1 = 0;
-    // m and qs are kept there and read where they are needed: in 128 registers a thread they were spilled, and 9 sequences of
-    // 2940 to 16102, 8 tokens each of 28 heads on 4 of 128, took 86 us instead of 72 (64 next tokens of 64 to 8192: 48.3, 46.6).
+    // m and qs are kept there and read where they are needed: in 128 registers a thread more is spilled than the 56 to 80 bytes that
+    // 16 rows still cost, and 9 sequences of 2940 to 16102, 8 tokens each of 28 heads on 4 of 128, take 84 us instead of 72.
     auto from_mem = [&](int what, float (&v)[R]) {
       if constexpr (KEPT) {
 #pragma unroll
@@ -701,8 +707,8 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
     // level is known to fit, and the next tile comes here as well.  The number of P V is odd, with an empty one if need be, so
     // that the phases of the barriers stay those of one a tile.  Rare, so that it is kept in loops that need few registers: S is read
     // again row by row (as a function of its own, with the call in the loop over tiles, all other tiles took half as long again).
-    // 64 sequences of 64 to 8192 tokens, 32 heads on 8 of 128: 49 us with scales within 2^5, 270 with a scale of its own out of 2^9 for
-    // each page, 465 out of 2^60; 4 of 90001 to 131071, 8 heads on 1 of 256: 51, 133 and 255.
+    // 64 sequences of 64 to 8192 tokens, 32 heads on 8 of 128: 49 us with scales within 2^5, 272 with a scale of its own out of 2^9 for
+    // each page, 467 out of 2^60; 4 of 90001 to 131071, 8 heads on 1 of 256: 52, 168 and 255.
     auto apart = [&](int c, int tok, int len, int lim_min, int g0, bool first, bool moved) {
       const float4* const infos = page_info[c % HALF];
       int4* const lv = &level_mem[quarter];
@@ -1048,6 +1054,8 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
 
 // Joins the parts of the units that were cut, each with its share of the unit's sum: block (c, y) does two or four rows of the unit that starts in piece c.  A row's
 // parts are dealt out to groups of D / 4 threads, which take four head dims each; the groups' sums are then added in order.
+// Half and twice the rows a block: heads of 256, 4 sequences of 90001 to 131071, 46.2 and 52.9 us (48.4 so), 16 of 3000 to 9000 with 2
+// tokens each, 25.9 and 26.0 (25.2); heads of 64, 16 of 100 to 4001 with 4 tokens each, 18.7 and 17.5 (17.1); of 128, 51.2, 53.5 (51.9).
 constexpr int PAGED_JOIN_THREADS = 512;
 template <int D>
 constexpr int PAGED_JOIN_ROWS = D == 256 ? 2 : 4;

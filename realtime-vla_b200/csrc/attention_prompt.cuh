@@ -10,7 +10,8 @@
 //     P             = exp2(S scale - m)   one thread per row, straight from TMEM, written back over S as 16-bit pairs
 //     O[128 x dim] += P . V_chunk         tcgen05.mma, A = P in TMEM, B = V as it lies in memory (MN-major), so V needs
 //                                         neither a transposed copy nor a pass through registers
-// The maximum m a row subtracts is only moved when it grows by more than 2^8 (probabilities then stay below 2^8, sums in
+// P is rounded to the operands' type, because P V takes both of one type; a row's sum is of the unrounded ones, which costs half a step
+// of the type on each probability and no more.  The maximum m a row subtracts is only moved when it grows by more than 2^8 (probabilities then stay below 2^8, sums in
 // fp32), so that O in TMEM is rescaled a few times per tile instead of once per chunk.
 // Roles: warp 0 = tile lookup and TMA producer, warp 1 = MMA issuer and TMEM owner, warps 2..5 = softmax and epilogue.
 // All mbarrier waits are bounded.
@@ -39,8 +40,8 @@ struct PromptAttnParams {
 // share its tensor core and its exponentials; wider heads need the whole SM, with chunks of 128 keys whose K and V come in
 // halves of 32 KB.
 // What bounds it: an MMA of 128 rows and 16 steps of K takes about 85 clocks for N = 64 as for N = 128 and 125 for N = 256, so
-// S of 64 keys costs as much as S of 128.  Measured: one causal prompt of 8192, 32 heads on 8 of 128, 475 us, 1.15 PFLOP/s; 48
-// ragged prompts of the same heads 134 us.  With chunks of 128 keys there is TMEM for one S buffer a CTA only: 674 and
+// S of 64 keys costs as much as S of 128.  Measured: one causal prompt of 8192, 32 heads on 8 of 128, 482 to 500 us, 1.1 PFLOP/s (566 in
+// a long row of calls, when the clock falls); 48 ragged prompts of the same heads 134 us (146).  With chunks of 128 keys there is TMEM for one S buffer a CTA only: 674 and
 // 198 us.  32 prompts of 276 to 968, 8 heads on 1 of 256, 138 us, 0.72 PFLOP/s: there the loads before a tile's first MMA and
 // the stores behind its last, 11,600 of 25,600 clocks, run under nothing.
 template <bool WIDE>

@@ -1,6 +1,6 @@
 // Python binding of the operators around a key/value cache in pages (vla_ops.py documents them): checks of the tensors,
-// outputs and workspaces from torch's allocator, the current stream, then the C entry point.  These calls take three to ten
-// microseconds on the GPU; here the host needs 5 to 9 for each, of which the launch is 3, and through ctypes it needed 11 to 19.
+// outputs and workspaces from torch's allocator, the current stream, then the C entry point.  The smallest calls take three to ten
+// microseconds on the GPU; here the host needs 5 to 10 for each, of which the launch is 3, and through ctypes it needed 11 to 19.
 #include <ATen/ATen.h>
 #include <ATen/core/LegacyTypeDispatch.h>
 #include <c10/core/AutogradState.h>

@@ -148,7 +148,7 @@ int vla_op_block_plan(const vla_block_plan_desc* d, void* stream) {
     if (smem > 40 * 1024)
       if (cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(block_plan_kernel), (2 * PLAN_MAX_SEQS + 2) * (int)sizeof(int)); e != cudaSuccess)
         return launched(who, e);
-    // one row a thread, or a CTA on each SM: with four rows a thread 140k rows of 512 prompts take 6.4 us instead of 5.0
+    // one row a thread, or a CTA on each SM: with four rows a thread 140k rows of 512 requests take 6.2 us instead of 5.2
     const int ctas = std::min((std::max(std::max(d->total_new, d->n_seqs), 1) - 1) / PLAN_THREADS + 1, sm_count());
     return launched(who, launch_ex(block_plan_kernel, dim3(ctas), dim3(PLAN_THREADS), smem, reinterpret_cast<cudaStream_t>(stream), 1, true, p));
   });
@@ -179,7 +179,7 @@ int vla_op_cache_append(const vla_cache_append_desc* d, void* stream) {
     p.block_recip = d->block_size == 16 ? 0 : (uint32_t)(((1ull << 32) + d->block_size / 16 - 1) / (d->block_size / 16));
     const long long per_cta = APPEND_THREADS / 32, items = 2ll * d->kv_heads;
     // As many warps as run at once, and no more: a warp whose window starts no run is launched for
-    // nothing.  16,000 tokens of a head of 256 take 4.6 us; with room for 28 warps an SM, which are not there, 6.3.
+    // nothing.  16,000 tokens of a head of 256 take 4.6 us; with room for 28 warps an SM, of which 16 are there, 6.3.
     const long long at_once = (long long)append_ctas(d->head_dim) * per_cta * sm_count();
     for (p.window = 1; p.window < APPEND_WINDOW && d->tokens / p.window * items > at_once;) p.window *= 2;
     const long long jobs = ((long long)d->tokens + p.window - 1) / p.window * items;

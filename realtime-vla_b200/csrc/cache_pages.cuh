@@ -82,7 +82,7 @@ __device__ __forceinline__ long long plan_scan(long long x, int lane) {
 // kernel to do it, keeps them in shared memory and then writes its share of the tokens and of the new table entries.
 // A few dependent steps on little data: what counts is how much code they run through once (some 8 clocks an instruction
 // until it is in the caches), so loops stay loops and there is no division.
-// Measured: 256 requests with a new token each 4.8 us (25 KB of code took 6.5), 140k rows of 512 prompts 5.5 us.
+// Measured: 256 requests with a new token each 4.8 us (25 KB of code took 6.5), 512 requests with 1 to 2048 new tokens 5.5 us.
 __global__ void __launch_bounds__(PLAN_THREADS) block_plan_kernel(const __grid_constant__ PlanParams p) {
   extern __shared__ int plan_smem[];
   int* cu = plan_smem;                   // [n_seqs + 1] first token row of each request
@@ -295,10 +295,11 @@ constexpr int APPEND_WINDOW = 16;        // token rows a warp looks for runs in,
 // Bound by memory where there are many tokens, and two trips to memory long where there are few: the slots of a window and
 // the row before it come in one load (a lane each), then 16 rows of a run, all in flight, with the block's scale; they stay
 // in registers between the maximum and the rounding.  Only runs of more than 16 tokens are read twice.  The window is as
-// wide as leaves a warp for every place on the GPU: 4096 rows of 8 heads of 64 take 13.7 us with windows of one row and
-// 4.0 us with 16, one new token in each of 256 sequences 2.6 us either way.
-// Measured (8 heads of 128, keys and values): 64 new tokens 3.2 us; 16k tokens of prompts 22 us, 4.4 TB/s of what must be
-// read and written; 32k tokens of heads of 256 70 us, 5.7 TB/s.
+// wide as leaves a warp for every place on the GPU: 4096 rows of 8 heads of 64 take 18.3 us with windows of one row and
+// 3.1 us with 16, one new token in each of 256 sequences 4.3 us either way.
+// Measured (8 heads of 128, keys and values): 64 new tokens 2.9 us; 24 prompts of 40 to 2048 tokens 21.9 us, 4.5 TB/s of what must be
+// read and written; 32k tokens of heads of 256 67 us, 5.8 TB/s.  What the prompts wait for is memory (long scoreboard 4.7 of 11
+// stalls an issue, issue slots 42% active): a warp loads nothing while it rounds.
 template <typename T, int D>
 __global__ void __launch_bounds__(APPEND_THREADS, append_ctas(D)) cache_append_kernel(const __grid_constant__ AppendParams p) {
   constexpr int LPR = D / 8;              // lanes per row: 8 elements (16 bytes) each

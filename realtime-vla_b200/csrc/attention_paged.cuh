@@ -23,8 +23,8 @@
 // Roles, all walking the same piece on their own: warp 0 pages and TMA, warp 1 MMA, warp 2 Q pieces of the next unit, warps
 // 3..6 softmax, one token (and, at a unit's end, one head dim) per thread.  All mbarrier waits are bounded.  Code that
 // runs once per unit is kept in loops: run straight through, it costs about 8 clocks an instruction to fetch.
-// Measured: 64 sequences of 64 to 8192 tokens, 32 heads on 8 of 128, 48.3 us, 4.5 TB/s of codes and scales; 4 of 90001 to 131071, 8
-// heads on 1 of 256, 51.8 us, 4.5 TB/s; one of 809 tokens 9.4 us.
+// Measured: 64 sequences of 64 to 8192 tokens, 32 heads on 8 of 128, 49.5 us, 4.4 TB/s of codes and scales; 4 of 90001 to 131071, 8
+// heads on 1 of 256, 51.8 us, 4.5 TB/s; one of 809 tokens 9.5 us.
 #pragma once
 #include "cache_pages.cuh"
 
@@ -295,6 +295,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
   // as well: what O of the part at hand is relative to, O = sum 2^(s - m + 7) s_v / 2^x; the levels from which, y, and up to which, w, x may
   // follow the scales without a look at the scores; the highest level so far, z
   __shared__ int4 level_mem[4];
+  __shared__ int late_mem[4];                       // a wait for a tile's scales has run out, here or in another warp
   __shared__ float4 warp_max[R], warp_sums[2][R];   // by row, of the four softmax warps (sums: of odd and even units)
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t pad = (1024u - (raw_addr & 1023u)) & 1023u;
@@ -330,7 +331,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
     }
     mbar_init(p_ready, 128);
     mbar_init(o_done, 1);
-    abort_mem = again_mem = 0;
+    abort_mem = again_mem = late_mem[0] = late_mem[1] = late_mem[2] = late_mem[3] = 0;
     poison_mem[0] = poison_mem[1] = poison_mem[2] = 0;
     mbar_fence_init();
     tma_prefetch_desc(&p.tmK);
@@ -624,7 +625,8 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
     }
   } else {
     // ---- softmax: thread = token of the tile; at a unit's end, thread = head dim.  A wait that runs out raises the abort
-    // flag and the loop goes on with whatever is there, because the 128 threads meet at barriers. ----
+    // flag and the loop goes on with whatever is there, because the 128 threads meet at barriers; what decides which barriers those are
+    // is the same in all of them: the walk, and the pages' scales, once nobody's wait for them has run out. ----
     const int quarter = warp & 3, tid = quarter * 32 + lane;
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     auto wait = [&](uint32_t bar, uint32_t parity) {
@@ -707,8 +709,8 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
     // level is known to fit, and the next tile comes here as well.  The number of P V is odd, with an empty one if need be, so
     // that the phases of the barriers stay those of one a tile.  Rare, so that it is kept in loops that need few registers: S is read
     // again row by row (as a function of its own, with the call in the loop over tiles, all other tiles took half as long again).
-    // 64 sequences of 64 to 8192 tokens, 32 heads on 8 of 128: 49 us with scales within 2^5, 272 with a scale of its own out of 2^9 for
-    // each page, 467 out of 2^60; 4 of 90001 to 131071, 8 heads on 1 of 256: 52, 168 and 255.
+    // 64 sequences of 64 to 8192 tokens, 32 heads on 8 of 128: 50 us with scales within 2^5, 272 with a scale of its own out of 2^9 for
+    // each page, 466 out of 2^60; 4 of 90001 to 131071, 8 heads on 1 of 256: 52, 171 and 256.
     auto apart = [&](int c, int tok, int len, int lim_min, int g0, bool first, bool moved) {
       const float4* const infos = page_info[c % HALF];
       int4* const lv = &level_mem[quarter];
@@ -809,7 +811,8 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
 #pragma unroll 1
       for (int tile = w.t0; tile < w.t1; ++tile, ++c) {
         const int s = 2 * (c % HALF), tok = tile * 128 + tid;
-        wait(full(s + 1), (uint32_t)(c / HALF) & 1u);
+        const bool late = !paged_wait(full(s + 1), (uint32_t)(c / HALF) & 1u, abort_flag);
+        __syncwarp();
         const float4 info = page_info[c % HALF][tid >> 4];
         const bool edge = tile * 128 + 128 > lim_min;
         if (edge || !__all_sync(0xffffffffu, info.y != 0.f)) {
@@ -835,6 +838,14 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
           }
           __syncwarp();
         }
+        if (tile == w.t0) {                      // a part begins with the level of its first tile, if there is one for all of it
+          const int hi = __float_as_int(info.w) >> 16, lo = (int)(short)__float_as_int(info.w), at = max(hi, -100);
+          if (lane == 0) level_mem[quarter] = make_int4(at, hi - lo <= PAGED_SPAN ? at - PAGED_SPAN : -PAGED_NONE, at, at + PAGED_SPAN);
+          __syncwarp();
+        }
+        const int2 lv = *reinterpret_cast<const int2*>(&level_mem[quarter]);
+        // the same in all threads, unless a wait for the scales has run out, of which all know by the barrier below: they have to go one way
+        const bool out = __float_as_int(info.w) >> 16 > lv.x || (int)(short)__float_as_int(info.w) < lv.y;
         wait(s_full(c & 1), (uint32_t)(c >> 1) & 1u);
         tc_fence_after();
         if (tile == w.t0) {
@@ -872,12 +883,8 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
             }
           }
         }
-        if (tile == w.t0 && lane == 0) {         // a part begins with the level of its first tile, if there is one for all of it
-          const int hi = __float_as_int(info.w) >> 16, lo = (int)(short)__float_as_int(info.w), at = max(hi, -100);
-          level_mem[quarter] = make_int4(at, hi - lo <= PAGED_SPAN ? at - PAGED_SPAN : -PAGED_NONE, at, at + PAGED_SPAN);
-        }
         from_mem(1, m);
-        bool grow = false, moved = false;
+        bool grow = late, moved = false;
 #pragma unroll
         for (int r = 0; r < R; ++r) grow |= x[r] > m[r] + 1.f;
         // The subtracted maximum moves when a token has outgrown it by more than 2: P stays below 2 * 2^7, in e4m3's range.
@@ -890,7 +897,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
           }
           if (tile > w.t0) wait(o_done, (uint32_t)(c - 1) & 1u);
           tc_fence_after();
-          named_barrier_sync(1, 128);
+          if (barrier_any(1, late)) late_mem[quarter] = 1;
           float a[R];
 #pragma unroll
           for (int r = 0; r < R; ++r) {
@@ -916,22 +923,22 @@ __global__ void __launch_bounds__(PAGED_THREADS, (PagedCfg<D, NT>::PER_SM)) page
           }
         }
         from_mem(1, m);
-        // read again instead of kept, and the levels as well: registers are short here
-        const float2 scale = *reinterpret_cast<const float2*>(&page_info[c % HALF][tid >> 4].z);
-        const int2 lv = *reinterpret_cast<const int2*>(&level_mem[quarter]);
-        const int hi = __float_as_int(scale.y) >> 16, lo = (int)(short)__float_as_int(scale.y);       // the same in all threads
-        if (__builtin_expect(hi > lv.x || lo < lv.y, 0) && !follow(c, hi, lo, tile == w.t0)) {
+        if (__builtin_expect(out, 0)) {
+          const int levels = __float_as_int(page_info[c % HALF][tid >> 4].w);
+          if (!late_mem[quarter] && !follow(c, levels >> 16, (int)(short)levels, tile == w.t0)) {
 #pragma unroll
-          for (int r = 0; r < R; ++r) l[r] += ex2_approx(x[r] - (m[r] == -INFINITY ? 0.f : m[r]) + 7.f);
-          if (!KEPT) {
-            to_mem(0, qs);
-            to_mem(1, m);
+            for (int r = 0; r < R; ++r) l[r] += ex2_approx(x[r] - (m[r] == -INFINITY ? 0.f : m[r]) + 7.f);
+            if (!KEPT) {
+              to_mem(0, qs);
+              to_mem(1, m);
+            }
+            apart(c, tok, w.len, lim_min, g0, tile == w.t0, moved);
+            continue;
           }
-          apart(c, tok, w.len, lim_min, g0, tile == w.t0, moved);
-          continue;
         }
+        // read again instead of kept: registers are short here
+        const float f = below_level(page_info[c % HALF][tid >> 4].z, level_mem[quarter].x);
         if (c > 0) wait(o_done, (uint32_t)(c - 1) & 1u);   // P of the tile before has been read
-        const float f = below_level(scale.x, level_mem[quarter].x);
 #pragma unroll
         for (int r = 0; r < R; r += 2) {
           float e[2];

@@ -324,9 +324,10 @@ int vla_op_cache_append(const vla_cache_append_desc* d, void* stream);
 
 /* O = softmax(scale Q K^T) V of the last n_q tokens of every sequence over the cache: q, o [n_seqs][n_q][heads][head_dim] by
  * strides; query i of sequence b is token seq_lens[b] - n_q + i and sees itself and what is before it (a row before the
- * sequence's start is zero).  Page ids outside the cache are not seen; seq_lens is cut to width * block_size.  A probability is
- * held to 2^-12 of itself, and of a row's largest to 2^-25 where the pages' v_scale are alike, 2^-18 (and more slowly
- * from 2^7 on) where they differ by up to 2^80; what lies further below a row's largest v_scale may be lost.
+ * sequence's start is zero).  Page ids outside the cache are not seen; seq_lens is cut to width * block_size.
+ * An element of q is held to 2^-12 of itself and 2^-25 of its row's largest; a probability to 2^-12 of itself and, of its row's
+ * largest, 2^-25 where the pages' v_scale are alike, 2^-18 where they differ by up to 2^80 (which takes several times as long from
+ * 2^7 on).  What lies further below the largest v_scale that a row sees may be lost.
  * heads is a multiple of kv_heads (consecutive query heads share a key/value head); head_dim 64 | 128 | 256. */
 typedef struct vla_paged_attn_desc {
   const void* q; void* o;
@@ -359,8 +360,9 @@ typedef struct vla_prompt_attn_desc {
 int vla_op_prompt_attention(const vla_prompt_attn_desc* d, void* stream);
 
 /* Status word of the calls above on the current device: bit 0 = a bounded wait inside a kernel ran out (none does unless something is
- * wrong), and the output of a call since the last look is not to be trusted; rows that are known to be incomplete are NaN.  Waits for all work on the device, on every stream,
- * returns the word and clears it.  Not while a stream is captured. */
+ * wrong), and the output of a call since the last look is not to be trusted; rows that are
+ * known to be incomplete are NaN.  Waits for all work on the device, on every stream, returns the word and clears it.  Not while
+ * a stream is captured. */
 int vla_op_cache_status(int* out);
 /* Enqueues a wait that nothing ends, for limit_us microseconds (1 to 1000000), which then raises bit 0 as the waits of the calls above
  * do: for programs and tests to see that they notice. */

@@ -6,7 +6,7 @@
 // from TMA straight into tcgen05.mma (kind f8f6f4), so no thread ever touches one; what the threads do is the softmax of
 // 8 or 16 numbers per token.  For that, the other operand has to be e4m3 as well, without losing what bf16 or fp16
 // hold: Q and P are each split into three e4m3 numbers, x = x0 + x1 / 16 + x2 / 256, each the rounding of what is left
-// (4 bits a piece, 12 bits in all).  The pieces are further columns of the MMA's N side, which costs nothing that counts:
+// (4 bits a piece, 12 bits in all, down to 2^-25 of the row's largest element).  The pieces are further columns of the MMA's N side, which costs nothing that counts:
 //     S[128 tokens x 3R]      = K_tile . (Q0 Q1 Q2)^T       A = K tile, K-major;    R = 8 NT rows
 //     O[128 head dims x 3R]  += V_tile^T . (P0 P1 P2)       A = V tile, MN-major: as the page lies in memory
 // The page's scale of K multiplies S.  That of V multiplies P: P = 2^(s - m + 7) s_v / 2^L, with m the running maximum of s and

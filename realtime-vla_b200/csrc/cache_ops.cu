@@ -178,8 +178,8 @@ int vla_op_cache_append(const vla_cache_append_desc* d, void* stream) {
     p.n_slots = (long long)d->num_blocks * d->block_size;
     p.block_recip = d->block_size == 16 ? 0 : (uint32_t)(((1ull << 32) + d->block_size / 16 - 1) / (d->block_size / 16));
     const long long per_cta = APPEND_THREADS / 32, items = 2ll * d->kv_heads;
-    // As many warps as run at once, and no more: a warp whose window starts no run is launched for
-    // nothing.  16,000 tokens of a head of 256 take 4.6 us; with room for 28 warps an SM, of which 16 are there, 6.3.
+    // As many warps as run at once, and no more: a warp whose window starts no run is launched for nothing.  16,000 tokens of a head
+    // of 256 take 4.6 us; with room for 28 warps an SM, of which 16 are there, 6.3.
     const long long at_once = (long long)append_ctas(d->head_dim) * per_cta * sm_count();
     for (p.window = 1; p.window < APPEND_WINDOW && d->tokens / p.window * items > at_once;) p.window *= 2;
     const long long jobs = ((long long)d->tokens + p.window - 1) / p.window * items;
